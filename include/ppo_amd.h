@@ -527,6 +527,78 @@ int ppo_clip_adam_step(int n_tensors, float *const *params, float *const *exp_av
                        double max_grad_norm, double lr, double beta1, double beta2, double eps,
                        long step, void *stream);
 
+/* ---- token policies: wide action heads, masked sequences, linear layers ------------------------------------------
+ * The entry points below have no counterpart in the reference, whose agents act with small heads on flat minibatches;
+ * they stand beside ppo_loss_fwd_bwd, ppo_loss_logits_fwd_bwd and ppo_linear_wgrad and keep their conventions. */
+#define PPO_DTYPE_F32 0
+#define PPO_DTYPE_BF16 1
+#define PPO_DTYPE_F16 2
+
+/*
+ * log p(action) and entropy of the categorical distribution softmax(logits / temperature), one row a token:
+ * Categorical(logits).log_prob / .entropy (src/ppo.py:186-189, :212-214) for any number of actions.
+ *   logits   [batch, length, num_actions] of `dtype`, actions contiguous, strides in elements (>= 0) of the other two axes;
+ *            -inf marks an illegal action
+ *   actions  [batch * length] i32 or i64 (action_bytes 4 / 8).  ignore_index: the row is not read, its outputs and its
+ *            gradient are 0.  Any other value outside [0, num_actions): the row's outputs and gradient are NaN.
+ *   logp     [batch * length] f32; entropy the same or NULL; stats [batch * length, 2] f32 {max logit, ln sum} for the
+ *            backward call.  A row without a legal action: logp -inf, entropy 0.  NaN or +inf in a row: NaN.
+ *   temperature in [1e-6, 1e6].
+ * ppo_token_logprobs_bwd: g_logits [batch * length, num_actions] of `dtype`, contiguous, = the gradient of
+ * sum g_logp logp + g_entropy entropy (either may be NULL, not both; entropy may be NULL without g_entropy); 0 in rows that
+ * are ignored or have no legal action.  g_logits must not overlap any input.
+ */
+int ppo_token_logprobs_fwd(const void *logits, int dtype, long batch, long length, long num_actions, long batch_stride,
+                           long token_stride, const void *actions, int action_bytes, double temperature, long ignore_index,
+                           float *logp, float *entropy, float *stats, void *stream);
+int ppo_token_logprobs_bwd(const void *logits, int dtype, long batch, long length, long num_actions, long batch_stride,
+                           long token_stride, const void *actions, int action_bytes, const float *stats, const float *entropy,
+                           const float *g_logp, const float *g_entropy, double temperature, long ignore_index, void *g_logits,
+                           void *stream);
+
+/*
+ * Clipped policy loss with a KL term over padded sequences, and its gradient with respect to log_probs: the surrogate of
+ * src/ppo.py:502-508 per token.  With d = log_probs - old_log_probs, r = e^d, e = log_probs - ref_log_probs:
+ *   l = -min(r A, clip(r, 1 - clip_low, 1 + clip_high) A) + kl_coef k(e)
+ *   PPO_KL_K1: k = e;  PPO_KL_K2: k = e^2 / 2;  PPO_KL_K3: k = e^-e - 1 + e
+ *   out6 = {mean l, mean surrogate term, mean k, share of r outside the clip range, mean r - 1 - ln r, unmasked tokens}
+ * sequence_mean 0: means over the unmasked tokens; 1: over the sequences that have one, of their tokens' means.  No token
+ * unmasked: 0.  mask [batch, length] u8 (0 = masked) or NULL; what masked tokens hold is not used, their gradient is 0.
+ * advantages [batch, length], or with per_sequence [batch] (adv_stride apart).  ref_log_probs may be NULL (no KL term).
+ * Every array has rows of its own stride (elements, >= 0) and contiguous tokens; g_log_probs [batch, length] contiguous or
+ * NULL.  clip_low in [0, 1), clip_high >= 0.  Workspace: ppo_policy_kl_loss_workspace_bytes(batch), 8-byte aligned.
+ */
+#define PPO_KL_K1 1
+#define PPO_KL_K2 2
+#define PPO_KL_K3 3
+size_t ppo_policy_kl_loss_workspace_bytes(long batch);
+int ppo_policy_kl_loss(const float *log_probs, long lp_stride, const float *old_log_probs, long old_stride, const float *advantages,
+                       long adv_stride, int per_sequence, const float *ref_log_probs, long ref_stride, const uint8_t *mask,
+                       long mask_stride, long batch, long length, double clip_low, double clip_high, double kl_coef, int kl_kind,
+                       int sequence_mean, float *out6, float *g_log_probs, void *workspace, size_t workspace_bytes, void *stream);
+
+/*
+ * Preference loss on paired log ratios, and its gradients with respect to the token log-probs.  Per pair, over the
+ * unmasked tokens, D = sum(chosen - ref_chosen) - sum(rejected - ref_rejected) (means instead of sums with `average`; a
+ * sequence without tokens counts 0), z = beta D:
+ *   PPO_PREF_SIGMOID: -(1 - label_smoothing) ln s(z) - label_smoothing ln s(-z);  PPO_PREF_HINGE: max(0, 1 - z);
+ *   PPO_PREF_IPO: (D - 1 / (2 beta))^2
+ *   out2 = {mean loss, share of pairs with z > 0};  rewards [pairs, 2] = beta times the two sums (means)
+ * The two sides have lengths and row strides (elements, >= 0) of their own; ref_* and mask_* may be NULL; g_chosen
+ * [pairs, chosen_length] and g_rejected contiguous, or NULL.  Workspace: ppo_preference_loss_workspace_bytes(...), 8-byte
+ * aligned.
+ */
+#define PPO_PREF_SIGMOID 0
+#define PPO_PREF_HINGE 1
+#define PPO_PREF_IPO 2
+size_t ppo_preference_loss_workspace_bytes(long pairs, long chosen_length, long rejected_length);
+int ppo_preference_loss(const float *chosen, long chosen_stride, const float *ref_chosen, long ref_chosen_stride,
+                        const uint8_t *mask_chosen, long mask_chosen_stride, long chosen_length, const float *rejected,
+                        long rejected_stride, const float *ref_rejected, long ref_rejected_stride, const uint8_t *mask_rejected,
+                        long mask_rejected_stride, long rejected_length, long pairs, int kind, double beta, double label_smoothing,
+                        int average, float *out2, float *rewards, float *g_chosen, float *g_rejected, void *workspace,
+                        size_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

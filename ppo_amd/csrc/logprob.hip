@@ -1,0 +1,385 @@
+// Log-probabilities and entropy of actions under a wide categorical head, forward and backward -- gfx950.
+//
+// The front end that loss.hip's ppo_loss_logits_fwd_bwd has for 2 .. 8 actions (Categorical(logits).log_prob / .entropy,
+// reference src/ppo.py:186-189, :212-214), for any number of actions, rows of tokens and 16-bit logits.  With
+// z = logits / temperature of one row, top = max z, s = sum e^(z - top), u = sum e^(z - top) (z - top):
+//     log p_a = z_a - top - ln s          H = -sum p ln p = ln s - u / s
+//     d log p_a / d z_k = [k = a] - p_k   d H / d z_k = -p_k (ln p_k + H)
+// One pass over the logits forward (running maximum; s and u are rescaled when it moves), one pass backward that reads
+// the logits again and writes their gradient.  Both are bound by HBM.  What is kept per row for the backward pass is the
+// PAIR {max logit, ln s}: their sum, the usual log-sum-exp, loses ln s in rows of large magnitude (a row of the type's
+// lowest value is a uniform one), and (logit - max) is exact where the two are near.
+// All sums are f32 over chunks of at most 32 elements, then over the lanes' chunks, then over lanes: 131072 terms are
+// off by a few 1e-7.
+#include "token_common.h"
+
+using namespace ppo_token;
+
+namespace {
+
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+constexpr float LOWEST = -1e30f;   // stands for -inf as the factor of a weight that is 0 (0 * -inf would be NaN)
+
+struct Row {
+    float m, s, u;   // max of the raw logits; sum 2^t; sum t 2^t with t = (x - m) * c, c = log2(e) / temperature
+};
+
+__device__ __forceinline__ Row row_none() { return Row{-INFINITY, 0.0f, 0.0f}; }
+
+// (m, s, u) seen from the maximum m2 >= m
+__device__ __forceinline__ void row_move(Row &r, float m2, float c)
+{
+    const float base = m2 == -INFINITY ? 0.0f : m2;
+    const float t = (r.m - base) * c;                  // -inf for an empty part: s and u are 0 then
+    const float f = __builtin_amdgcn_exp2f(t);
+    r.u = (r.u + r.s * fmaxf(t, LOWEST)) * f;
+    r.s *= f;
+    r.m = m2;
+}
+
+__device__ __forceinline__ Row row_join(Row a, Row b, float c)
+{
+    const float m = fmaxf(a.m, b.m);
+    row_move(a, m, c);
+    row_move(b, m, c);
+    return Row{m, a.s + b.s, a.u + b.u};
+}
+
+template <int N> __device__ __forceinline__ void row_add(Row &r, const float (&x)[N], float c)
+{
+    float m = r.m;
+#pragma unroll
+    for (int i = 0; i < N; ++i) m = fmaxf(m, x[i]);
+    if (m > r.m) row_move(r, m, c);
+    const float base = r.m == -INFINITY ? 0.0f : r.m;
+    float s = 0.0f, u = 0.0f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const float t = (x[i] - base) * c;
+        const float e = __builtin_amdgcn_exp2f(t);     // NaN stays in s
+        s += e;
+        u += e * fmaxf(t, LOWEST);
+    }
+    r.s += s;
+    r.u += u;
+}
+
+template <int G> __device__ __forceinline__ Row row_lanes(Row r, float c)
+{
+#pragma unroll
+    for (int off = G / 2; off > 0; off >>= 1) {
+        const Row o = {__shfl_xor(r.m, off, 64), __shfl_xor(r.s, off, 64), __shfl_xor(r.u, off, 64)};
+        r = row_join(r, o, c);
+    }
+    return r;
+}
+
+struct FwdArgs {
+    const void *logits, *actions;
+    float *logp, *entropy, *stats;
+    long rows, length, A, batch_stride, token_stride, ignore;
+    float c, inv_t;
+    int action_bytes;
+};
+
+__device__ __forceinline__ long action_of(const void *actions, int bytes, long row)
+{
+    return bytes == 8 ? reinterpret_cast<const long *>(actions)[row] : (long)reinterpret_cast<const int *>(actions)[row];
+}
+
+__device__ __forceinline__ long row_offset(long row, long rows, long length, long batch_stride, long token_stride)
+{
+    if (length == rows) return row * token_stride;     // one batch, or evenly spaced ones (even_rows)
+    const long b = row / length;
+    return b * batch_stride + (row - b * length) * token_stride;
+}
+
+__device__ __forceinline__ void write_ignored(const FwdArgs &a, long row)
+{
+    a.logp[row] = 0.0f;
+    if (a.entropy) a.entropy[row] = 0.0f;
+    a.stats[2 * row] = 0.0f;
+    a.stats[2 * row + 1] = 0.0f;
+}
+
+template <class T> __device__ __forceinline__ void write_row(const FwdArgs &a, long row, const typename T::raw *x, long act, Row r)
+{
+    float logp, H, lns;
+    if (act < 0 || act >= a.A) {                       // no such action: the row's outputs and gradients are NaN
+        logp = H = lns = __builtin_nanf("");
+    } else if (r.m == -INFINITY && r.s == 0.0f) {      // no legal action in the row
+        logp = -INFINITY;
+        H = lns = 0.0f;
+    } else {
+        lns = logf(r.s);
+        H = lns - LN2 * (r.u / r.s);
+        logp = (T::load(x[act]) - r.m) * a.inv_t - lns;
+    }
+    a.logp[row] = logp;
+    if (a.entropy) a.entropy[row] = H;
+    a.stats[2 * row] = r.m;
+    a.stats[2 * row + 1] = lns;
+}
+
+// G lanes a row, one element a lane and turn: rows of a few dozen actions
+template <class T, int G> __global__ void __launch_bounds__(256) k_logprobs_short(FwdArgs a)
+{
+    const long row = (long)blockIdx.x * (256 / G) + threadIdx.x / G;
+    const int l = threadIdx.x % G;
+    if (row >= a.rows) return;
+    const long act = action_of(a.actions, a.action_bytes, row);
+    if (act == a.ignore) {
+        if (l == 0) write_ignored(a, row);
+        return;
+    }
+    const typename T::raw *x = reinterpret_cast<const typename T::raw *>(a.logits) + row_offset(row, a.rows, a.length, a.batch_stride, a.token_stride);
+    Row r = row_none();
+    for (long k = l; k < a.A; k += 4 * G) {
+        float v[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = k + i * G < a.A ? T::load(x[k + i * G]) : -INFINITY;
+        row_add<4>(r, v, a.c);
+    }
+    r = row_lanes<G>(r, a.c);
+    if (l == 0) write_row<T>(a, row, x, act, r);
+}
+
+// a workgroup of THREADS (a wave, 256 or 1024 threads) a row, 16-byte loads
+template <class T, int THREADS> __global__ void __launch_bounds__(THREADS < 256 ? 256 : THREADS) k_logprobs_long(FwdArgs a)
+{
+    constexpr int E = 16 / T::BYTES, CHUNK = 32, U = CHUNK / E;
+    const long row = THREADS == 64 ? (long)blockIdx.x * 4 + threadIdx.x / 64 : (long)blockIdx.x;
+    const int tid = THREADS == 64 ? threadIdx.x % 64 : threadIdx.x;
+    if (row >= a.rows) return;
+    const long act = action_of(a.actions, a.action_bytes, row);
+    if (act == a.ignore) {
+        if (tid == 0) write_ignored(a, row);
+        return;
+    }
+    const typename T::raw *x = reinterpret_cast<const typename T::raw *>(a.logits) + row_offset(row, a.rows, a.length, a.batch_stride, a.token_stride);
+    Row r = row_none();
+    long at = 0;
+    for (; at + (long)THREADS * CHUNK <= a.A; at += (long)THREADS * CHUNK) {
+        float v[CHUNK];
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+            float w[E];
+            load16<T>(x + at + ((long)i * THREADS + tid) * E, w);
+#pragma unroll
+            for (int j = 0; j < E; ++j) v[i * E + j] = w[j];
+        }
+        row_add<CHUNK>(r, v, a.c);
+    }
+    for (; at + tid * E < a.A; at += (long)THREADS * E) {
+        const long k = at + tid * E;
+        float w[E];
+        if (k + E <= a.A) {
+            load16<T>(x + k, w);
+        } else {
+#pragma unroll
+            for (int j = 0; j < E; ++j) w[j] = k + j < a.A ? T::load(x[k + j]) : -INFINITY;
+        }
+        row_add<E>(r, w, a.c);
+    }
+    r = row_lanes<64>(r, a.c);
+    if constexpr (THREADS > 64) {
+        __shared__ Row part[THREADS / 64];
+        if ((tid & 63) == 0) part[tid >> 6] = r;
+        __syncthreads();
+        if (tid < 64) {
+            r = tid < THREADS / 64 ? part[tid] : row_none();
+            r = row_lanes<THREADS / 64>(r, a.c);
+        }
+    }
+    if (tid == 0) write_row<T>(a, row, x, act, r);
+}
+
+struct BwdArgs {
+    const void *logits, *actions;
+    const float *stats, *entropy, *g_logp, *g_entropy;
+    void *g;
+    long rows, length, A, batch_stride, token_stride, ignore;
+    float c, inv_t;
+    int action_bytes;
+};
+
+// d loss / d logit_k = -p_k (ga + gb log2 p_k) + [k = a] gl
+struct Grad {
+    float base, lns2, ga, gb, gl;
+    long act;
+    bool live;
+};
+
+__device__ __forceinline__ Grad grad_of(const BwdArgs &a, long row)
+{
+    Grad g;
+    g.act = action_of(a.actions, a.action_bytes, row);
+    g.live = g.act != a.ignore;
+    g.base = g.lns2 = g.ga = g.gb = g.gl = 0.0f;
+    if (!g.live) return g;
+    const float m = a.stats[2 * row], lns = a.stats[2 * row + 1];
+    if (m == -INFINITY && lns == 0.0f) {               // no legal action: no gradient
+        g.live = false;
+        return g;
+    }
+    const float glp = a.g_logp ? a.g_logp[row] : 0.0f, gh = a.g_entropy ? a.g_entropy[row] : 0.0f;
+    const float H = a.g_entropy ? a.entropy[row] : 0.0f;
+    g.base = m;
+    g.lns2 = lns * LOG2E;
+    g.gl = glp * a.inv_t;
+    g.ga = g.gl + gh * H * a.inv_t;
+    g.gb = gh * LN2 * a.inv_t;
+    return g;
+}
+
+__device__ __forceinline__ float grad_at(const Grad &g, float x, float c)
+{
+    const float t = (x - g.base) * c - g.lns2;         // log2 p
+    const float p = __builtin_amdgcn_exp2f(t);
+    return -p * (g.ga + g.gb * fmaxf(t, LOWEST));
+}
+
+template <class T, int G> __global__ void __launch_bounds__(256) k_logprobs_bwd_short(BwdArgs a)
+{
+    const long row = (long)blockIdx.x * (256 / G) + threadIdx.x / G;
+    const int l = threadIdx.x % G;
+    if (row >= a.rows) return;
+    const Grad g = grad_of(a, row);
+    const typename T::raw *x = reinterpret_cast<const typename T::raw *>(a.logits) + row_offset(row, a.rows, a.length, a.batch_stride, a.token_stride);
+    typename T::raw *o = reinterpret_cast<typename T::raw *>(a.g) + row * a.A;
+    for (long k = l; k < a.A; k += G) {
+        float v = 0.0f;
+        if (g.live) v = grad_at(g, T::load(x[k]), a.c) + (k == g.act ? g.gl : 0.0f);
+        o[k] = T::store(v);
+    }
+}
+
+// (row, chunk of 256 * 32 elements) a workgroup
+template <class T> __global__ void __launch_bounds__(256) k_logprobs_bwd_long(BwdArgs a, int chunks)
+{
+    constexpr int E = 16 / T::BYTES, CHUNK = 32, U = CHUNK / E;
+    const long row = blockIdx.x / chunks;
+    const long at = (long)(blockIdx.x % chunks) * (256 * CHUNK);
+    const Grad g = grad_of(a, row);
+    const typename T::raw *x = reinterpret_cast<const typename T::raw *>(a.logits) + row_offset(row, a.rows, a.length, a.batch_stride, a.token_stride);
+    typename T::raw *o = reinterpret_cast<typename T::raw *>(a.g) + row * a.A;
+    const bool whole = at + 256 * CHUNK <= a.A;
+    float w[U][E];
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+        const long k = at + ((long)i * 256 + threadIdx.x) * E;
+        if (g.live && (whole || k + E <= a.A)) {
+            load16<T>(x + k, w[i]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < E; ++j) w[i][j] = g.live && k + j < a.A ? T::load(x[k + j]) : 0.0f;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+        const long k = at + ((long)i * 256 + threadIdx.x) * E;
+#pragma unroll
+        for (int j = 0; j < E; ++j) w[i][j] = g.live ? grad_at(g, w[i][j], a.c) : 0.0f;
+        if (g.live && g.act >= k && g.act < k + E) {
+#pragma unroll
+            for (int j = 0; j < E; ++j) w[i][j] += k + j == g.act ? g.gl : 0.0f;
+        }
+        if (whole || k + E <= a.A) {
+            store16<T>(o + k, w[i]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < E; ++j)
+                if (k + j < a.A) o[k + j] = T::store(w[i][j]);
+        }
+    }
+}
+
+bool logits_ok(const void *logits, int dtype, long batch, long length, long A, long batch_stride, long token_stride,
+               const void *actions, int action_bytes, double temperature)
+{
+    if (!dtype_known(dtype) || batch < 1 || length < 1 || A < 1 || (action_bytes != 4 && action_bytes != 8)) return false;
+    if (!logits || !actions || !ppo_aligned(logits, dtype_bytes(dtype)) || !ppo_aligned(actions, action_bytes)) return false;
+    if (!(temperature > 0.0) || !(temperature <= 1e6) || !(temperature >= 1e-6)) return false;
+    // the largest index of any element stays far from 2^63, the number of workgroups below 2^31
+    const long MOST = 1L << 40;
+    if (batch > MOST / length || A > MOST || batch * length > (1L << 31) - 1) return false;
+    if (batch_stride < 0 || token_stride < 0) return false;
+    return (__int128)(batch - 1) * batch_stride + (__int128)(length - 1) * token_stride + A < ((__int128)1 << 60);
+}
+
+// rows whose offsets are row * token_stride throughout need no division by length
+template <class Args> void even_rows(Args &a, long batch)
+{
+    if (batch == 1 || a.batch_stride == a.length * a.token_stride) a.length = a.rows;
+}
+
+}  // namespace
+
+extern "C" {
+
+int ppo_token_logprobs_fwd(const void *logits, int dtype, long batch, long length, long num_actions, long batch_stride,
+                           long token_stride, const void *actions, int action_bytes, double temperature, long ignore_index,
+                           float *logp, float *entropy, float *stats, void *stream)
+{
+    if (batch == 0 || length == 0) return 0;
+    PPO_REQUIRE(logits_ok(logits, dtype, batch, length, num_actions, batch_stride, token_stride, actions, action_bytes, temperature));
+    PPO_REQUIRE(logp && stats && ppo_aligned(logp, 4) && ppo_aligned(entropy, 4) && ppo_aligned(stats, 8));
+    FwdArgs a;
+    a.logits = logits; a.actions = actions; a.logp = logp; a.entropy = entropy; a.stats = stats;
+    a.rows = batch * length; a.length = length; a.A = num_actions; a.batch_stride = batch_stride; a.token_stride = token_stride;
+    a.ignore = ignore_index; a.action_bytes = action_bytes;
+    a.inv_t = (float)(1.0 / temperature);
+    a.c = (float)(1.4426950408889634 / temperature);
+    even_rows(a, batch);
+    hipStream_t s = (hipStream_t)stream;
+    return by_dtype(dtype, [&](auto t) {
+        using T = decltype(t);
+        const unsigned rows = (unsigned)a.rows;
+        if (a.A <= 32)
+            hipLaunchKernelGGL((k_logprobs_short<T, 8>), dim3((rows + 31) / 32), dim3(256), 0, s, a);
+        else if (a.A <= 256)
+            hipLaunchKernelGGL((k_logprobs_short<T, 64>), dim3((rows + 3) / 4), dim3(256), 0, s, a);
+        else if (a.A <= 4096)
+            hipLaunchKernelGGL((k_logprobs_long<T, 64>), dim3((rows + 3) / 4), dim3(256), 0, s, a);
+        else if (a.rows >= 1024)
+            hipLaunchKernelGGL((k_logprobs_long<T, 256>), dim3(rows), dim3(256), 0, s, a);
+        else
+            hipLaunchKernelGGL((k_logprobs_long<T, 1024>), dim3(rows), dim3(1024), 0, s, a);
+        return ppo_launch_status();
+    });
+}
+
+int ppo_token_logprobs_bwd(const void *logits, int dtype, long batch, long length, long num_actions, long batch_stride,
+                           long token_stride, const void *actions, int action_bytes, const float *stats, const float *entropy,
+                           const float *g_logp, const float *g_entropy, double temperature, long ignore_index, void *g_logits,
+                           void *stream)
+{
+    if (batch == 0 || length == 0) return 0;
+    PPO_REQUIRE(logits_ok(logits, dtype, batch, length, num_actions, batch_stride, token_stride, actions, action_bytes, temperature));
+    PPO_REQUIRE(stats && g_logits && (g_logp || g_entropy) && (!g_entropy || entropy));
+    PPO_REQUIRE(ppo_aligned(stats, 8) && ppo_aligned(g_logits, dtype_bytes(dtype)) && ppo_aligned(entropy, 4) && ppo_aligned(g_logp, 4) &&
+                ppo_aligned(g_entropy, 4));
+    BwdArgs a;
+    a.logits = logits; a.actions = actions; a.stats = stats; a.entropy = entropy; a.g_logp = g_logp; a.g_entropy = g_entropy;
+    a.g = g_logits; a.rows = batch * length; a.length = length; a.A = num_actions; a.batch_stride = batch_stride;
+    a.token_stride = token_stride; a.ignore = ignore_index; a.action_bytes = action_bytes;
+    a.inv_t = (float)(1.0 / temperature);
+    a.c = (float)(1.4426950408889634 / temperature);
+    even_rows(a, batch);
+    const long chunks = (a.A + 256 * 32 - 1) / (256 * 32);
+    PPO_REQUIRE(a.A <= 1024 || chunks <= ((1L << 31) - 1) / a.rows);
+    hipStream_t s = (hipStream_t)stream;
+    return by_dtype(dtype, [&](auto t) {
+        using T = decltype(t);
+        const unsigned rows = (unsigned)a.rows;
+        if (a.A <= 32)
+            hipLaunchKernelGGL((k_logprobs_bwd_short<T, 8>), dim3((rows + 31) / 32), dim3(256), 0, s, a);
+        else if (a.A <= 1024)
+            hipLaunchKernelGGL((k_logprobs_bwd_short<T, 64>), dim3((rows + 3) / 4), dim3(256), 0, s, a);
+        else
+            hipLaunchKernelGGL((k_logprobs_bwd_long<T>), dim3((unsigned)(a.rows * chunks)), dim3(256), 0, s, a, (int)chunks);
+        return ppo_launch_status();
+    });
+}
+
+}  // extern "C"

@@ -683,3 +683,255 @@ def clip_adam_step(opt, group: "GradGroup", max_grad_norm: float):
                                 float(g["eps"]), step, _stream())
     _lib.check(rc, "ppo_clip_adam_step")
     _note_inplace_update(params)
+
+
+# ---- token policies: wide action heads, losses over padded sequences (csrc/logprob.hip, seqloss.hip) ------------------
+_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}      # include/ppo_amd.h: PPO_DTYPE_*
+KL_KINDS = {"k1": 1, "k2": 2, "k3": 3}                                 # PPO_KL_*
+PREFERENCE_KINDS = {"sigmoid": 0, "hinge": 1, "ipo": 2}                # PPO_PREF_*
+
+
+def _need(cond, what: str):
+    if not cond:
+        raise _lib.PpoAmdError(what)
+
+
+def _on_tensor_device(fn):
+    """Launches go to the first tensor's device and that device's current stream."""
+    @functools.wraps(fn)
+    def call(first, *args, **kwargs):
+        _need(isinstance(first, torch.Tensor), f"{fn.__name__} takes tensors")
+        if first.is_cuda and first.get_device() != torch._C._cuda_getDevice():
+            with torch.cuda.device(first.device):
+                return fn(first, *args, **kwargs)
+        return fn(first, *args, **kwargs)
+    return call
+
+
+def _device_tensors(name: str, *tensors):
+    dev = tensors[0].device
+    _need(dev.type == "cuda", f"{name} needs HIP device tensors; there is no CPU fallback")
+    for t in tensors[1:]:
+        _need(t is None or t.device == dev, f"{name}: every tensor has to be on {dev}")
+
+
+def _token_rows(name, logits, actions, temperature):
+    """(logits with contiguous actions, actions, [batch, length, batch stride, token stride])"""
+    _need(logits.dtype in _DTYPES, f"{name}: logits are float32, bfloat16 or float16, not {logits.dtype}")
+    _need(logits.dim() >= 1 and logits.shape[-1] >= 1, f"{name}: logits are [..., actions] with at least one action")
+    _need(isinstance(actions, torch.Tensor) and actions.dtype in (torch.int32, torch.int64), f"{name}: actions are int32 or int64")
+    _need(actions.shape == logits.shape[:-1], f"{name}: actions {tuple(actions.shape)} for logits {tuple(logits.shape)}")
+    _need(1e-6 <= float(temperature) <= 1e6, f"{name}: temperature {temperature} outside [1e-6, 1e6]")
+    _device_tensors(name, logits, actions)
+    if logits.dim() > 3:
+        logits = logits.reshape(-1, *logits.shape[-2:])
+    if logits.shape[-1] > 1 and logits.stride(-1) != 1:
+        logits = logits.contiguous()
+    if logits.dim() == 3:
+        geometry = (logits.shape[0], logits.shape[1], logits.stride(0), logits.stride(1))
+    elif logits.dim() == 2:
+        geometry = (1, logits.shape[0], 0, logits.stride(0))
+    else:
+        geometry = (1, 1, 0, 0)
+    return logits, actions.contiguous(), geometry
+
+
+@_on_tensor_device
+def token_logprobs_fwd(logits, actions, temperature=1.0, ignore_index=-100, want_entropy=True):
+    """ppo_token_logprobs_fwd: (log p(action), entropy or None, stats) of softmax(logits / temperature), f32, shaped like
+    `actions`: what ppo_losses_discrete does inside for 2 .. 8 actions (reference src/ppo.py:186-189, :212-214), for any
+    number of them.  logits [..., actions] f32 / bf16 / f16: the actions contiguous (copied otherwise), the one or two
+    axes before them of any stride, so `logits[:, :-1]` is read in place.  -inf marks an illegal action; a token whose
+    action is ignore_index gives 0; a row without a legal action gives log p -inf and entropy 0; an action out of range
+    gives NaN.  stats [..., 2] is what token_logprobs_bwd needs."""
+    lib = _lib.load()
+    lg, act, (batch, length, bs, ts) = _token_rows("token_logprobs", logits, actions, temperature)
+    shape, dev = actions.shape, lg.device
+    logp = torch.empty(shape, dtype=torch.float32, device=dev)
+    entropy = torch.empty(shape, dtype=torch.float32, device=dev) if want_entropy else None
+    stats = torch.empty((*shape, 2), dtype=torch.float32, device=dev)
+    rc = lib.ppo_token_logprobs_fwd(lg.data_ptr(), _DTYPES[lg.dtype], batch, length, lg.shape[-1], bs, ts, act.data_ptr(),
+                                    act.element_size(), float(temperature), int(ignore_index), logp.data_ptr(), _ptr(entropy),
+                                    stats.data_ptr(), _stream())
+    _lib.check(rc, "ppo_token_logprobs_fwd")
+    return logp, entropy, stats
+
+
+@_on_tensor_device
+def token_logprobs_bwd(logits, actions, stats, entropy, g_logp, g_entropy=None, temperature=1.0, ignore_index=-100):
+    """ppo_token_logprobs_bwd: d (sum g_logp log p + sum g_entropy entropy) / d logits, contiguous, of the logits' dtype,
+    from the inputs and outputs of token_logprobs_fwd.  g_logp or g_entropy may be None."""
+    lib = _lib.load()
+    name = "token_logprobs_bwd"
+    lg, act, (batch, length, bs, ts) = _token_rows(name, logits, actions, temperature)
+    _need(g_logp is not None or g_entropy is not None, f"{name}: a gradient of log p or of the entropy is needed")
+    _need(g_entropy is None or entropy is not None, f"{name}: the entropy's gradient needs the entropy")
+    _need(stats.dtype == torch.float32 and stats.shape == (*actions.shape, 2) and stats.is_contiguous(), f"{name}: stats are those of the forward call")
+    rows = []
+    for t in (entropy, g_logp, g_entropy):
+        _need(t is None or (t.dtype == torch.float32 and t.shape == actions.shape), f"{name}: entropy and gradients are float32 of the actions' shape")
+        rows.append(None if t is None else t.contiguous())
+    _device_tensors(name, lg, stats, *rows)
+    g = torch.empty(logits.shape, dtype=lg.dtype, device=lg.device)
+    rc = lib.ppo_token_logprobs_bwd(lg.data_ptr(), _DTYPES[lg.dtype], batch, length, lg.shape[-1], bs, ts, act.data_ptr(),
+                                    act.element_size(), stats.data_ptr(), *[_ptr(t) for t in rows], float(temperature),
+                                    int(ignore_index), g.data_ptr(), _stream())
+    _lib.check(rc, "ppo_token_logprobs_bwd")
+    return g
+
+
+class _TokenLogprobs(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, actions, temperature, ignore_index):
+        logp, entropy, stats = token_logprobs_fwd(logits, actions, temperature, ignore_index)
+        ctx.save_for_backward(logits, actions, stats, entropy)
+        ctx.meta = (temperature, ignore_index)
+        ctx.set_materialize_grads(False)
+        return logp, entropy
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g_logp, g_entropy):
+        if g_logp is None and g_entropy is None:
+            return None, None, None, None
+        logits, actions, stats, entropy = ctx.saved_tensors
+        return token_logprobs_bwd(logits, actions, stats, entropy, g_logp, g_entropy, *ctx.meta), None, None, None
+
+
+def token_logprobs(logits, actions, temperature=1.0, ignore_index=-100):
+    """(log p(action), entropy) of token_logprobs_fwd, both differentiable with respect to the logits."""
+    if torch.is_grad_enabled() and logits.requires_grad:
+        return _TokenLogprobs.apply(logits, actions, float(temperature), int(ignore_index))
+    return token_logprobs_fwd(logits, actions, temperature, ignore_index)[:2]
+
+
+def _sequence_rows(name, what, t, shape, dtypes=(torch.float32,)):
+    """(tensor whose tokens are contiguous, its row stride); (None, 0) for None"""
+    if t is None:
+        return None, 0
+    _need(isinstance(t, torch.Tensor) and t.dtype in dtypes, f"{name}: {what} is {' or '.join(str(d) for d in dtypes)}")
+    _need(tuple(t.shape) == tuple(shape), f"{name}: {what} is {tuple(t.shape)}, not {tuple(shape)}")
+    if t.dim() == 2 and t.shape[1] > 1 and t.stride(1) != 1:
+        t = t.contiguous()
+    return t, t.stride(0)
+
+
+_MASK_TYPES = (torch.bool, torch.uint8)
+
+
+@_on_tensor_device
+def policy_kl_loss_fwd_bwd(new_lp, old_lp, adv, mask=None, ref_lp=None, clip_low=0.2, clip_high=0.2, kl_coef=0.0, kl="k3",
+                           reduction="token", want_grad=True):
+    """ppo_policy_kl_loss: the clipped surrogate (reference src/ppo.py:502-508) plus kl_coef times a KL estimate to a
+    reference policy, over [B, L] tokens.  Returns (out6, g_new_lp or None); out6 = device f32 {loss, policy loss, kl,
+    clip fraction, mean r - 1 - ln r, unmasked tokens}.  Per token -min(r A, clip(r, 1 - clip_low, 1 + clip_high) A)
+    + kl_coef k(new - ref); kl "k1": e, "k2": e^2 / 2, "k3": e^-e - 1 + e; without ref_lp there is no KL term.
+    reduction "token": means over the unmasked tokens, "sequence": over the non-empty sequences of their means.  mask
+    [B, L] bool or uint8; adv [B, L], or [B] for one advantage a sequence.  Log-probs and advantages are f32; rows may be
+    strided."""
+    lib = _lib.load()
+    name = "policy_kl_loss"
+    _need(new_lp.dim() == 2, f"{name}: log-probs are [sequences, tokens]")
+    _need(kl in KL_KINDS, f"{name}: kl is one of {sorted(KL_KINDS)}")
+    _need(reduction in ("token", "sequence"), f"{name}: reduction is 'token' or 'sequence'")
+    _need(0.0 <= float(clip_low) < 1.0 and 0.0 <= float(clip_high) <= 1e30, f"{name}: clip_low in [0, 1), clip_high >= 0")
+    _need(float(kl_coef) == float(kl_coef), f"{name}: kl_coef is NaN")
+    B, L = shape = tuple(new_lp.shape)
+    new, new_s = _sequence_rows(name, "new_lp", new_lp, shape)
+    old, old_s = _sequence_rows(name, "old_lp", old_lp, shape)
+    ref, ref_s = _sequence_rows(name, "ref_lp", ref_lp, shape)
+    msk, msk_s = _sequence_rows(name, "mask", mask, shape, _MASK_TYPES)
+    per_sequence = isinstance(adv, torch.Tensor) and adv.dim() == 1
+    a, a_s = _sequence_rows(name, "adv", adv, shape[:1] if per_sequence else shape)
+    _need(old is not None and a is not None, f"{name}: old_lp and adv are needed")
+    _device_tensors(name, new, old, ref, msk, a)
+    dev = new.device
+    g = torch.empty(shape, dtype=torch.float32, device=dev) if want_grad else None
+    if B == 0 or L == 0:
+        return torch.zeros(6, dtype=torch.float32, device=dev), g
+    out6 = torch.empty(6, dtype=torch.float32, device=dev)
+    nws = lib.ppo_policy_kl_loss_workspace_bytes(B)
+    ws = torch.empty(nws, dtype=torch.uint8, device=dev)
+    rc = lib.ppo_policy_kl_loss(new.data_ptr(), new_s, old.data_ptr(), old_s, a.data_ptr(), a_s, int(per_sequence), _ptr(ref),
+                                ref_s, _ptr(msk), msk_s, B, L, float(clip_low), float(clip_high), float(kl_coef), KL_KINDS[kl],
+                                int(reduction == "sequence"), out6.data_ptr(), _ptr(g), ws.data_ptr(), nws, _stream())
+    _lib.check(rc, "ppo_policy_kl_loss")
+    return out6, g
+
+
+def policy_kl_loss(new_lp, old_lp, adv, mask=None, ref_lp=None, clip_low=0.2, clip_high=0.2, kl_coef=0.0, kl="k3", reduction="token"):
+    """(loss, policy_loss, kl, clip_frac, kl_div), each 0-d f32: policy_kl_loss_fwd_bwd with the loss differentiable with
+    respect to new_lp (kl_div = mean r - 1 - ln r against the old policy, as ppo_losses reports it)."""
+    need = torch.is_grad_enabled() and new_lp.requires_grad
+    with torch.no_grad():
+        out6, g = policy_kl_loss_fwd_bwd(new_lp, old_lp, adv, mask, ref_lp, clip_low, clip_high, kl_coef, kl, reduction, want_grad=need)
+    loss = out6[0]
+    if need:
+        loss = _AttachGrad.apply(new_lp, loss, g)
+    return loss, out6[1], out6[2], out6[3], out6[4]
+
+
+@_on_tensor_device
+def preference_loss_fwd_bwd(chosen_lp, rejected_lp, ref_chosen_lp=None, ref_rejected_lp=None, chosen_mask=None, rejected_mask=None,
+                            beta=0.1, kind="sigmoid", label_smoothing=0.0, average=False, want_grad=True):
+    """ppo_preference_loss: the mean over pairs of a loss on D = sum(chosen - ref) - sum(rejected - ref) over the unmasked
+    tokens (means with `average`), z = beta D: "sigmoid" -(1 - e) ln s(z) - e ln s(-z) with label_smoothing e, "hinge"
+    max(0, 1 - z), "ipo" (D - 1 / (2 beta))^2.  chosen_lp [pairs, Lc], rejected_lp [pairs, Lr] token log-probs, f32, rows
+    may be strided (the two halves of one batch are views of it).  Returns (out2 {loss, share of pairs with z > 0}, rewards
+    [pairs, 2] = beta times the two sums, g_chosen, g_rejected)."""
+    lib = _lib.load()
+    name = "preference_loss"
+    _need(chosen_lp.dim() == 2 and isinstance(rejected_lp, torch.Tensor) and rejected_lp.dim() == 2 and rejected_lp.shape[0] == chosen_lp.shape[0],
+          f"{name}: log-probs are [pairs, tokens], as many pairs chosen as rejected")
+    _need(kind in PREFERENCE_KINDS, f"{name}: kind is one of {sorted(PREFERENCE_KINDS)}")
+    _need(0.0 < float(beta) <= 1e30, f"{name}: beta > 0")
+    _need(0.0 <= float(label_smoothing) < 0.5, f"{name}: label_smoothing in [0, 0.5)")
+    pairs = chosen_lp.shape[0]
+    sides, tensors, grads = [], [], []
+    for what, lp, ref, mask in (("chosen", chosen_lp, ref_chosen_lp, chosen_mask), ("rejected", rejected_lp, ref_rejected_lp, rejected_mask)):
+        x, xs = _sequence_rows(name, what + "_lp", lp, lp.shape)
+        r, rs = _sequence_rows(name, f"ref_{what}_lp", ref, lp.shape)
+        m, ms = _sequence_rows(name, what + "_mask", mask, lp.shape, _MASK_TYPES)
+        tensors += [x, r, m]
+        sides += [x.data_ptr(), xs, _ptr(r), rs, _ptr(m), ms, lp.shape[1]]
+    _device_tensors(name, *tensors)
+    dev = chosen_lp.device
+    for lp in (chosen_lp, rejected_lp):
+        grads.append(torch.empty(lp.shape, dtype=torch.float32, device=dev) if want_grad else None)
+    rewards = torch.empty((pairs, 2), dtype=torch.float32, device=dev)
+    if pairs == 0:
+        return torch.zeros(2, dtype=torch.float32, device=dev), rewards, *grads
+    out2 = torch.empty(2, dtype=torch.float32, device=dev)
+    nws = lib.ppo_preference_loss_workspace_bytes(pairs, chosen_lp.shape[1], rejected_lp.shape[1])
+    ws = torch.empty(nws, dtype=torch.uint8, device=dev)
+    rc = lib.ppo_preference_loss(*sides, pairs, PREFERENCE_KINDS[kind], float(beta), float(label_smoothing), int(bool(average)),
+                                 out2.data_ptr(), rewards.data_ptr(), _ptr(grads[0]), _ptr(grads[1]), ws.data_ptr(), nws, _stream())
+    _lib.check(rc, "ppo_preference_loss")
+    return out2, rewards, *grads
+
+
+class _PairLoss(torch.autograd.Function):
+    """value(a, b) with both gradients precomputed by ppo_preference_loss."""
+
+    @staticmethod
+    def forward(ctx, a, b, value, g_a, g_b):
+        ctx.save_for_backward(g_a, g_b)
+        return value.clone()
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g_out):
+        g_a, g_b = ctx.saved_tensors
+        return (g_a * g_out if ctx.needs_input_grad[0] else None, g_b * g_out if ctx.needs_input_grad[1] else None, None, None, None)
+
+
+def preference_loss(chosen_lp, rejected_lp, ref_chosen_lp=None, ref_rejected_lp=None, chosen_mask=None, rejected_mask=None, beta=0.1,
+                    kind="sigmoid", label_smoothing=0.0, average=False):
+    """(loss, accuracy, rewards [pairs, 2]): preference_loss_fwd_bwd with the loss differentiable with respect to the
+    chosen and the rejected log-probs."""
+    need = torch.is_grad_enabled() and (chosen_lp.requires_grad or rejected_lp.requires_grad)
+    with torch.no_grad():
+        out2, rewards, g_c, g_r = preference_loss_fwd_bwd(chosen_lp, rejected_lp, ref_chosen_lp, ref_rejected_lp, chosen_mask,
+                                                          rejected_mask, beta, kind, label_smoothing, average, want_grad=need)
+    loss = _PairLoss.apply(chosen_lp, rejected_lp, out2[0], g_c, g_r) if need else out2[0]
+    return loss, out2[1], rewards
