@@ -599,6 +599,34 @@ int ppo_preference_loss(const float *chosen, long chosen_stride, const float *re
                         int average, float *out2, float *rewards, float *g_chosen, float *g_rejected, void *workspace,
                         size_t workspace_bytes, void *stream);
 
+/*
+ * y = act(x W^T + bias) + residual and its gradients, for layers of any size (ppo_linear_wgrad serves layers of at most
+ * 64 x 64 over huge batches).  x [rows, inputs], weight [outputs, inputs], residual [rows, outputs] of `dtype`, rows
+ * x_stride, weight_stride, residual_stride elements apart; bias [outputs] or NULL; residual NULL for none.
+ *   y [rows, outputs] contiguous; deriv the same or NULL: act'(z) for the backward call, f16 for PPO_DTYPE_BF16, f32 for
+ *   the other types.
+ * Sums are f32: 16-bit inputs on the 16-bit matrix cores; f32 inputs as three bf16 pieces each (PPO_NET_BF16X3), f32-grade,
+ * except that magnitudes above 3.38e38 and infinities give NaN where more than 8 rows make the matrix cores worth while.
+ * ppo_linear_act_bwd: with u = g_y * deriv (deriv NULL: u = g_y), rounded to `dtype`:
+ *   g_x [rows, inputs] = u W, g_weight [outputs, inputs] = u^T x, g_bias [outputs] = column sums of the unrounded u; each
+ *   contiguous, of `dtype`, or NULL.  The residual's gradient is g_y.
+ * rows, inputs and outputs are at most 2^22 - 128, and no matrix has more than 2^38 elements.  Results do not depend on anything but the arguments (sums have a fixed order).
+ * Workspaces: the two functions' bytes, 16-byte aligned.  No output may overlap an input.
+ */
+#define PPO_ACT_NONE 0
+#define PPO_ACT_TANH 1
+#define PPO_ACT_RELU 2
+#define PPO_ACT_GELU 3 /* z Phi(z), the normal distribution's */
+#define PPO_ACT_SILU 4
+size_t ppo_linear_act_fwd_workspace_bytes(long rows, long inputs, long outputs, int dtype);
+int ppo_linear_act_fwd(const void *x, long x_stride, const void *weight, long weight_stride, const void *bias, const void *residual,
+                       long residual_stride, int dtype, long rows, long inputs, long outputs, int activation, void *y, void *deriv,
+                       void *workspace, size_t workspace_bytes, void *stream);
+size_t ppo_linear_act_bwd_workspace_bytes(long rows, long inputs, long outputs, int dtype);
+int ppo_linear_act_bwd(const void *g_y, long g_stride, const void *x, long x_stride, const void *weight, long weight_stride,
+                       const void *deriv, int dtype, long rows, long inputs, long outputs, void *g_x, void *g_weight, void *g_bias,
+                       void *workspace, size_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

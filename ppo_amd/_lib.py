@@ -61,6 +61,10 @@ SIGNATURES = {
     "ppo_policy_kl_loss": (_i, [_vp, _l, _vp, _l, _vp, _l, _i, _vp, _l, _vp, _l, _l, _l, _d, _d, _d, _i, _i, _vp, _vp, _vp, _sz, _vp]),
     "ppo_preference_loss_workspace_bytes": (_sz, [_l, _l, _l]),
     "ppo_preference_loss": (_i, [_vp, _l, _vp, _l, _vp, _l, _l] * 2 + [_l, _i, _d, _d, _i, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "ppo_linear_act_fwd_workspace_bytes": (_sz, [_l, _l, _l, _i]),
+    "ppo_linear_act_fwd": (_i, [_vp, _l, _vp, _l, _vp, _vp, _l, _i, _l, _l, _l, _i, _vp, _vp, _vp, _sz, _vp]),
+    "ppo_linear_act_bwd_workspace_bytes": (_sz, [_l, _l, _l, _i]),
+    "ppo_linear_act_bwd": (_i, [_vp, _l, _vp, _l, _vp, _l, _vp, _i, _l, _l, _l, _vp, _vp, _vp, _vp, _sz, _vp]),
     "ppo_rollout_fused_packed": (_i, [_i, _vp, _vp, _vp, _vp, _vp, _vp, _u64, _u64, _vp, _i, _i, _u64, _vp, _vp, _vp, _vp,
                                       _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _vp]),
 }

@@ -1,0 +1,719 @@
+// y = act(x W^T + b) + residual, forward and backward, on the matrix cores -- gfx950.
+//
+// Beside ppo_linear_wgrad (wgrad.hip: layers of at most 64 x 64 over millions of rows) for layers of any size and for
+// 16-bit types.  With z = x W^T + b, y = act(z) + r the forward pass also keeps d = act'(z) where a gradient will be
+// asked for; then for a gradient g of y
+//     u = g d,   g_x = u W,   g_W = u^T x,   g_b = sum over rows of u.
+// d is kept rather than z: act'(z) of a z rounded to bf16 is off by 1.5 % for tanh at z = 4.  It is kept in f16 for bf16
+// layers (|d| < 1.2: 8 times finer than bf16) and in f32 for the others, so that the one rounding that counts beside the
+// outputs' own is that of u to the inputs' type, which the two products need; g_b sums u unrounded, in f32.
+//
+// One product, C[m, n] = sum_k A[m, k] B[n, k] with k contiguous in both, serves all three: backward, the operands whose
+// k is not contiguous are transposed by k_prep first (a pass over memory against M N K operations).
+//   * 16-bit inputs: v_mfma_f32_16x16x32_{bf16,f16}, f32 accumulators.
+//   * f32 inputs: every operand split in registers into three bf16 pieces that represent it exactly (mfma_split.h), six
+//     products of order <= 2 into one f32 accumulator: the three left out are below 2^-23 of the product.  f32 matrix
+//     instructions run at 1/16 of the bf16 rate, so six of these are 2.7 times as fast.  An infinite operand gives NaN.
+// A workgroup of 8 waves computes 256 x 256 of C (4 waves: 128 x 128, where there would be too few of the larger ones),
+// a wave 128 x 64 (64 x 64) of it.  Rows of 128 bytes of k (64 halves, 32 floats) are brought straight into LDS, two
+// stages, the next one on its way while the matrix cores work on this one.  16-byte pieces are swizzled inside their row
+// so that the 16 rows a fragment read touches fall into different banks; A and B have their own swizzles because B's rows
+// are read in an order that gives a lane 16 neighbouring n of the result, i.e. whole 32- or 64-byte stores.
+// The operands of v_mfma are swapped (B first), so that a lane's accumulators run along n.
+#include "token_common.h"
+#include "mfma_split.h"
+
+using namespace ppo_token;
+
+namespace {
+
+using f32x4 = __attribute__((ext_vector_type(4))) float;
+using u32x4 = __attribute__((ext_vector_type(4))) uint32_t;
+using h8v = __attribute__((ext_vector_type(8))) _Float16;
+using b8v = __attribute__((ext_vector_type(8))) __bf16;
+
+template <class T> __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c)
+{
+    if constexpr (std::is_same_v<T, F16>)
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8v, a), __builtin_bit_cast(h8v, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8v, a), __builtin_bit_cast(b8v, b), c, 0, 0, 0);
+}
+
+// ---- activations: value and derivative ------------------------------------------------------------------------------
+__device__ __forceinline__ void activate(int act, float z, float &y, float &d)
+{
+    switch (act) {
+    case PPO_ACT_TANH: {
+        const float e = expf(-2.0f * fabsf(z)), t = (1.0f - e) / (1.0f + e);
+        y = fabsf(z) < 0.1f ? tanhf(z) : copysignf(t, z);
+        d = 4.0f * e / ((1.0f + e) * (1.0f + e));           // 1 - tanh^2 without its cancellation
+        if (z != z) y = d = z;
+        break;
+    }
+    case PPO_ACT_RELU:
+        y = z > 0.0f ? z : (z != z ? z : 0.0f);
+        d = z > 0.0f ? 1.0f : 0.0f;
+        break;
+    case PPO_ACT_GELU: {
+        const float phi = 0.5f * erfcf(-0.70710678f * z);   // P(normal < z), without cancellation in the left tail
+        y = z * phi;
+        if (z == -INFINITY) y = 0.0f;
+        d = phi + z * expf(-0.5f * z * z) * 0.3989422804f;
+        if (fabsf(z) == INFINITY) d = z > 0.0f ? 1.0f : 0.0f;
+        break;
+    }
+    case PPO_ACT_SILU: {
+        const float s = 1.0f / (1.0f + expf(-z));
+        y = z == -INFINITY ? 0.0f : z * s;
+        d = fabsf(z) == INFINITY ? s : s * (1.0f + z * (1.0f - s));
+        break;
+    }
+    default:
+        y = z;
+        d = 1.0f;
+    }
+}
+
+template <class T> struct DerivOf { using type = F32; };
+template <> struct DerivOf<BF16> { using type = F16; };
+template <class T> using D = typename DerivOf<T>::type;
+
+// N neighbouring elements of 16 bytes a piece
+template <class T, int N> __device__ __forceinline__ void load_n(const typename T::raw *p, float (&v)[N])
+{
+    constexpr int E = 16 / T::BYTES;
+    if constexpr (N <= E) {
+        struct __attribute__((packed, aligned(T::BYTES))) Part { typename T::raw r[N]; };
+        const Part w = *reinterpret_cast<const Part *>(p);
+#pragma unroll
+        for (int j = 0; j < N; ++j) v[j] = T::load(w.r[j]);
+    } else {
+#pragma unroll
+        for (int q = 0; q < N; q += E) {
+            float w[E];
+            load16<T>(p + q, w);
+#pragma unroll
+            for (int j = 0; j < E; ++j) v[q + j] = w[j];
+        }
+    }
+}
+
+template <class T, int N> __device__ __forceinline__ void store_n(typename T::raw *p, const float (&v)[N])
+{
+    constexpr int E = 16 / T::BYTES;
+    static_assert(N % E == 0, "whole pieces");
+#pragma unroll
+    for (int q = 0; q < N; q += E) {
+        float w[E];
+#pragma unroll
+        for (int j = 0; j < E; ++j) w[j] = v[q + j];
+        store16<T>(p + q, w);
+    }
+}
+
+// ---- operand preparation: pad, multiply by d, transpose, sum columns -----------------------------------------------
+// src [R, C] of T with row stride ld (times mul [R, C] of D<T>, contiguous) -> rows [R, Cp] and / or cols [C, Rp] of T, Cp and Rp
+// the next multiples of a k step, zero-filled; sums [tiles of 64 rows][C] f32 = column sums of a tile.
+struct PrepArgs {
+    const void *src, *mul;
+    void *rows, *cols;
+    float *sums;
+    long R, C, ld, Rp, Cp;
+};
+
+template <class T> __global__ void __launch_bounds__(256) k_prep(PrepArgs a)
+{
+    constexpr int E = 16 / T::BYTES, TPR = 64 / E, RPP = 256 / TPR;   // threads a row of 64, rows a pass
+    using raw = typename T::raw;
+    __shared__ raw tile[64][64 + 4 / T::BYTES];
+    __shared__ float colsum[RPP][64];
+    const long r0 = (long)blockIdx.y * 64, c0 = (long)blockIdx.x * 64;
+    const int tc = threadIdx.x % TPR * E, tr = threadIdx.x / TPR;
+    const raw *src = reinterpret_cast<const raw *>(a.src);
+    const typename D<T>::raw *mul = reinterpret_cast<const typename D<T>::raw *>(a.mul);
+    float sum[E];
+#pragma unroll
+    for (int j = 0; j < E; ++j) sum[j] = 0.0f;
+#pragma unroll
+    for (int p = 0; p < 64 / RPP; ++p) {
+        const int r = p * RPP + tr;
+        const long gr = r0 + r, gc = c0 + tc;
+        float v[E];
+        if (gr < a.R && gc + E <= a.C) {
+            load16<T>(src + gr * a.ld + gc, v);
+            if (mul) {
+                float w[E];
+                load_n<D<T>, E>(mul + gr * a.C + gc, w);
+#pragma unroll
+                for (int j = 0; j < E; ++j) v[j] *= w[j];
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < E; ++j) {
+                v[j] = 0.0f;
+                if (gr < a.R && gc + j < a.C) {
+                    v[j] = T::load(src[gr * a.ld + gc + j]);
+                    if (mul) v[j] *= D<T>::load(mul[gr * a.C + gc + j]);
+                }
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < E; ++j) sum[j] += v[j];
+        if (a.rows && gr < a.R && gc < a.Cp) store16<T>(reinterpret_cast<raw *>(a.rows) + gr * a.Cp + gc, v);
+        if (a.cols) {
+#pragma unroll
+            for (int j = 0; j < E; ++j) tile[r][tc + j] = T::store(v[j]);
+        }
+    }
+    if (a.sums) {
+#pragma unroll
+        for (int j = 0; j < E; ++j) colsum[tr][tc + j] = sum[j];
+    }
+    __syncthreads();
+    if (a.cols) {
+#pragma unroll
+        for (int p = 0; p < 64 / RPP; ++p) {
+            const int c = p * RPP + tr;
+            const long gc = c0 + c, gr = r0 + tc;
+            if (gc < a.C && gr < a.Rp) {
+                raw v[E];
+#pragma unroll
+                for (int j = 0; j < E; ++j) v[j] = tile[tc + j][c];
+                *reinterpret_cast<u32x4 *>(reinterpret_cast<raw *>(a.cols) + gc * a.Rp + gr) = __builtin_bit_cast(u32x4, v);
+            }
+        }
+    }
+    if (a.sums && threadIdx.x < 64 && c0 + threadIdx.x < a.C) {
+        float s = 0.0f;
+        for (int k = 0; k < RPP; ++k) s += colsum[k][threadIdx.x];
+        a.sums[(long)blockIdx.y * a.C + c0 + threadIdx.x] = s;
+    }
+}
+
+template <class T> __global__ void __launch_bounds__(256) k_bias_grad(const float *sums, long tiles, long C, typename T::raw *out)
+{
+    // 64 columns a workgroup, four waves share the tiles of rows
+    __shared__ float part[4][64];
+    const long c = (long)blockIdx.x * 64 + (threadIdx.x & 63);
+    const int w = threadIdx.x >> 6;
+    float s = 0.0f;
+    if (c < C)
+        for (long t = w; t < tiles; t += 4) s += sums[t * C + c];
+    part[w][threadIdx.x & 63] = s;
+    __syncthreads();
+    if (w == 0 && c < C) out[c] = T::store((part[0][threadIdx.x] + part[1][threadIdx.x]) + (part[2][threadIdx.x] + part[3][threadIdx.x]));
+}
+
+// ---- the product -----------------------------------------------------------------------------------------------------
+struct GemmArgs {
+    const void *A, *B;                 // [M, k], [N, k]; rows lda, ldb bytes apart
+    long M, N, lda, ldb;
+    int steps, steps_per_split;        // steps of 128 bytes of k
+    int tiles_m, tiles_n;
+    float *partial;                    // [splits][M][N], or NULL: the epilogue below
+    const void *bias, *residual;
+    long res_ld;
+    void *out, *deriv;                 // [M, N] contiguous
+    int act;
+};
+
+template <class T> __device__ __forceinline__ void finish(const GemmArgs &g, long m, long n, float z, float &y, float &d)
+{
+    using raw = typename T::raw;
+    if (g.bias) z += T::load(reinterpret_cast<const raw *>(g.bias)[n]);
+    activate(g.act, z, y, d);
+    if (g.residual) y += T::load(reinterpret_cast<const raw *>(g.residual)[m * g.res_ld + n]);
+}
+
+// CNT (at most 16) neighbouring results of row m
+template <class T, int CNT> __device__ __forceinline__ void epilogue(const GemmArgs &g, long m, long n, const float (&z)[CNT])
+{
+    using raw = typename T::raw;
+    constexpr int E = 16 / T::BYTES;
+    if (m >= g.M || n >= g.N) return;
+    raw *out = reinterpret_cast<raw *>(g.out) + m * g.N + n;
+    typename D<T>::raw *der = g.deriv ? reinterpret_cast<typename D<T>::raw *>(g.deriv) + m * g.N + n : nullptr;
+    if (n + CNT <= g.N) {
+#pragma unroll
+        for (int q = 0; q < CNT; q += E) {
+            float b[E], r[E], y[E], d[E];
+            if (g.bias) load16<T>(reinterpret_cast<const raw *>(g.bias) + n + q, b);
+            if (g.residual) load16<T>(reinterpret_cast<const raw *>(g.residual) + m * g.res_ld + n + q, r);
+#pragma unroll
+            for (int j = 0; j < E; ++j) {
+                activate(g.act, g.bias ? z[q + j] + b[j] : z[q + j], y[j], d[j]);
+                if (g.residual) y[j] += r[j];
+            }
+            store16<T>(out + q, y);
+            if (der) store_n<D<T>, E>(der + q, d);
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < CNT; ++j) {
+            if (n + j < g.N) {
+                float y, d;
+                finish<T>(g, m, n + j, z[j], y, d);
+                out[j] = T::store(y);
+                if (der) der[j] = D<T>::store(d);
+            }
+        }
+    }
+}
+
+// swizzles: which 16-byte piece of an LDS row holds piece c of the operand's row
+__device__ __forceinline__ int swizzle_a(int row) { return (row & 7) ^ ((row >> 3) & 1); }
+__device__ __forceinline__ int swizzle_b(int row) { return ((row & 3) | ((row >> 2) & 4)) ^ ((row >> 5) & 1); }
+
+// 64 lanes bring 16 bytes each from rsrc[voff + soff] to LDS at lds + 16 lane.  In asm because the compiler's own form of
+// this load makes every LDS read wait for all of them; it has no destination register, and the loop below waits itself.
+__device__ __forceinline__ void load_lds(u32x4 rsrc, uint32_t voff, int soff, uint32_t lds)
+{
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(lds), "v"(voff), "s"(rsrc), "s"(soff) : "memory");
+}
+
+__device__ __forceinline__ u32x4 buffer_of(const void *p, long bytes)
+{
+    const uint64_t at = reinterpret_cast<uint64_t>(p);
+    const uint32_t n = bytes > 0xffffffffL ? 0xffffffffu : (uint32_t)bytes;
+    return u32x4{(uint32_t)__builtin_amdgcn_readfirstlane((int)at), (uint32_t)__builtin_amdgcn_readfirstlane((int)(at >> 32)) & 0xffffu,
+                 (uint32_t)__builtin_amdgcn_readfirstlane((int)n), 0x00027000u};
+}
+
+template <class T, int BM, int BN, int WAVES_M, int WAVES_N>
+__global__ void __launch_bounds__(64 * WAVES_M * WAVES_N) k_gemm(GemmArgs g)
+{
+    constexpr int WAVES = WAVES_M * WAVES_N, WM = BM / WAVES_M, WN = BN / WAVES_N, MI = WM / 16, NI = WN / 16;
+    static_assert(WN == 64 && MI * 16 * WAVES_M == BM, "a lane's 16 neighbouring n need 64 columns a wave");
+    constexpr int LA = BM / 8 / WAVES, LB = BN / 8 / WAVES;          // loads a wave and stage (8 rows each)
+    constexpr int STAGE = (BM + BN) * 128;
+    __shared__ __align__(1024) char lds[2 * STAGE];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wm = wave / WAVES_N, wn = wave % WAVES_N;
+
+    // tiles: an XCD (workgroups go round them one by one) takes a run of neighbouring ones, in bands of 8 rows of tiles,
+    // so that what its L2 holds is used by several of its workgroups
+    const int tiles = g.tiles_m * g.tiles_n;
+    int id = blockIdx.x;
+    {
+        const int x = id % 8, q = tiles / 8, rem = tiles % 8;
+        id = x * q + (x < rem ? x : rem) + id / 8;
+    }
+    const int band = 8 * g.tiles_n, first = id / band * 8, high = g.tiles_m - first < 8 ? g.tiles_m - first : 8;
+    const long m0 = (long)(first + id % band % high) * BM, n0 = (long)(id % band / high) * BN;
+    const int s0 = blockIdx.y * g.steps_per_split, s1 = s0 + g.steps_per_split < g.steps ? s0 + g.steps_per_split : g.steps;
+
+    const long kbytes = (long)g.steps * 128;
+    const long rows_a = g.M - m0 < BM ? g.M - m0 : BM, rows_b = g.N - n0 < BN ? g.N - n0 : BN;
+    const u32x4 ra = buffer_of(reinterpret_cast<const char *>(g.A) + m0 * g.lda, (rows_a - 1) * g.lda + kbytes);
+    const u32x4 rb = buffer_of(reinterpret_cast<const char *>(g.B) + n0 * g.ldb, (rows_b - 1) * g.ldb + kbytes);
+    uint32_t va[LA], vb[LB];           // (256 rows of less than 2^24 bytes: below 2^32)
+#pragma unroll
+    for (int i = 0; i < LA; ++i) {
+        const int row = (i * WAVES + wave) * 8 + lane / 8, have = row < rows_a ? row : (int)rows_a - 1;   // rows past the end repeat the last
+        va[i] = (uint32_t)have * (uint32_t)g.lda + ((lane % 8) ^ swizzle_a(row)) * 16;
+    }
+#pragma unroll
+    for (int i = 0; i < LB; ++i) {
+        const int row = (i * WAVES + wave) * 8 + lane / 8, have = row < rows_b ? row : (int)rows_b - 1;
+        vb[i] = (uint32_t)have * (uint32_t)g.ldb + ((lane % 8) ^ swizzle_b(row)) * 16;
+    }
+    const uint32_t base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds;
+    auto stage = [&](int s) {
+        const uint32_t to = base + (s & 1) * STAGE + wave * 1024;
+        const int k = s * 128;
+#pragma unroll
+        for (int i = 0; i < LA; ++i) load_lds(ra, va[i], k, to + i * WAVES * 1024);
+#pragma unroll
+        for (int i = 0; i < LB; ++i) load_lds(rb, vb[i], k, to + BM * 128 + i * WAVES * 1024);
+    };
+
+    // fragment reads: lane q = lane % 16 reads k piece lane / 16 of row ... of A: 16 mi + q, of B: 16 (q / 4) + 4 ni + q % 4
+    const int q = lane & 15, kg = lane >> 4;
+    const int row_a = wm * WM + q, row_b = wn * WN + (q >> 2) * 16 + (q & 3);
+    const int pa = row_a * 128, pb = BM * 128 + row_b * 128, xa = swizzle_a(row_a), xb = swizzle_b(row_b);
+
+    f32x4 acc[MI][NI];
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
+#pragma unroll
+        for (int j = 0; j < NI; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    ppo_net::Bf16Select sel;
+    if constexpr (T::BYTES == 4) sel.init();
+
+    if (s0 < s1) stage(s0);
+    for (int s = s0; s < s1; ++s) {
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();                       // stage s has landed for every wave, and nobody reads the other one
+        asm volatile("" ::: "memory");
+        if (s + 1 < s1) stage(s + 1);
+        const char *at = lds + (s & 1) * STAGE;
+        if constexpr (T::BYTES == 2) {
+#pragma unroll
+            for (int ks = 0; ks < 2; ++ks) {
+                u32x4 fa[MI], fb[NI];
+                const int ca = ((ks * 4 + kg) ^ xa) * 16, cb = ((ks * 4 + kg) ^ xb) * 16;
+#pragma unroll
+                for (int j = 0; j < NI; ++j) fb[j] = *reinterpret_cast<const u32x4 *>(at + pb + j * 512 + cb);
+#pragma unroll
+                for (int i = 0; i < MI; ++i) fa[i] = *reinterpret_cast<const u32x4 *>(at + pa + i * 2048 + ca);
+#pragma unroll
+                for (int i = 0; i < MI; ++i)
+#pragma unroll
+                    for (int j = 0; j < NI; ++j) acc[i][j] = mfma<T>(fb[j], fa[i], acc[i][j]);
+            }
+        } else {
+            u32x4 fb[NI][3];
+            const int ca0 = ((2 * kg) ^ xa) * 16, ca1 = ((2 * kg + 1) ^ xa) * 16, cb0 = ((2 * kg) ^ xb) * 16, cb1 = ((2 * kg + 1) ^ xb) * 16;
+            auto split = [&](const char *p0, const char *p1, u32x4(&f)[3]) {
+                const f32x4 lo = *reinterpret_cast<const f32x4 *>(p0), hi = *reinterpret_cast<const f32x4 *>(p1);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    uint32_t w0, w1, w2;
+                    ppo_net::split3_bf16(e < 2 ? lo[2 * e] : hi[2 * e - 4], e < 2 ? lo[2 * e + 1] : hi[2 * e - 3], sel, w0, w1, w2);
+                    f[0][e] = w0;
+                    f[1][e] = w1;
+                    f[2][e] = w2;
+                }
+            };
+#pragma unroll
+            for (int j = 0; j < NI; ++j) split(at + pb + j * 512 + cb0, at + pb + j * 512 + cb1, fb[j]);
+#pragma unroll
+            for (int i = 0; i < MI; ++i) {
+                u32x4 fa[3];
+                split(at + pa + i * 2048 + ca0, at + pa + i * 2048 + ca1, fa);
+#pragma unroll
+                for (int t = 0; t < 6; ++t) {
+                    constexpr int PA[6] = {0, 2, 1, 0, 1, 0}, PB[6] = {2, 0, 1, 1, 0, 0};   // small terms first
+#pragma unroll
+                    for (int j = 0; j < NI; ++j) acc[i][j] = mfma<BF16>(fb[j][PB[t]], fa[PA[t]], acc[i][j]);
+                }
+            }
+        }
+    }
+
+    // acc[i][j][e] is C[m0 + wm WM + 16 i + q][n0 + wn WN + 16 kg + 4 j + e].  One row of tiles at a time in a loop, the
+    // others moving down a place: unrolled, the activations' code would be there MI times (90 KB of it)
+    const long n = n0 + wn * WN + kg * 16;
+    long m = m0 + wm * WM + q;
+#pragma clang loop unroll(disable)
+    for (int i = 0; i < MI; ++i, m += 16) {
+        float z[16];
+#pragma unroll
+        for (int j = 0; j < NI; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) z[j * 4 + e] = acc[0][j][e];
+#pragma unroll
+        for (int k = 0; k + 1 < MI; ++k)
+#pragma unroll
+            for (int j = 0; j < NI; ++j) acc[k][j] = acc[k + 1][j];
+        if (g.partial) {
+            if (m < g.M && n < g.N) {
+                float *p = g.partial + ((long)blockIdx.y * g.M + m) * g.N + n;
+                if (n + 16 <= g.N) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const float w[4] = {z[4 * j], z[4 * j + 1], z[4 * j + 2], z[4 * j + 3]};
+                        store16<F32>(p + 4 * j, w);
+                    }
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 16; ++j)
+                        if (n + j < g.N) p[j] = z[j];
+                }
+            }
+        } else {
+            epilogue<T, 16>(g, m, n, z);
+        }
+    }
+}
+
+// sums the splits of a row's 16 / BYTES neighbouring results, in order, and finishes them
+template <class T> __global__ void __launch_bounds__(256) k_join(GemmArgs g, int splits)
+{
+    constexpr int E = 16 / T::BYTES;
+    const long per_row = (g.N + E - 1) / E, id = (long)blockIdx.x * 256 + threadIdx.x;
+    const long m = id / per_row, n = (id - m * per_row) * E;
+    if (m >= g.M) return;
+    float z[E];
+#pragma unroll
+    for (int j = 0; j < E; ++j) z[j] = 0.0f;
+    const int have = g.N - n < E ? (int)(g.N - n) : E;
+    for (int s = 0; s < splits; ++s) {
+        const float *p = g.partial + ((long)s * g.M + m) * g.N + n;
+        if (have == E) {
+#pragma unroll
+            for (int j = 0; j < E; j += 4) {
+                float w[4];
+                load16<F32>(p + j, w);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) z[j + k] += w[k];
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < E; ++j)
+                if (j < have) z[j] += p[j];
+        }
+    }
+    epilogue<T, E>(g, m, n, z);
+}
+
+// ---- few rows: the weights are read once, by the vector units --------------------------------------------------------
+// a wave COLS rows of W, lanes along k; ROWS rows of x
+template <class T, int ROWS, int COLS> __global__ void __launch_bounds__(256) k_few_rows(GemmArgs g, long K)
+{
+    constexpr int E = 16 / T::BYTES;
+    using raw = typename T::raw;
+    const int lane = threadIdx.x & 63;
+    const long n0 = ((long)blockIdx.x * 4 + (threadIdx.x >> 6)) * COLS, m0 = (long)blockIdx.y * ROWS;
+    if (n0 >= g.N) return;
+    const raw *x[ROWS], *w[COLS];
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) x[r] = reinterpret_cast<const raw *>(reinterpret_cast<const char *>(g.A) + (m0 + r < g.M ? m0 + r : g.M - 1) * g.lda);
+#pragma unroll
+    for (int c = 0; c < COLS; ++c) w[c] = reinterpret_cast<const raw *>(reinterpret_cast<const char *>(g.B) + (n0 + c < g.N ? n0 + c : g.N - 1) * g.ldb);
+    float acc[ROWS][COLS];
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r)
+#pragma unroll
+        for (int c = 0; c < COLS; ++c) acc[r][c] = 0.0f;
+    long k = (long)lane * E;
+    for (; k + E <= K; k += 64 * E) {
+        float wv[COLS][E];
+#pragma unroll
+        for (int c = 0; c < COLS; ++c) load16<T>(w[c] + k, wv[c]);
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r) {
+            float xv[E];
+            load16<T>(x[r] + k, xv);
+#pragma unroll
+            for (int c = 0; c < COLS; ++c)
+#pragma unroll
+                for (int j = 0; j < E; ++j) acc[r][c] = __builtin_fmaf(xv[j], wv[c][j], acc[r][c]);
+        }
+    }
+    for (; k < K; ++k) {                                    // (at most one lane has a part of 16 bytes left)
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r)
+#pragma unroll
+            for (int c = 0; c < COLS; ++c) acc[r][c] = __builtin_fmaf(T::load(x[r][k]), T::load(w[c][k]), acc[r][c]);
+        if (k % E == E - 1) break;
+    }
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r)
+#pragma unroll
+        for (int c = 0; c < COLS; ++c) {
+#pragma unroll
+            for (int off = 32; off > 0; off >>= 1) acc[r][c] += __shfl_xor(acc[r][c], off, 64);
+        }
+    if (lane < ROWS && m0 + lane < g.M) {
+#pragma unroll
+        for (int c = 0; c < COLS; ++c) {
+            float z = 0.0f;
+#pragma unroll
+            for (int r = 0; r < ROWS; ++r) z = lane == r ? acc[r][c] : z;
+            const float one[1] = {z};
+            if (n0 + c < g.N) {
+                float y, d;
+                finish<T>(g, m0 + lane, n0 + c, one[0], y, d);
+                reinterpret_cast<raw *>(g.out)[(m0 + lane) * g.N + n0 + c] = T::store(y);
+                if (g.deriv) reinterpret_cast<typename D<T>::raw *>(g.deriv)[(m0 + lane) * g.N + n0 + c] = D<T>::store(d);
+            }
+        }
+    }
+}
+
+// ---- host: how a product is cut -------------------------------------------------------------------------------------
+constexpr long FEW_ROWS = 8;           // at most so many rows go to k_few_rows
+constexpr long MOST_K = (1L << 22) - 128;   // 256 padded rows of so many floats still have 32-bit offsets
+
+long k_padded(long k, long e) { return (k * e + 127) / 128 * 128 / e; }
+
+struct Plan {
+    bool large;
+    int tiles_m, tiles_n, steps, per_split, splits;
+};
+
+Plan plan_of(long M, long N, long K, long e)
+{
+    Plan p;
+    p.steps = (int)(k_padded(K, e) * e / 128);
+    const long big = ((M + 255) / 256) * ((N + 255) / 256);
+    p.large = big >= 192;
+    const long b = p.large ? 256 : 128;
+    p.tiles_m = (int)((M + b - 1) / b);
+    p.tiles_n = (int)((N + b - 1) / b);
+    const long tiles = (long)p.tiles_m * p.tiles_n;
+    long splits = p.large ? 1 : 512 / tiles;
+    if (splits > p.steps / 8) splits = p.steps / 8;
+    if (splits < 1) splits = 1;
+    p.per_split = (int)((p.steps + splits - 1) / splits);
+    p.splits = (p.steps + p.per_split - 1) / p.per_split;
+    return p;
+}
+
+size_t round256(size_t n) { return (n + 255) / 256 * 256; }
+size_t partial_bytes(const Plan &p, long M, long N) { return p.splits > 1 ? round256((size_t)p.splits * M * N * 4) : 0; }
+
+bool in_place(const void *p, long ld, long K, long e) { return ppo_aligned(p, 16) && ld * e % 16 == 0 && K * e % 128 == 0 && ld <= MOST_K; }
+
+template <class T> int prep(const void *src, long ld, const void *mul, long R, long C, void *rows, void *cols, float *sums, hipStream_t s)
+{
+    constexpr long e = T::BYTES;
+    PrepArgs a{src, mul, rows, cols, sums, R, C, ld, k_padded(R, e), k_padded(C, e)};
+    // whole k steps in both directions: what lies past the matrix becomes zero
+    const long gr = cols ? (a.Rp + 63) / 64 : (R + 63) / 64, gc = rows ? (a.Cp + 63) / 64 : (C + 63) / 64;
+    PPO_REQUIRE(gr < 65536 && gc < (1L << 31));
+    hipLaunchKernelGGL(k_prep<T>, dim3((unsigned)gc, (unsigned)gr), dim3(256), 0, s, a);
+    return ppo_launch_status();
+}
+
+template <class T> int gemm(GemmArgs g, const Plan &p, hipStream_t s)
+{
+    g.steps = p.steps;
+    g.steps_per_split = p.per_split;
+    g.tiles_m = p.tiles_m;
+    g.tiles_n = p.tiles_n;
+    if (p.splits == 1) g.partial = nullptr;
+    const dim3 grid((unsigned)(p.tiles_m * p.tiles_n), (unsigned)p.splits);
+    if (p.large)
+        hipLaunchKernelGGL((k_gemm<T, 256, 256, 2, 4>), grid, dim3(512), 0, s, g);
+    else
+        hipLaunchKernelGGL((k_gemm<T, 128, 128, 2, 2>), grid, dim3(256), 0, s, g);
+    int rc = ppo_launch_status();
+    if (rc || p.splits == 1) return rc;
+    constexpr long E = 16 / T::BYTES;
+    const long threads = g.M * ((g.N + E - 1) / E);
+    hipLaunchKernelGGL(k_join<T>, dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, s, g, p.splits);
+    return ppo_launch_status();
+}
+
+bool sizes_ok(long rows, long inputs, long outputs, int dtype)
+{
+    // 32-bit workgroup counts and offsets inside a tile; rows are also the k of the weight gradient
+    return dtype_known(dtype) && rows >= 1 && inputs >= 1 && outputs >= 1 && rows <= MOST_K && inputs <= MOST_K && outputs <= MOST_K &&
+           (__int128)rows * outputs < ((__int128)1 << 38) && (__int128)rows * inputs < ((__int128)1 << 38) &&
+           (__int128)inputs * outputs < ((__int128)1 << 38);
+}
+
+bool matrix_ok(const void *p, long ld, long cols, long e) { return p && ppo_aligned(p, e) && ld >= cols && ld <= (1L << 32); }
+
+}  // namespace
+
+extern "C" {
+
+size_t ppo_linear_act_fwd_workspace_bytes(long rows, long inputs, long outputs, int dtype)
+{
+    if (!sizes_ok(rows, inputs, outputs, dtype) || rows <= FEW_ROWS) return 0;
+    const long e = dtype_bytes(dtype), Kp = k_padded(inputs, e);
+    return round256((size_t)rows * Kp * e) + round256((size_t)outputs * Kp * e) + partial_bytes(plan_of(rows, outputs, inputs, e), rows, outputs);
+}
+
+int ppo_linear_act_fwd(const void *x, long x_stride, const void *weight, long weight_stride, const void *bias, const void *residual,
+                       long residual_stride, int dtype, long rows, long inputs, long outputs, int activation, void *y, void *deriv,
+                       void *workspace, size_t workspace_bytes, void *stream)
+{
+    if (rows == 0) return 0;
+    PPO_REQUIRE(sizes_ok(rows, inputs, outputs, dtype));
+    const long e = dtype_bytes(dtype);
+    PPO_REQUIRE(matrix_ok(x, x_stride, inputs, e) && matrix_ok(weight, weight_stride, inputs, e));
+    PPO_REQUIRE(!residual || matrix_ok(residual, residual_stride, outputs, e));
+    PPO_REQUIRE(y && ppo_aligned(y, e) && ppo_aligned(deriv, dtype == PPO_DTYPE_BF16 ? 2 : 4) && ppo_aligned(bias, e) && activation >= PPO_ACT_NONE && activation <= PPO_ACT_SILU);
+    PPO_REQUIRE(workspace_bytes >= ppo_linear_act_fwd_workspace_bytes(rows, inputs, outputs, dtype));
+    PPO_REQUIRE(rows <= FEW_ROWS || (workspace && ppo_aligned(workspace, 16)));
+    hipStream_t s = (hipStream_t)stream;
+    return by_dtype(dtype, [&](auto t) {
+        using T = decltype(t);
+        GemmArgs g{};
+        g.A = x; g.B = weight; g.M = rows; g.N = outputs; g.lda = x_stride * e; g.ldb = weight_stride * e;
+        g.bias = bias; g.residual = residual; g.res_ld = residual_stride; g.out = y; g.deriv = deriv; g.act = activation;
+        if (rows <= FEW_ROWS) {
+            constexpr int COLS = 4;
+            const dim3 grid((unsigned)((outputs + 4 * COLS - 1) / (4 * COLS)));
+            if (rows == 1)
+                hipLaunchKernelGGL((k_few_rows<T, 1, COLS>), grid, dim3(256), 0, s, g, inputs);
+            else if (rows <= 4)
+                hipLaunchKernelGGL((k_few_rows<T, 4, COLS>), grid, dim3(256), 0, s, g, inputs);
+            else
+                hipLaunchKernelGGL((k_few_rows<T, 8, COLS>), grid, dim3(256), 0, s, g, inputs);
+            return ppo_launch_status();
+        }
+        char *ws = reinterpret_cast<char *>(workspace);
+        const long Kp = k_padded(inputs, e);
+        if (!in_place(x, x_stride, inputs, e)) {
+            const int rc = prep<T>(x, x_stride, nullptr, rows, inputs, ws, nullptr, nullptr, s);
+            if (rc) return rc;
+            g.A = ws;
+            g.lda = Kp * e;
+        }
+        ws += round256((size_t)rows * Kp * e);
+        if (!in_place(weight, weight_stride, inputs, e)) {
+            const int rc = prep<T>(weight, weight_stride, nullptr, outputs, inputs, ws, nullptr, nullptr, s);
+            if (rc) return rc;
+            g.B = ws;
+            g.ldb = Kp * e;
+        }
+        ws += round256((size_t)outputs * Kp * e);
+        g.partial = reinterpret_cast<float *>(ws);
+        return gemm<T>(g, plan_of(rows, outputs, inputs, e), s);
+    });
+}
+
+size_t ppo_linear_act_bwd_workspace_bytes(long rows, long inputs, long outputs, int dtype)
+{
+    if (!sizes_ok(rows, inputs, outputs, dtype)) return 0;
+    const long e = dtype_bytes(dtype), Mp = k_padded(rows, e), Np = k_padded(outputs, e);
+    const size_t px = partial_bytes(plan_of(rows, inputs, outputs, e), rows, inputs), pw = partial_bytes(plan_of(outputs, inputs, rows, e), outputs, inputs);
+    return round256((size_t)rows * Np * e) + round256((size_t)outputs * Mp * e) + round256((size_t)inputs * Np * e) +
+           round256((size_t)inputs * Mp * e) + round256((size_t)((Mp + 63) / 64) * outputs * 4) + (px > pw ? px : pw);
+}
+
+int ppo_linear_act_bwd(const void *g_y, long g_stride, const void *x, long x_stride, const void *weight, long weight_stride,
+                       const void *deriv, int dtype, long rows, long inputs, long outputs, void *g_x, void *g_weight, void *g_bias,
+                       void *workspace, size_t workspace_bytes, void *stream)
+{
+    PPO_REQUIRE(sizes_ok(rows, inputs, outputs, dtype));
+    const long e = dtype_bytes(dtype);
+    PPO_REQUIRE(matrix_ok(g_y, g_stride, outputs, e) && matrix_ok(x, x_stride, inputs, e) && matrix_ok(weight, weight_stride, inputs, e));
+    PPO_REQUIRE(ppo_aligned(deriv, dtype == PPO_DTYPE_BF16 ? 2 : 4) && ppo_aligned(g_x, e) && ppo_aligned(g_weight, e) && ppo_aligned(g_bias, e));
+    PPO_REQUIRE(workspace && ppo_aligned(workspace, 16) && workspace_bytes >= ppo_linear_act_bwd_workspace_bytes(rows, inputs, outputs, dtype));
+    if (!g_x && !g_weight && !g_bias) return 0;
+    hipStream_t s = (hipStream_t)stream;
+    return by_dtype(dtype, [&](auto t) {
+        using T = decltype(t);
+        const long Mp = k_padded(rows, e), Np = k_padded(outputs, e);
+        char *ws = reinterpret_cast<char *>(workspace);
+        auto take = [&](size_t n) { char *p = ws; ws += round256(n); return p; };
+        char *u = take((size_t)rows * Np * e), *ut = take((size_t)outputs * Mp * e), *wt = take((size_t)inputs * Np * e), *xt = take((size_t)inputs * Mp * e);
+        float *sums = reinterpret_cast<float *>(take((size_t)((Mp + 63) / 64) * outputs * 4));
+        float *partial = reinterpret_cast<float *>(ws);
+        const bool as_is = !deriv && in_place(g_y, g_stride, outputs, e);
+        const bool want_rows = g_x && !as_is;
+        int rc = 0;
+        if (want_rows || g_weight || g_bias)
+            rc = prep<T>(g_y, g_stride, deriv, rows, outputs, want_rows ? u : nullptr, g_weight ? ut : nullptr, g_bias ? sums : nullptr, s);
+        if (!rc && g_bias) {
+            const long tiles = ((g_weight ? Mp : rows) + 63) / 64;
+            hipLaunchKernelGGL(k_bias_grad<T>, dim3((unsigned)((outputs + 63) / 64)), dim3(256), 0, s, sums, tiles, outputs,
+                               reinterpret_cast<typename T::raw *>(g_bias));
+            rc = ppo_launch_status();
+        }
+        if (!rc && g_x) {
+            rc = prep<T>(weight, weight_stride, nullptr, outputs, inputs, nullptr, wt, nullptr, s);
+            GemmArgs g{};
+            g.A = as_is ? g_y : u; g.lda = (as_is ? g_stride : Np) * e; g.B = wt; g.ldb = Np * e;
+            g.M = rows; g.N = inputs; g.out = g_x; g.act = PPO_ACT_NONE; g.partial = partial;
+            if (!rc) rc = gemm<T>(g, plan_of(rows, inputs, outputs, e), s);
+        }
+        if (!rc && g_weight) {
+            rc = prep<T>(x, x_stride, nullptr, rows, inputs, nullptr, xt, nullptr, s);
+            GemmArgs g{};
+            g.A = ut; g.lda = Mp * e; g.B = xt; g.ldb = Mp * e;
+            g.M = outputs; g.N = inputs; g.out = g_weight; g.act = PPO_ACT_NONE; g.partial = partial;
+            if (!rc) rc = gemm<T>(g, plan_of(outputs, inputs, rows, e), s);
+        }
+        return rc;
+    });
+}
+
+}  // extern "C"

@@ -935,3 +935,120 @@ def preference_loss(chosen_lp, rejected_lp, ref_chosen_lp=None, ref_rejected_lp=
                                                           rejected_mask, beta, kind, label_smoothing, average, want_grad=need)
     loss = _PairLoss.apply(chosen_lp, rejected_lp, out2[0], g_c, g_r) if need else out2[0]
     return loss, out2[1], rewards
+
+
+# ---- linear layers of any size with their epilogue (csrc/linear.hip) ----------------------------------------------------
+ACTIVATIONS = {"none": 0, "tanh": 1, "relu": 2, "gelu": 3, "silu": 4}   # include/ppo_amd.h: PPO_ACT_*
+_LINEAR_MOST = (1 << 22) - 128
+
+
+def _deriv_dtype(dtype):
+    return torch.float16 if dtype == torch.bfloat16 else torch.float32
+
+
+def _matrix(t):
+    """(rows, matrix whose rows are contiguous and do not overlap, its row stride) of [..., columns]"""
+    m = t if t.dim() == 2 else t.reshape(-1, t.shape[-1])
+    if (m.shape[1] > 1 and m.stride(1) != 1) or (m.shape[0] > 1 and m.stride(0) < m.shape[1]):
+        m = m.contiguous()
+    return m.shape[0], m, max(m.stride(0), m.shape[1])
+
+
+def _linear_inputs(name, x, weight, others):
+    _need(x.dtype in _DTYPES, f"{name}: x is float32, bfloat16 or float16, not {x.dtype}")
+    _need(isinstance(weight, torch.Tensor) and weight.dim() == 2 and x.dim() >= 1 and x.shape[-1] == weight.shape[1],
+          f"{name}: x [..., inputs] and weight [outputs, inputs]")
+    _need(weight.shape[0] >= 1 and weight.shape[1] >= 1, f"{name}: at least one input and one output")
+    n, k = weight.shape
+    for what, t, shape in others:
+        _need(t is None or (isinstance(t, torch.Tensor) and tuple(t.shape) == tuple(shape)), f"{name}: {what} is not {tuple(shape)}")
+    for what, t in [("weight", weight)] + [(what, t) for what, t, _ in others]:
+        dtype = _deriv_dtype(x.dtype) if what == "deriv" else x.dtype
+        _need(t is None or t.dtype == dtype, f"{name}: {what} is {dtype} where x is {x.dtype}")
+    rows = x.numel() // k
+    _need(max(rows, n, k) <= _LINEAR_MOST and max(rows * n, rows * k, n * k) < 1 << 38, f"{name}: sizes beyond {_LINEAR_MOST} or 2^38 elements")
+    _device_tensors(name, x, weight, *[t for _, t, _ in others])
+
+
+@_on_tensor_device
+def linear_act_fwd(x, weight, bias=None, activation="none", residual=None, want_deriv=False):
+    """ppo_linear_act_fwd: (y, deriv) with y = act(x W^T + bias) + residual; activation "none", "tanh", "relu", "gelu"
+    (z Phi(z)) or "silu".  x [..., inputs], weight [outputs, inputs], residual [..., outputs], all f32, bf16 or f16; sums in
+    f32.  deriv (want_deriv, and an activation) is act'(z) for linear_act_bwd, f16 for bf16 layers and f32 for others, else None."""
+    lib = _lib.load()
+    name = "linear_act"
+    _need(activation in ACTIVATIONS, f"{name}: activation is one of {sorted(ACTIVATIONS)}")
+    _need(isinstance(weight, torch.Tensor) and weight.dim() == 2, f"{name}: weight is [outputs, inputs]")
+    n, k = weight.shape
+    shape = (*x.shape[:-1], n)
+    _linear_inputs(name, x, weight, [("bias", bias, (n,)), ("residual", residual, shape)])
+    rows, xm, xs = _matrix(x)
+    _, wm, ws_ = _matrix(weight)
+    bias = None if bias is None else bias.contiguous()
+    rm, rs = None, 0
+    if residual is not None:
+        _, rm, rs = _matrix(residual)
+    y = torch.empty(shape, dtype=x.dtype, device=x.device)
+    deriv = torch.empty(shape, dtype=_deriv_dtype(x.dtype), device=x.device) if want_deriv and activation != "none" else None
+    if rows == 0:
+        return y, deriv
+    dt = _DTYPES[x.dtype]
+    nws = lib.ppo_linear_act_fwd_workspace_bytes(rows, k, n, dt)
+    ws = torch.empty(nws, dtype=torch.uint8, device=x.device) if nws else None
+    rc = lib.ppo_linear_act_fwd(xm.data_ptr(), xs, wm.data_ptr(), ws_, _ptr(bias), _ptr(rm), rs, dt, rows, k, n, ACTIVATIONS[activation],
+                                y.data_ptr(), _ptr(deriv), _ptr(ws), nws, _stream())
+    _lib.check(rc, "ppo_linear_act_fwd")
+    return y, deriv
+
+
+@_on_tensor_device
+def linear_act_bwd(g, x, weight, deriv=None, want_input=True, want_weight=True, want_bias=True):
+    """ppo_linear_act_bwd: (g_x, g_weight, g_bias), None where not wanted, for the gradient g of linear_act_fwd's y and the
+    deriv it returned: with u = g deriv, g_x = u W, g_weight = u^T x, g_bias = column sums of u.  (The residual's gradient
+    is g itself.)"""
+    lib = _lib.load()
+    name = "linear_act_bwd"
+    _need(isinstance(x, torch.Tensor) and isinstance(weight, torch.Tensor) and weight.dim() == 2, f"{name}: x [..., inputs] and weight [outputs, inputs]")
+    n, k = weight.shape
+    shape = (*x.shape[:-1], n)
+    _linear_inputs(name, x, weight, [("g", g, shape), ("deriv", deriv, shape)])
+    rows, gm, gs = _matrix(g)
+    _, xm, xs = _matrix(x)
+    _, wm, ws_ = _matrix(weight)
+    make = lambda want, s: torch.empty(s, dtype=x.dtype, device=x.device) if want else None  # noqa: E731
+    g_x, g_w, g_b = make(want_input, x.shape), make(want_weight, (n, k)), make(want_bias, (n,))
+    if rows == 0:
+        return g_x, None if g_w is None else g_w.zero_(), None if g_b is None else g_b.zero_()
+    if deriv is not None:
+        deriv = deriv.contiguous()
+    dt = _DTYPES[x.dtype]
+    nws = lib.ppo_linear_act_bwd_workspace_bytes(rows, k, n, dt)
+    ws = torch.empty(nws, dtype=torch.uint8, device=x.device)
+    rc = lib.ppo_linear_act_bwd(gm.data_ptr(), gs, xm.data_ptr(), xs, wm.data_ptr(), ws_, _ptr(deriv), dt, rows, k, n, _ptr(g_x), _ptr(g_w),
+                                _ptr(g_b), ws.data_ptr(), nws, _stream())
+    _lib.check(rc, "ppo_linear_act_bwd")
+    return g_x, g_w, g_b
+
+
+class _LinearAct(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, activation, residual):
+        y, deriv = linear_act_fwd(x, weight, bias, activation, residual, want_deriv=True)
+        ctx.save_for_backward(x, weight, deriv)
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        x, weight, deriv = ctx.saved_tensors
+        want_x, want_w, want_b, _, want_r = ctx.needs_input_grad
+        g_x, g_w, g_b = linear_act_bwd(g, x, weight, deriv, want_x, want_w, want_b) if want_x or want_w or want_b else (None, None, None)
+        return g_x, g_w, g_b, None, g if want_r else None
+
+
+def linear_act(x, weight, bias=None, activation="none", residual=None):
+    """y of linear_act_fwd, differentiable with respect to x, weight, bias and residual.  (ops.linear, for the agents'
+    layers of at most 64 x 64, keeps their f32 library product.)"""
+    if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in (x, weight, bias, residual)):
+        return _LinearAct.apply(x, weight, bias, activation, residual)
+    return linear_act_fwd(x, weight, bias, activation, residual)[0]

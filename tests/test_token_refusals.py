@@ -78,3 +78,43 @@ def test_c_entries_refuse():
     for kw in ({"c": None}, {"c": p + 2}, {"s": -1}, {"L": -1}, {"b": 0}, {"b": 1 << 29}, {"kind": 3}, {"beta": 0.0}, {"beta": float("nan")}, {"eps": 0.5},
                {"out": None}, {"rew": None}, {"ws": None}, {"nws": n - 1}):
         assert pref(**kw) == INVALID, kw
+
+
+def test_linear_wrapper_refuses():
+    x, w = z(3, 5), z(7, 5)
+    for args, kw in (
+            ((x, z(7, 4)), {}), ((x, z(7)), {}), ((x, None), {}), ((x.double(), w.double()), {}), ((x, w.half()), {}), ((x, w, z(5)), {}), ((x, w, z(7).half()), {}),
+            ((x, w, None, "gelu2"), {}), ((x, w, None, "none", z(3, 5)), {}), ((x, w, None, "none", z(3, 7).half()), {}), ((x, z(0, 5)), {}), ((z(3, 0), z(7, 0)), {}),
+            ((z(1, 1).expand(1 << 22, 1), z(1, 1)), {}), ((x, w), {})):
+        with pytest.raises(BAD):
+            ops.linear_act_fwd(*args, **kw)
+    y = z(3, 7)
+    for args, kw in (((z(3, 6), x, w), {}), ((y, x, w, z(3, 6)), {}), ((y.half(), x, w), {}), ((y, x, w, y.half()), {}), ((y, x, z(7)), {}), ((y, None, w), {}),
+                     ((y, x, w), {})):
+        with pytest.raises(BAD):
+            ops.linear_act_bwd(*args, **kw)
+    h = torch.bfloat16
+    with pytest.raises(BAD, match="deriv is torch.float16"):
+        ops.linear_act_bwd(z(3, 7, dtype=h), z(3, 5, dtype=h), z(7, 5, dtype=h), z(3, 7, dtype=h))
+
+
+def test_linear_c_entries_refuse():
+    lib = _lib.load()
+    buf = (ctypes.c_char * 4096)()
+    p = (ctypes.addressof(buf) + 63) // 64 * 64
+    n = lib.ppo_linear_act_fwd_workspace_bytes(16, 8, 8, 0)
+    assert lib.ppo_linear_act_fwd_workspace_bytes(8, 8, 8, 0) == 0 and n > 0
+    fwd = lambda x=p, xs=8, w=p, ws_=8, b=p, r=p, rs=8, dt=0, M=16, K=8, N=8, act=1, y=p, d=p, ws=p, nws=n: lib.ppo_linear_act_fwd(  # noqa: E731
+        x, xs, w, ws_, b, r, rs, dt, M, K, N, act, y, d, ws, nws, None)
+    assert fwd(M=0) == 0
+    for kw in ({"x": None}, {"x": p + 2}, {"xs": 7}, {"w": None}, {"ws_": 7}, {"w": p + 1}, {"b": p + 2}, {"r": p + 2}, {"rs": 7}, {"dt": 3}, {"dt": -1}, {"M": -1},
+               {"K": 0}, {"N": 0}, {"M": 1 << 22}, {"K": 1 << 22, "xs": 1 << 22, "ws_": 1 << 22}, {"N": 1 << 22}, {"act": 5}, {"act": -1}, {"y": None}, {"y": p + 2},
+               {"d": p + 2}, {"ws": None}, {"ws": p + 8}, {"nws": n - 1}):
+        assert fwd(**kw) == INVALID, kw
+    n = lib.ppo_linear_act_bwd_workspace_bytes(16, 8, 8, 0)
+    bwd = lambda g=p, gs=8, x=p, xs=8, w=p, ws_=8, d=p, dt=0, M=16, K=8, N=8, gx=p, gw=p, gb=p, ws=p, nws=n: lib.ppo_linear_act_bwd(  # noqa: E731
+        g, gs, x, xs, w, ws_, d, dt, M, K, N, gx, gw, gb, ws, nws, None)
+    for kw in ({"g": None}, {"g": p + 2}, {"gs": 7}, {"x": None}, {"xs": 7}, {"w": None}, {"ws_": 7}, {"d": p + 2}, {"dt": 3}, {"M": 0}, {"K": 0}, {"N": 0}, {"M": 1 << 22},
+               {"gx": p + 2}, {"gw": p + 1}, {"gb": p + 2}, {"ws": None}, {"ws": p + 8}, {"nws": n - 1}):
+        assert bwd(**kw) == INVALID, kw
+    assert bwd(gx=None, gw=None, gb=None) == 0

@@ -90,5 +90,6 @@ def linear(x, weight, bias=None, activation="none", residual=None):
     if bias is not None:
         z = z + bias.double()
     f = torch.nn.functional
-    y = {"none": lambda v: v, "tanh": torch.tanh, "relu": f.relu, "gelu": f.gelu, "silu": f.silu}[activation](z)
+    gelu = lambda v: v * 0.5 * torch.erfc(v * -math.sqrt(0.5))  # noqa: E731  (1 + erf loses its left tail even in 64 bits)
+    y = {"none": lambda v: v, "tanh": torch.tanh, "relu": f.relu, "gelu": gelu, "silu": f.silu}[activation](z)
     return y if residual is None else y + residual.double()
