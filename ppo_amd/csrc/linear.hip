@@ -41,14 +41,33 @@ template <class T> __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4
 }
 
 // ---- activations: value and derivative ------------------------------------------------------------------------------
-__device__ __forceinline__ void activate(int act, float z, float &y, float &d)
+// To f32's accuracy for f32 layers; for 16-bit ones to a few 1e-7 of max(1, |value|), far below their half steps, in a
+// quarter of the instructions: the hardware's exp2 and reciprocal, and for the normal distribution's tail,
+// P(> a) = e^(-a^2 / 2) h(1 / (1 + 0.38 a / sqrt 2)), whose exponential is the density that the derivative needs as well,
+// a polynomial h of degree 7, fitted by Lawson's iteration: 1e-6 of the tail as far as f16 and bf16 results go.  (With
+// the library's functions the gelu layer's forward product took 1284 us, and takes 969 without an activation.)
+__device__ __forceinline__ float exp_fast(float x) { return __builtin_amdgcn_exp2f(x * 1.442695041f); }
+
+template <bool FAST> __device__ __forceinline__ void activate(int act, float z, float &y, float &d)
 {
     switch (act) {
     case PPO_ACT_TANH: {
-        const float e = expf(-2.0f * fabsf(z)), t = (1.0f - e) / (1.0f + e);
-        y = fabsf(z) < 0.1f ? tanhf(z) : copysignf(t, z);
-        d = 4.0f * e / ((1.0f + e) * (1.0f + e));           // 1 - tanh^2 without its cancellation
-        if (z != z) y = d = z;
+        const float a = fabsf(z);
+        float e, r;
+        if constexpr (FAST) {
+            e = exp_fast(-2.0f * a);
+            r = __builtin_amdgcn_rcpf(1.0f + e);
+        } else {
+            e = expf(-2.0f * a);
+            r = 1.0f / (1.0f + e);
+        }
+        float t = (1.0f - e) * r;
+        if constexpr (FAST)
+            t = a < 0.02f ? a - a * a * a * (1.0f / 3) : t;   // (what is left out: 2 a^5 / 15)
+        else if (a < 0.1f)
+            t = tanhf(a);
+        y = copysignf(t, z);
+        d = 4.0f * e * r * r;                               // 1 - tanh^2 without its cancellation
         break;
     }
     case PPO_ACT_RELU:
@@ -56,15 +75,34 @@ __device__ __forceinline__ void activate(int act, float z, float &y, float &d)
         d = z > 0.0f ? 1.0f : 0.0f;
         break;
     case PPO_ACT_GELU: {
-        const float phi = 0.5f * erfcf(-0.70710678f * z);   // P(normal < z), without cancellation in the left tail
-        y = z * phi;
-        if (z == -INFINITY) y = 0.0f;
-        d = phi + z * expf(-0.5f * z * z) * 0.3989422804f;
-        if (fabsf(z) == INFINITY) d = z > 0.0f ? 1.0f : 0.0f;
+        float phi, g;                                       // the normal distribution's P(< z), and sqrt(2 pi) times its density
+        if constexpr (FAST) {
+            const float a = fabsf(z), t = __builtin_amdgcn_rcpf(__builtin_fmaf(a, 0.38f * 0.70710678f, 1.0f));
+            g = __builtin_amdgcn_exp2f(a * a * -0.7213475204f);
+            float q = -0.0627071038f;
+            q = __builtin_fmaf(q, t, 0.168012768f);
+            q = __builtin_fmaf(q, t, -0.0349497572f);
+            q = __builtin_fmaf(q, t, 0.123912774f);
+            q = __builtin_fmaf(q, t, 0.0902986899f);
+            q = __builtin_fmaf(q, t, 0.108288437f);
+            q = __builtin_fmaf(q, t, 0.107143678f);
+            q = q * t * g;
+            phi = z > 0.0f ? 1.0f - q : q;
+        } else {
+            phi = 0.5f * erfcf(-0.70710678f * z);           // no cancellation in the left tail
+            g = expf(-0.5f * z * z);
+        }
+        const bool far = fabsf(z) > 20.0f;                  // (NaN: near)
+        y = far ? fmaxf(z, 0.0f) : z * phi;
+        d = far ? (z > 0.0f ? 1.0f : 0.0f) : __builtin_fmaf(z * 0.3989422804f, g, phi);
         break;
     }
     case PPO_ACT_SILU: {
-        const float s = 1.0f / (1.0f + expf(-z));
+        float s;
+        if constexpr (FAST)
+            s = __builtin_amdgcn_rcpf(1.0f + exp_fast(-z));
+        else
+            s = 1.0f / (1.0f + expf(-z));
         y = z == -INFINITY ? 0.0f : z * s;
         d = fabsf(z) == INFINITY ? s : s * (1.0f + z * (1.0f - s));
         break;
@@ -222,7 +260,7 @@ template <class T> __device__ __forceinline__ void finish(const GemmArgs &g, lon
 {
     using raw = typename T::raw;
     if (g.bias) z += T::load(reinterpret_cast<const raw *>(g.bias)[n]);
-    activate(g.act, z, y, d);
+    activate<T::BYTES == 2>(g.act, z, y, d);
     if (g.residual) y += T::load(reinterpret_cast<const raw *>(g.residual)[m * g.res_ld + n]);
 }
 
@@ -242,7 +280,7 @@ template <class T, int CNT> __device__ __forceinline__ void epilogue(const GemmA
             if (g.residual) load16<T>(reinterpret_cast<const raw *>(g.residual) + m * g.res_ld + n + q, r);
 #pragma unroll
             for (int j = 0; j < E; ++j) {
-                activate(g.act, g.bias ? z[q + j] + b[j] : z[q + j], y[j], d[j]);
+                activate<T::BYTES == 2>(g.act, g.bias ? z[q + j] + b[j] : z[q + j], y[j], d[j]);
                 if (g.residual) y[j] += r[j];
             }
             store16<T>(out + q, y);
@@ -261,9 +299,18 @@ template <class T, int CNT> __device__ __forceinline__ void epilogue(const GemmA
     }
 }
 
-// swizzles: which 16-byte piece of an LDS row holds piece c of the operand's row
-__device__ __forceinline__ int swizzle_a(int row) { return (row & 7) ^ ((row >> 3) & 1); }
-__device__ __forceinline__ int swizzle_b(int row) { return ((row & 3) | ((row >> 2) & 4)) ^ ((row >> 5) & 1); }
+// Swizzles: piece c (16 bytes) of a row of 128 bytes lies at c ^ f(row) in LDS.  A ds_read_b128 is served 16 lanes a cycle
+// from 64 banks: lanes {0-3, 12-15, 20-23, 24-27}, {4-11, 16-19, 28-31} and these + 32.  In a fragment read lane l wants
+// piece l / 16 of the fragment's row l % 16, so with f = a r1 ^ b r2 ^ d r3 (r1 .. r3 the row's bits that are lane bits 1 .. 3)
+// the lanes of a group fall into different places (row & 1, c ^ f) if 0, b ^ d, 1 ^ b and 1 ^ d differ modulo a: (4, 2, 3).
+// The f32 fragments' pieces are two apart, which makes that 0, b ^ d, 2 ^ b, 2 ^ d: (4, 1, 3).  (f = row & 7 costs twice the
+// cycles a read.)
+template <int BYTES> __device__ __forceinline__ int swizzle(int r1, int r2, int r3)
+{
+    return (r1 & 1) * 4 ^ (r2 & 1) * (BYTES == 2 ? 2 : 1) ^ (r3 & 1) * 3;
+}
+template <int BYTES> __device__ __forceinline__ int swizzle_a(int row) { return swizzle<BYTES>(row >> 1, row >> 2, row >> 3); }
+template <int BYTES> __device__ __forceinline__ int swizzle_b(int row) { return swizzle<BYTES>(row >> 1, row >> 4, row >> 5); }
 
 // 64 lanes bring 16 bytes each from rsrc[voff + soff] to LDS at lds + 16 lane.  In asm because the compiler's own form of
 // this load makes every LDS read wait for all of them; it has no destination register, and the loop below waits itself.
@@ -283,11 +330,11 @@ __device__ __forceinline__ u32x4 buffer_of(const void *p, long bytes)
 template <class T, int BM, int BN, int WAVES_M, int WAVES_N>
 __global__ void __launch_bounds__(64 * WAVES_M * WAVES_N) k_gemm(GemmArgs g)
 {
-    constexpr int WAVES = WAVES_M * WAVES_N, WM = BM / WAVES_M, WN = BN / WAVES_N, MI = WM / 16, NI = WN / 16;
+    constexpr int WAVES = WAVES_M * WAVES_N, WM = BM / WAVES_M, WN = BN / WAVES_N, MI = WM / 16, NI = 4;
     static_assert(WN == 64 && MI * 16 * WAVES_M == BM, "a lane's 16 neighbouring n need 64 columns a wave");
     constexpr int LA = BM / 8 / WAVES, LB = BN / 8 / WAVES;          // loads a wave and stage (8 rows each)
-    constexpr int STAGE = (BM + BN) * 128;
-    __shared__ __align__(1024) char lds[2 * STAGE];
+    constexpr int A_STAGE = BM * 128, B_STAGE = BN * 128, B_AT = 3 * A_STAGE;
+    __shared__ __align__(1024) char lds[3 * A_STAGE + 2 * B_STAGE];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave / WAVES_N, wn = wave % WAVES_N;
 
@@ -311,27 +358,31 @@ __global__ void __launch_bounds__(64 * WAVES_M * WAVES_N) k_gemm(GemmArgs g)
 #pragma unroll
     for (int i = 0; i < LA; ++i) {
         const int row = (i * WAVES + wave) * 8 + lane / 8, have = row < rows_a ? row : (int)rows_a - 1;   // rows past the end repeat the last
-        va[i] = (uint32_t)have * (uint32_t)g.lda + ((lane % 8) ^ swizzle_a(row)) * 16;
+        va[i] = (uint32_t)have * (uint32_t)g.lda + ((lane % 8) ^ swizzle_a<T::BYTES>(row)) * 16;
     }
 #pragma unroll
     for (int i = 0; i < LB; ++i) {
         const int row = (i * WAVES + wave) * 8 + lane / 8, have = row < rows_b ? row : (int)rows_b - 1;
-        vb[i] = (uint32_t)have * (uint32_t)g.ldb + ((lane % 8) ^ swizzle_b(row)) * 16;
+        vb[i] = (uint32_t)have * (uint32_t)g.ldb + ((lane % 8) ^ swizzle_b<T::BYTES>(row)) * 16;
     }
     const uint32_t base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds;
-    auto stage = [&](int s) {
-        const uint32_t to = base + (s & 1) * STAGE + wave * 1024;
-        const int k = s * 128;
+    // load i of a stage's A or B to the place that begins at `to`
+    auto load_a = [&](int s, int to, int i) { load_lds(ra, va[i], s * 128, base + wave * 1024 + to + i * WAVES * 1024); };
+    auto load_b = [&](int s, int to, int i) { load_lds(rb, vb[i], s * 128, base + wave * 1024 + B_AT + to + i * WAVES * 1024); };
+    auto stage_a = [&](int s, int to) {
 #pragma unroll
-        for (int i = 0; i < LA; ++i) load_lds(ra, va[i], k, to + i * WAVES * 1024);
+        for (int i = 0; i < LA; ++i) load_a(s, to, i);
+    };
+    auto stage_b = [&](int s, int to) {
 #pragma unroll
-        for (int i = 0; i < LB; ++i) load_lds(rb, vb[i], k, to + BM * 128 + i * WAVES * 1024);
+        for (int i = 0; i < LB; ++i) load_b(s, to, i);
     };
 
-    // fragment reads: lane q = lane % 16 reads k piece lane / 16 of row ... of A: 16 mi + q, of B: 16 (q / 4) + 4 ni + q % 4
+    // fragment reads: lane q = lane % 16 reads k piece lane / 16 of A's row q and of B's row n(q) = 16 (q / 4) + q % 4 (+ 4 j);
+    // a lane's results are those of B's fragment rows 4 (lane / 16) + e, e < 4, which n() makes 16 neighbours over the j
     const int q = lane & 15, kg = lane >> 4;
     const int row_a = wm * WM + q, row_b = wn * WN + (q >> 2) * 16 + (q & 3);
-    const int pa = row_a * 128, pb = BM * 128 + row_b * 128, xa = swizzle_a(row_a), xb = swizzle_b(row_b);
+    const int pa = row_a * 128, pb = B_AT + row_b * 128, xa = swizzle_a<T::BYTES>(row_a), xb = swizzle_b<T::BYTES>(row_b);
 
     f32x4 acc[MI][NI];
 #pragma unroll
@@ -341,30 +392,111 @@ __global__ void __launch_bounds__(64 * WAVES_M * WAVES_N) k_gemm(GemmArgs g)
     ppo_net::Bf16Select sel;
     if constexpr (T::BYTES == 4) sel.init();
 
-    if (s0 < s1) stage(s0);
-    for (int s = s0; s < s1; ++s) {
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-        __builtin_amdgcn_s_barrier();                       // stage s has landed for every wave, and nobody reads the other one
-        asm volatile("" ::: "memory");
-        if (s + 1 < s1) stage(s + 1);
-        const char *at = lds + (s & 1) * STAGE;
-        if constexpr (T::BYTES == 2) {
+    if constexpr (T::BYTES == 2) {
+        // A stage is two halves of 32 k.  While the matrix cores work on one half's fragments the next half's are read, so
+        // no product waits for LDS, and the barrier between two stages lies between two runs of products whose operands
+        // are in registers already: behind it this stage's places are free (its second half has been read by all) and the
+        // next stage has landed.  160 KB hold three stages of A and two of B: B's loads have one stage's time to arrive,
+        // A's, which go out behind them, two.  (What bounds this loop is the way from L2 and the last-level cache: without
+        // the products it takes 605 of its 790 us for 8192 x 4096 x 16384; with two places for both, sent out together, a
+        // load had to arrive within 1.5 us and the loop waited for it.  Rows of 64 bytes in a ring of five stages double
+        // the requests and are slower still.)
+        struct Half { u32x4 a[MI], b[NI]; };
+        Half h0, h1;
+        // one read of a half's fragments, in the order in which its products want them
+        auto fetch = [&](int at_a, int at_b, int half, Half &h, int r) {
+            const int c = half * 4 + kg;
+            if (r < NI)
+                h.b[r] = *reinterpret_cast<const u32x4 *>(lds + at_b + pb + r * 512 + (c ^ xb) * 16);
+            else
+                h.a[r - NI] = *reinterpret_cast<const u32x4 *>(lds + at_a + pa + (r - NI) * 2048 + (c ^ xa) * 16);
+        };
+        // a half's products one by one, and between them, in this order, the reads of the next half and the loads: left to
+        // itself the compiler sends all loads first, which blocks the wave, and with it its products, until the address
+        // unit has taken them
+        auto work = [&](const Half &now, auto &&between) {
+            constexpr int P = MI * NI;
 #pragma unroll
-            for (int ks = 0; ks < 2; ++ks) {
-                u32x4 fa[MI], fb[NI];
-                const int ca = ((ks * 4 + kg) ^ xa) * 16, cb = ((ks * 4 + kg) ^ xb) * 16;
-#pragma unroll
-                for (int j = 0; j < NI; ++j) fb[j] = *reinterpret_cast<const u32x4 *>(at + pb + j * 512 + cb);
-#pragma unroll
-                for (int i = 0; i < MI; ++i) fa[i] = *reinterpret_cast<const u32x4 *>(at + pa + i * 2048 + ca);
-#pragma unroll
-                for (int i = 0; i < MI; ++i)
-#pragma unroll
-                    for (int j = 0; j < NI; ++j) acc[i][j] = mfma<T>(fb[j], fa[i], acc[i][j]);
+            for (int p = 0; p < P; ++p) {
+                const int i = p / NI, j = p % NI;
+                acc[i][j] = mfma<T>(now.b[j], now.a[i], acc[i][j]);
+                __builtin_amdgcn_sched_barrier(0);
+                between(p, P);
+                __builtin_amdgcn_sched_barrier(0);
             }
+        };
+        constexpr int R = MI + NI;                          // a read to every other product, the last few without
+        static_assert(2 * R <= MI * NI, "room for the reads");
+        const int n = s1 - s0;
+        int a_now = 0, a_next = A_STAGE, b_now = 0, b_next = B_STAGE;
+        auto turn = [&](int s, auto left) {                 // left: stages behind this one, 3 for three or more
+            work(h0, [&](int p, int) {
+                if (p % 2 == 0 && p / 2 < R) fetch(a_now, b_now, 1, h1, p / 2);
+            });
+            if constexpr (left() >= 2)
+                asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(LA) : "memory");   // A of stage s + 2 may be on its way
+            else
+                asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
+            __builtin_amdgcn_sched_barrier(0);
+            work(h1, [&](int p, int P) {
+                constexpr int NL = LB + LA;
+                const int l = p * NL / P;
+                if (l != (p + 1) * NL / P) {
+                    if constexpr (left() >= 2) {
+                        if (l < LB) load_b(s0 + s + 2, b_now, l);
+                    }
+                    if constexpr (left() >= 3) {
+                        if (l >= LB) load_a(s0 + s + 3, a_now, l - LB);
+                    }
+                }
+                if constexpr (left() >= 1) {
+                    if (p % 2 == 0 && p / 2 < R) fetch(a_next, b_next, 0, h0, p / 2);
+                }
+            });
+            const int was = b_now;
+            b_now = b_next;
+            b_next = was;
+            a_now = a_next;
+            a_next = a_next == 2 * A_STAGE ? 0 : a_next + A_STAGE;
+        };
+        stage_a(s0, 0);
+        stage_b(s0, 0);
+        if (n > 1) {
+            stage_a(s0 + 1, A_STAGE);
+            stage_b(s0 + 1, B_STAGE);
+        }
+        if (n > 2) {
+            stage_a(s0 + 2, 2 * A_STAGE);
+            asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * LA + LB) : "memory");
+        } else if (n > 1) {
+            asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LA + LB) : "memory");
         } else {
-            u32x4 fb[NI][3];
-            const int ca0 = ((2 * kg) ^ xa) * 16, ca1 = ((2 * kg + 1) ^ xa) * 16, cb0 = ((2 * kg) ^ xb) * 16, cb1 = ((2 * kg + 1) ^ xb) * 16;
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        }
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+#pragma unroll
+        for (int r = 0; r < R; ++r) fetch(0, 0, 0, h0, r);
+        int s = 0;
+        for (; s + 3 < n; ++s) turn(s, std::integral_constant<int, 3>{});
+        if (n > 2) turn(s++, std::integral_constant<int, 2>{});
+        if (n > 1) turn(s++, std::integral_constant<int, 1>{});
+        turn(s, std::integral_constant<int, 0>{});
+    } else {
+        stage_a(s0, 0);
+        stage_b(s0, 0);
+        for (int s = s0; s < s1; ++s) {
+            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+            __builtin_amdgcn_s_barrier();                   // stage s has landed for every wave, and nobody reads the other one
+            asm volatile("" ::: "memory");
+            const int now = (s - s0) & 1;
+            if (s + 1 < s1) {
+                stage_a(s + 1, (now ^ 1) * A_STAGE);
+                stage_b(s + 1, (now ^ 1) * B_STAGE);
+            }
+            const char *at_a = lds + now * A_STAGE, *at_b = lds + now * B_STAGE;
             auto split = [&](const char *p0, const char *p1, u32x4(&f)[3]) {
                 const f32x4 lo = *reinterpret_cast<const f32x4 *>(p0), hi = *reinterpret_cast<const f32x4 *>(p1);
 #pragma unroll
@@ -376,12 +508,14 @@ __global__ void __launch_bounds__(64 * WAVES_M * WAVES_N) k_gemm(GemmArgs g)
                     f[2][e] = w2;
                 }
             };
+            const int c = 2 * kg, ca0 = (c ^ xa) * 16, ca1 = ((c + 1) ^ xa) * 16, cb0 = (c ^ xb) * 16, cb1 = ((c + 1) ^ xb) * 16;
+            u32x4 fb[NI][3];
 #pragma unroll
-            for (int j = 0; j < NI; ++j) split(at + pb + j * 512 + cb0, at + pb + j * 512 + cb1, fb[j]);
+            for (int j = 0; j < NI; ++j) split(at_b + pb + j * 512 + cb0, at_b + pb + j * 512 + cb1, fb[j]);
 #pragma unroll
             for (int i = 0; i < MI; ++i) {
                 u32x4 fa[3];
-                split(at + pa + i * 2048 + ca0, at + pa + i * 2048 + ca1, fa);
+                split(at_a + pa + i * 2048 + ca0, at_a + pa + i * 2048 + ca1, fa);
 #pragma unroll
                 for (int t = 0; t < 6; ++t) {
                     constexpr int PA[6] = {0, 2, 1, 0, 1, 0}, PB[6] = {2, 0, 1, 1, 0, 0};   // small terms first
@@ -392,9 +526,9 @@ __global__ void __launch_bounds__(64 * WAVES_M * WAVES_N) k_gemm(GemmArgs g)
         }
     }
 
-    // acc[i][j][e] is C[m0 + wm WM + 16 i + q][n0 + wn WN + 16 kg + 4 j + e].  One row of tiles at a time in a loop, the
+    // acc[i][j][e] is C[m0 + wm WM + 16 i + q][n0 + wn WN + 16 kg + 4 j + e].  One row of products at a time in a loop, the
     // others moving down a place: unrolled, the activations' code would be there MI times (90 KB of it)
-    const long n = n0 + wn * WN + kg * 16;
+    const long n1 = n0 + wn * WN + kg * 16;
     long m = m0 + wm * WM + q;
 #pragma clang loop unroll(disable)
     for (int i = 0; i < MI; ++i, m += 16) {
@@ -408,22 +542,18 @@ __global__ void __launch_bounds__(64 * WAVES_M * WAVES_N) k_gemm(GemmArgs g)
 #pragma unroll
             for (int j = 0; j < NI; ++j) acc[k][j] = acc[k + 1][j];
         if (g.partial) {
-            if (m < g.M && n < g.N) {
-                float *p = g.partial + ((long)blockIdx.y * g.M + m) * g.N + n;
-                if (n + 16 <= g.N) {
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const float w[4] = {z[4 * j], z[4 * j + 1], z[4 * j + 2], z[4 * j + 3]};
-                        store16<F32>(p + 4 * j, w);
-                    }
+            if (m < g.M && n1 < g.N) {
+                float *p = g.partial + ((long)blockIdx.y * g.M + m) * g.N + n1;
+                if (n1 + 16 <= g.N) {
+                    store_n<F32, 16>(p, z);
                 } else {
 #pragma unroll
-                    for (int j = 0; j < 16; ++j)
-                        if (n + j < g.N) p[j] = z[j];
+                    for (int e = 0; e < 16; ++e)
+                        if (n1 + e < g.N) p[e] = z[e];
                 }
             }
         } else {
-            epilogue<T, 16>(g, m, n, z);
+            epilogue<T, 16>(g, m, n1, z);
         }
     }
 }
