@@ -566,12 +566,13 @@ int ppo_token_logprobs_bwd(const void *logits, int dtype, long batch, long lengt
  * unmasked: 0.  mask [batch, length] u8 (0 = masked) or NULL; what masked tokens hold is not used, their gradient is 0.
  * advantages [batch, length], or with per_sequence [batch] (adv_stride apart).  ref_log_probs may be NULL (no KL term).
  * Every array has rows of its own stride (elements, >= 0) and contiguous tokens; g_log_probs [batch, length] contiguous or
- * NULL.  clip_low in [0, 1), clip_high >= 0.  Workspace: ppo_policy_kl_loss_workspace_bytes(batch), 8-byte aligned.
+ * NULL.  clip_low in [0, 1), clip_high >= 0.  Workspace: ppo_policy_kl_loss_workspace_bytes(batch, length), 8-byte
+ * aligned; none (0, NULL) for a few thousand tokens.
  */
 #define PPO_KL_K1 1
 #define PPO_KL_K2 2
 #define PPO_KL_K3 3
-size_t ppo_policy_kl_loss_workspace_bytes(long batch);
+size_t ppo_policy_kl_loss_workspace_bytes(long batch, long length);
 int ppo_policy_kl_loss(const float *log_probs, long lp_stride, const float *old_log_probs, long old_stride, const float *advantages,
                        long adv_stride, int per_sequence, const float *ref_log_probs, long ref_stride, const uint8_t *mask,
                        long mask_stride, long batch, long length, double clip_low, double clip_high, double kl_coef, int kl_kind,
@@ -586,7 +587,7 @@ int ppo_policy_kl_loss(const float *log_probs, long lp_stride, const float *old_
  *   out2 = {mean loss, share of pairs with z > 0};  rewards [pairs, 2] = beta times the two sums (means)
  * The two sides have lengths and row strides (elements, >= 0) of their own; ref_* and mask_* may be NULL; g_chosen
  * [pairs, chosen_length] and g_rejected contiguous, or NULL.  Workspace: ppo_preference_loss_workspace_bytes(...), 8-byte
- * aligned.
+ * aligned; none (0, NULL) for a few thousand tokens.
  */
 #define PPO_PREF_SIGMOID 0
 #define PPO_PREF_HINGE 1

@@ -57,7 +57,7 @@ SIGNATURES = {
                                _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _vp]),
     "ppo_token_logprobs_fwd": (_i, [_vp, _i, _l, _l, _l, _l, _l, _vp, _i, _d, _l, _vp, _vp, _vp, _vp]),
     "ppo_token_logprobs_bwd": (_i, [_vp, _i, _l, _l, _l, _l, _l, _vp, _i, _vp, _vp, _vp, _vp, _d, _l, _vp, _vp]),
-    "ppo_policy_kl_loss_workspace_bytes": (_sz, [_l]),
+    "ppo_policy_kl_loss_workspace_bytes": (_sz, [_l, _l]),
     "ppo_policy_kl_loss": (_i, [_vp, _l, _vp, _l, _vp, _l, _i, _vp, _l, _vp, _l, _l, _l, _d, _d, _d, _i, _i, _vp, _vp, _vp, _sz, _vp]),
     "ppo_preference_loss_workspace_bytes": (_sz, [_l, _l, _l]),
     "ppo_preference_loss": (_i, [_vp, _l, _vp, _l, _vp, _l, _l] * 2 + [_l, _i, _d, _d, _i, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),

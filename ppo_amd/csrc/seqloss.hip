@@ -43,19 +43,18 @@ template <int NV, int THREADS> __device__ __forceinline__ void block_sum(double 
 struct __attribute__((packed, aligned(1))) Bytes16 { uint32_t w[4]; };
 struct __attribute__((packed, aligned(1))) Bytes4 { uint32_t w; };
 
-// e^x - 1 - x without its cancellation at small |x|: the Taylor series there (the terms left out are below 2^-27 of it)
-__device__ __forceinline__ float expm1mx(float x)
+// e^x - 1 - x for |x| <= 1/2, where it would cancel: the Taylor series (the terms left out are below 2^-27 of it)
+__device__ __forceinline__ float expm1mx_near(float x)
 {
-    if (fabsf(x) > 0.5f) return expf(x) - 1.0f - x;
     float q = 1.0f / 3628800;                  // 1 / 10!
-    q = q * x + 1.0f / 362880;
-    q = q * x + 1.0f / 40320;
-    q = q * x + 1.0f / 5040;
-    q = q * x + 1.0f / 720;
-    q = q * x + 1.0f / 120;
-    q = q * x + 1.0f / 24;
-    q = q * x + 1.0f / 6;
-    q = q * x + 0.5f;
+    q = __builtin_fmaf(q, x, 1.0f / 362880);
+    q = __builtin_fmaf(q, x, 1.0f / 40320);
+    q = __builtin_fmaf(q, x, 1.0f / 5040);
+    q = __builtin_fmaf(q, x, 1.0f / 720);
+    q = __builtin_fmaf(q, x, 1.0f / 120);
+    q = __builtin_fmaf(q, x, 1.0f / 24);
+    q = __builtin_fmaf(q, x, 1.0f / 6);
+    q = __builtin_fmaf(q, x, 0.5f);
     return q * x * x;
 }
 
@@ -73,7 +72,7 @@ struct PolicyArgs {
 };
 
 // unmasked tokens of the rows that this workgroup visits, a wave a row
-template <int THREADS> __device__ __forceinline__ void count_rows(const PolicyArgs &a, long first, long step, double (&tot)[2])
+__device__ __forceinline__ void count_rows(const PolicyArgs &a, int *row_counts, long first, long step, double (&tot)[2])
 {
     const int lane = threadIdx.x & 63;
     tot[0] = tot[1] = 0.0;
@@ -99,7 +98,7 @@ template <int THREADS> __device__ __forceinline__ void count_rows(const PolicyAr
             n = (int)a.L;
         }
         if (lane == 0) {
-            if (a.sequence_mean) a.row_counts[b] = n;
+            if (a.sequence_mean) row_counts[b] = n;
             tot[0] += (double)n;
             tot[1] += n > 0 ? 1.0 : 0.0;
         }
@@ -110,7 +109,7 @@ __global__ void __launch_bounds__(SEQ_BLOCK) k_policy_count(PolicyArgs a)
 {
     __shared__ double part[SEQ_BLOCK / 64][2];
     double tot[2];
-    count_rows<SEQ_BLOCK>(a, (long)blockIdx.x * (SEQ_BLOCK / 64), (long)gridDim.x * (SEQ_BLOCK / 64), tot);
+    count_rows(a, a.row_counts, (long)blockIdx.x * (SEQ_BLOCK / 64), (long)gridDim.x * (SEQ_BLOCK / 64), tot);
     block_sum<2, SEQ_BLOCK>(tot, part);
     if (threadIdx.x == 0) {
         a.counts[2 * blockIdx.x] = tot[0];
@@ -131,8 +130,8 @@ template <class V> __device__ __forceinline__ void load4(const float *p, int n, 
 }
 
 // groups of four neighbouring tokens of a row
-template <int THREADS> __device__ __forceinline__ void policy_groups(const PolicyArgs &a, double tokens, double rows, long first, long step,
-                                                                      double (&acc)[NSUM])
+__device__ __forceinline__ void policy_groups(const PolicyArgs &a, const int *row_counts, double tokens, double rows, long first, long step,
+                                              double (&acc)[NSUM])
 {
     const double whole = a.sequence_mean ? (rows > 0 ? 1.0 / rows : 1.0) : (tokens > 0 ? 1.0 / tokens : 1.0);
     const long per_row = (a.L + 3) / 4, groups = a.B * per_row;
@@ -162,10 +161,12 @@ template <int THREADS> __device__ __forceinline__ void policy_groups(const Polic
         if (a.ref_lp) load4(a.ref_lp + b * a.ref_stride + t, n, ref);
         double w = 1.0;
         if (a.sequence_mean) {
-            const int c = a.row_counts[b];
+            const int c = row_counts[b];
             w = 1.0 / (double)(c > 0 ? c : 1);
         }
         const float gw = (float)(w * whole);
+        float s_pg = 0.0f, s_kl = 0.0f, s_drift = 0.0f;    // four terms in f32, then f64
+        int out = 0;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             g[i] = 0.0f;
@@ -174,11 +175,10 @@ template <int THREADS> __device__ __forceinline__ void policy_groups(const Polic
                 const bool above = d > a.log_hi, below = d < a.log_lo;
                 const float df = (float)d, r = expf(df), A = adv[i], rA = r * A;
                 const bool cut = A >= 0.0f ? above : below;
-                const float pg = cut ? A * (A >= 0.0f ? a.hi : a.lo) : rA;
+                s_pg -= cut ? A * (A >= 0.0f ? a.hi : a.lo) : rA;
                 float dl = cut ? 0.0f : -rA;
-                acc[0] -= w * (double)pg;
-                acc[2] += above || below ? w : 0.0;
-                acc[3] += w * (double)expm1mx(df);
+                out += above || below ? 1 : 0;
+                s_drift += fabsf(df) > 0.5f ? r - 1.0f - df : expm1mx_near(df);
                 if (a.ref_lp) {
                     const float e = lp[i] - ref[i];
                     float k, dk;
@@ -187,15 +187,19 @@ template <int THREADS> __device__ __forceinline__ void policy_groups(const Polic
                     } else if (a.kl == PPO_KL_K2) {
                         k = 0.5f * e * e; dk = e;
                     } else {
-                        k = expm1mx(-e);
+                        k = fabsf(e) > 0.5f ? expf(-e) - 1.0f + e : expm1mx_near(-e);
                         dk = e - k;                    // 1 - e^-e
                     }
-                    acc[1] += w * (double)k;
-                    dl += a.kl_coef_f * dk;
+                    s_kl += k;
+                    dl = __builtin_fmaf(a.kl_coef_f, dk, dl);
                 }
                 g[i] = gw * dl;
             }
         }
+        acc[0] += w * (double)s_pg;
+        acc[1] += w * (double)s_kl;
+        acc[2] += w * (double)out;
+        acc[3] += w * (double)s_drift;
         if (a.g) {
             float *o = a.g + b * a.L + t;
             if (n == 4) {
@@ -237,7 +241,7 @@ __global__ void __launch_bounds__(SEQ_BLOCK) k_policy_main(PolicyArgs a)
     __shared__ double part[SEQ_BLOCK / 64][NSUM];
     double tokens, rows, acc[NSUM] = {0.0, 0.0, 0.0, 0.0};
     totals(a, part2, tokens, rows);
-    policy_groups<SEQ_BLOCK>(a, tokens, rows, (long)blockIdx.x * SEQ_BLOCK + threadIdx.x, (long)gridDim.x * SEQ_BLOCK, acc);
+    policy_groups(a, a.row_counts, tokens, rows, (long)blockIdx.x * SEQ_BLOCK + threadIdx.x, (long)gridDim.x * SEQ_BLOCK, acc);
     block_sum<NSUM, SEQ_BLOCK>(acc, part);
     if (threadIdx.x == 0) {
 #pragma unroll
@@ -260,15 +264,16 @@ __global__ void __launch_bounds__(SEQ_BLOCK) k_policy_final(PolicyArgs a, int bl
 }
 
 // everything in one workgroup: a few thousand tokens, where launches are what costs
-constexpr int ONE_BLOCK = 1024;
+constexpr int ONE_BLOCK = 512, ONE_ROWS = 256, ONE_GROUPS = 4096;
 __global__ void __launch_bounds__(ONE_BLOCK) k_policy_one(PolicyArgs a)
 {
     __shared__ double part2[ONE_BLOCK / 64][2];
     __shared__ double part[ONE_BLOCK / 64][NSUM];
+    __shared__ int row_counts[ONE_ROWS];
     double tot[2], acc[NSUM] = {0.0, 0.0, 0.0, 0.0};
-    count_rows<ONE_BLOCK>(a, 0, ONE_BLOCK / 64, tot);
-    block_sum<2, ONE_BLOCK>(tot, part2);           // (its barriers order the row counts in global memory for this workgroup)
-    policy_groups<ONE_BLOCK>(a, tot[0], tot[1], threadIdx.x, ONE_BLOCK, acc);
+    count_rows(a, row_counts, 0, ONE_BLOCK / 64, tot);
+    block_sum<2, ONE_BLOCK>(tot, part2);           // (its barriers are the row counts' too)
+    policy_groups(a, row_counts, tot[0], tot[1], threadIdx.x, ONE_BLOCK, acc);
     block_sum<NSUM, ONE_BLOCK>(acc, part);
     if (threadIdx.x == 0) policy_out(a, acc, tot[0], tot[1]);
 }
@@ -283,85 +288,167 @@ struct PrefSide {
 
 struct PrefArgs {
     PrefSide side[2];                              // chosen, rejected
-    double *partials;                              // [2 B][chunks][2]: sum, tokens
-    double *pair;                                  // [B][2]: loss, accuracy of a pair
+    double *partials;                              // [2 B][chunks][2]: sum, tokens of a chunk
+    double *pair;                                  // [B][2]: loss, whether z > 0 of a pair (a workgroup a pair)
     float *out2, *rewards;
     long B;
-    double beta, smoothing;
+    double beta, smoothing, inv_pairs;             // (1 / B from the host: the division in every wave cost 13 us)
     int kind, average, chunks;
 };
 
-// sum of (lp - ref) and number of tokens over [from, to) of row b
-template <int THREADS> __device__ __forceinline__ void pref_sum(const PrefSide &s, long b, long from, long to, double (&acc)[2])
+// the mask's bytes of tokens t .. t + n - 1
+__device__ __forceinline__ uint32_t mask4(const uint8_t *m, long t, int n)
+{
+    if (!m) return 0x01010101u;
+    if (n == 4) return reinterpret_cast<const Bytes4 *>(m + t)->w;
+    uint32_t on = 0;
+    for (int i = 0; i < n; ++i) on |= (uint32_t)m[t + i] << (8 * i);
+    return on;
+}
+
+// sum of (lp - ref) and number of tokens over [from, to) of row b, thread tid's share
+template <int THREADS> __device__ __forceinline__ void pref_sum(const PrefSide &s, long b, long from, long to, int tid, double (&acc)[2])
 {
     const float *lp = s.lp + b * s.lp_stride, *ref = s.ref ? s.ref + b * s.ref_stride : nullptr;
     const uint8_t *m = s.mask ? s.mask + b * s.mask_stride : nullptr;
-    acc[0] = acc[1] = 0.0;
-    for (long t = from + threadIdx.x * 4L; t < to; t += THREADS * 4L) {
+    acc[0] = 0.0;
+    long count = 0;
+#pragma unroll 2
+    for (long t = from + tid * 4L; t < to; t += THREADS * 4L) {
         const int n = to - t < 4 ? (int)(to - t) : 4;
         float x[4], y[4] = {0.0f, 0.0f, 0.0f, 0.0f};
         load4(lp + t, n, x);
         if (ref) load4(ref + t, n, y);
+        const uint32_t on = mask4(m, t, n);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            if (i < n && (!m || m[t + i])) {
+            if (i < n && (on >> (8 * i) & 0xffu)) {
                 acc[0] += (double)x[i] - (double)y[i];
-                acc[1] += 1.0;
+                ++count;
             }
         }
     }
+    acc[1] = (double)count;
 }
 
-struct Pair {
-    double loss, hit, reward[2];
-    float g[2];                                    // d loss / d a token's log-prob, chosen and rejected
+// z = beta D and D of a pair, and beta times its two sums (means)
+struct Margin {
+    double z, delta, scale[2], reward[2];
 };
 
-__device__ __forceinline__ Pair pair_of(const PrefArgs &a, const double (&sum)[2], const double (&count)[2])
+__device__ __forceinline__ Margin margin_of(const PrefArgs &a, const double (&sum)[2], const double (&count)[2])
 {
-    Pair p;
-    double scale[2], mean[2];
+    Margin m;
+    double mean[2];
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
-        scale[k] = a.average ? 1.0 / (count[k] > 0.0 ? count[k] : 1.0) : 1.0;
-        mean[k] = sum[k] * scale[k];
-        p.reward[k] = a.beta * mean[k];
+        m.scale[k] = a.average ? 1.0 / (count[k] > 0.0 ? count[k] : 1.0) : 1.0;
+        mean[k] = sum[k] * m.scale[k];
+        m.reward[k] = a.beta * mean[k];
     }
-    const double delta = mean[0] - mean[1], z = a.beta * delta;
-    double g;
-    if (a.kind == PPO_PREF_SIGMOID) {
-        const double ez = exp(-fabs(z)), sp = log1p(ez);   // softplus(-|z|)
-        const double loss_pos = (z < 0.0 ? -z : 0.0) + sp, loss_neg = (z > 0.0 ? z : 0.0) + sp;   // -ln s(z), -ln s(-z)
-        const double near = ez / (1.0 + ez), far = 1.0 / (1.0 + ez);
-        const double s_neg = z >= 0.0 ? near : far, s_pos = z >= 0.0 ? far : near;   // s(-z), s(z)
-        p.loss = (1.0 - a.smoothing) * loss_pos + a.smoothing * loss_neg;
-        g = -a.beta * ((1.0 - a.smoothing) * s_neg - a.smoothing * s_pos);
-        if (z != z) p.loss = g = z;
-    } else if (a.kind == PPO_PREF_HINGE) {
-        p.loss = z < 1.0 ? 1.0 - z : (z != z ? z : 0.0);
-        g = z < 1.0 ? -a.beta : (z != z ? z : 0.0);
-    } else {
-        const double off = delta - 0.5 / a.beta;
-        p.loss = off * off;
-        g = 2.0 * off;
-    }
-    p.hit = z > 0.0 ? 1.0 : 0.0;
-    g /= (double)a.B;
-    p.g[0] = (float)(g * scale[0]);
-    p.g[1] = (float)(-g * scale[1]);
-    return p;
+    m.delta = mean[0] - mean[1];
+    m.z = a.beta * m.delta;
+    return m;
 }
 
-template <int THREADS> __device__ __forceinline__ void pref_write(const PrefSide &s, long b, long from, long to, float g)
+// e^-x for x >= 0 and ln(1 + y) for y in [0, 1]: short chains, since few lanes wait for them.  Taylor's series of e^r,
+// |r| <= ln 2 / 2, to r^12 / 12!; ln(1 + y) = 2 artanh(y / (2 + y)), whose argument is at most 1/3, to its 19th power: 2e-16
+// and 1e-11 relative.
+__device__ __forceinline__ double exp_minus(double x)
+{
+    if (x > 700.0) return 0.0;
+    const double k = rint(x * -1.4426950408889634), r = __builtin_fma(k, -1.9082149292705877e-10, __builtin_fma(k, -0.6931471803691238, -x));
+    double e = 1.0 / 479001600;
+    e = __builtin_fma(e, r, 1.0 / 39916800);
+    e = __builtin_fma(e, r, 1.0 / 3628800);
+    e = __builtin_fma(e, r, 1.0 / 362880);
+    e = __builtin_fma(e, r, 1.0 / 40320);
+    e = __builtin_fma(e, r, 1.0 / 5040);
+    e = __builtin_fma(e, r, 1.0 / 720);
+    e = __builtin_fma(e, r, 1.0 / 120);
+    e = __builtin_fma(e, r, 1.0 / 24);
+    e = __builtin_fma(e, r, 1.0 / 6);
+    e = __builtin_fma(e, r, 0.5);
+    e = __builtin_fma(e, r, 1.0);
+    e = __builtin_fma(e, r, 1.0);
+    return ldexp(e, (int)k);
+}
+
+__device__ __forceinline__ double log1p_unit(double y)
+{
+    const double s = y / (2.0 + y), q = s * s;
+    double sum = 1.0 / 19;
+    sum = __builtin_fma(sum, q, 1.0 / 17);
+    sum = __builtin_fma(sum, q, 1.0 / 15);
+    sum = __builtin_fma(sum, q, 1.0 / 13);
+    sum = __builtin_fma(sum, q, 1.0 / 11);
+    sum = __builtin_fma(sum, q, 1.0 / 9);
+    sum = __builtin_fma(sum, q, 1.0 / 7);
+    sum = __builtin_fma(sum, q, 1.0 / 5);
+    sum = __builtin_fma(sum, q, 1.0 / 3);
+    sum = __builtin_fma(sum, q, 1.0);
+    return 2.0 * s * sum;
+}
+
+// d mean loss / d a token's log-prob, chosen (k = 0) or rejected
+__device__ __forceinline__ float pair_grad(const PrefArgs &a, const Margin &m, int k)
+{
+    double g;
+    if (a.kind == PPO_PREF_SIGMOID) {
+        const double ez = exp_minus(fabs(m.z)), far = 1.0 / (1.0 + ez), near = ez * far;   // s(|z|), s(-|z|)
+        const double s_neg = m.z >= 0.0 ? near : far, s_pos = m.z >= 0.0 ? far : near;
+        g = -a.beta * ((1.0 - a.smoothing) * s_neg - a.smoothing * s_pos);
+        if (m.z != m.z) g = m.z;
+    } else if (a.kind == PPO_PREF_HINGE) {
+        g = m.z < 1.0 ? -a.beta : (m.z != m.z ? m.z : 0.0);
+    } else {
+        g = 2.0 * (m.delta - 0.5 / a.beta);
+    }
+    return (float)((k == 0 ? g * m.scale[0] : -g * m.scale[1]) * a.inv_pairs);
+}
+
+__device__ __forceinline__ double pair_loss(const PrefArgs &a, const Margin &m)
+{
+    if (a.kind == PPO_PREF_SIGMOID) {
+        const double sp = log1p_unit(exp_minus(fabs(m.z)));           // softplus(-|z|)
+        const double loss_pos = (m.z < 0.0 ? -m.z : 0.0) + sp, loss_neg = (m.z > 0.0 ? m.z : 0.0) + sp;   // -ln s(z), -ln s(-z)
+        return m.z != m.z ? m.z : (1.0 - a.smoothing) * loss_pos + a.smoothing * loss_neg;
+    }
+    if (a.kind == PPO_PREF_HINGE) return m.z < 1.0 ? 1.0 - m.z : (m.z != m.z ? m.z : 0.0);
+    const double off = m.delta - 0.5 / a.beta;
+    return off * off;
+}
+
+// the first two groups of four mask bytes that a thread will want in pref_write: asked for before the margin is known
+struct Ahead {
+    uint32_t on[2];
+};
+
+template <int THREADS> __device__ __forceinline__ Ahead pref_ahead(const PrefSide &s, long b, long from, long to, int tid)
+{
+    Ahead a = {{0x01010101u, 0x01010101u}};
+    if (s.mask && s.g) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const long t = from + (tid + i * THREADS) * 4L;
+            if (t < to) a.on[i] = mask4(s.mask + b * s.mask_stride, t, to - t < 4 ? (int)(to - t) : 4);
+        }
+    }
+    return a;
+}
+
+template <int THREADS> __device__ __forceinline__ void pref_write(const PrefSide &s, long b, long from, long to, int tid, const Ahead &ahead, float g)
 {
     if (!s.g) return;
     const uint8_t *m = s.mask ? s.mask + b * s.mask_stride : nullptr;
     float *o = s.g + b * s.L;
-    for (long t = from + threadIdx.x * 4L; t < to; t += THREADS * 4L) {
+    int turn = 0;
+    for (long t = from + tid * 4L; t < to; t += THREADS * 4L, ++turn) {
         const int n = to - t < 4 ? (int)(to - t) : 4;
+        const uint32_t on = turn == 0 ? ahead.on[0] : turn == 1 ? ahead.on[1] : mask4(m, t, n);
         float v[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = i < n && (!m || m[t + i]) ? g : 0.0f;
+        for (int i = 0; i < 4; ++i) v[i] = on >> (8 * i) & 0xffu ? g : 0.0f;
         if (n == 4) {
             store16<F32>(o + t, v);
         } else {
@@ -370,46 +457,51 @@ template <int THREADS> __device__ __forceinline__ void pref_write(const PrefSide
     }
 }
 
-__device__ __forceinline__ void pref_note(const PrefArgs &a, long b, const Pair &p)
+__device__ __forceinline__ void pref_rewards(const PrefArgs &a, long b, const Margin &m)
 {
-    a.pair[2 * b] = p.loss;
-    a.pair[2 * b + 1] = p.hit;
-    a.rewards[2 * b] = (float)p.reward[0];
-    a.rewards[2 * b + 1] = (float)p.reward[1];
+    a.rewards[2 * b] = (float)m.reward[0];
+    a.rewards[2 * b + 1] = (float)m.reward[1];
 }
 
-template <int THREADS> __device__ __forceinline__ void pref_final(const PrefArgs &a, double (*part)[2])
+__device__ __forceinline__ void pref_out(const PrefArgs &a, double loss, double hits)
 {
-    double acc[2] = {0.0, 0.0};
-    for (long b = threadIdx.x; b < a.B; b += THREADS) {
-        acc[0] += a.pair[2 * b];
-        acc[1] += a.pair[2 * b + 1];
-    }
-    block_sum<2, THREADS>(acc, part);
-    if (threadIdx.x == 0) {
-        a.out2[0] = (float)(acc[0] / (double)a.B);
-        a.out2[1] = (float)(acc[1] / (double)a.B);
-    }
+    a.out2[0] = (float)(loss * a.inv_pairs);
+    a.out2[1] = (float)(hits * a.inv_pairs);
 }
 
 // a workgroup a pair
 __global__ void __launch_bounds__(SEQ_BLOCK) k_pref_pair(PrefArgs a)
 {
-    __shared__ double part[SEQ_BLOCK / 64][2];
+    __shared__ double part[SEQ_BLOCK / 64][4];
     const long b = blockIdx.x;
-    double sum[2], count[2];
+    double v[4], acc[2];
+    pref_sum<SEQ_BLOCK>(a.side[0], b, 0, a.side[0].L, threadIdx.x, acc);
+    v[0] = acc[0]; v[1] = acc[1];
+    pref_sum<SEQ_BLOCK>(a.side[1], b, 0, a.side[1].L, threadIdx.x, acc);
+    v[2] = acc[0]; v[3] = acc[1];
+    const Ahead ahead[2] = {pref_ahead<SEQ_BLOCK>(a.side[0], b, 0, a.side[0].L, threadIdx.x), pref_ahead<SEQ_BLOCK>(a.side[1], b, 0, a.side[1].L, threadIdx.x)};
+    block_sum<4, SEQ_BLOCK>(v, part);
+    const double sum[2] = {v[0], v[2]}, count[2] = {v[1], v[3]};
+    const Margin m = margin_of(a, sum, count);
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-        double acc[2];
-        pref_sum<SEQ_BLOCK>(a.side[k], b, 0, a.side[k].L, acc);
-        block_sum<2, SEQ_BLOCK>(acc, part);
-        sum[k] = acc[0];
-        count[k] = acc[1];
+    for (int k = 0; k < 2; ++k) pref_write<SEQ_BLOCK>(a.side[k], b, 0, a.side[k].L, threadIdx.x, ahead[k], pair_grad(a, m, k));
+    if (threadIdx.x == 0) {
+        pref_rewards(a, b, m);
+        a.pair[2 * b] = pair_loss(a, m);
+        a.pair[2 * b + 1] = m.z > 0.0 ? 1.0 : 0.0;
     }
-    const Pair p = pair_of(a, sum, count);
-#pragma unroll
-    for (int k = 0; k < 2; ++k) pref_write<SEQ_BLOCK>(a.side[k], b, 0, a.side[k].L, p.g[k]);
-    if (threadIdx.x == 0) pref_note(a, b, p);
+}
+
+__global__ void __launch_bounds__(SEQ_BLOCK) k_pref_final(PrefArgs a)
+{
+    __shared__ double part[SEQ_BLOCK / 64][2];
+    double acc[2] = {0.0, 0.0};
+    for (long b = threadIdx.x; b < a.B; b += SEQ_BLOCK) {
+        acc[0] += a.pair[2 * b];
+        acc[1] += a.pair[2 * b + 1];
+    }
+    block_sum<2, SEQ_BLOCK>(acc, part);
+    if (threadIdx.x == 0) pref_out(a, acc[0], acc[1]);
 }
 
 // long rows, few pairs: a workgroup a chunk of one row
@@ -428,7 +520,7 @@ __global__ void __launch_bounds__(SEQ_BLOCK) k_pref_sum(PrefArgs a)
     long from, to;
     chunk_of(a, a.side[k].L, c, from, to);
     double acc[2];
-    pref_sum<SEQ_BLOCK>(a.side[k], b, from, to, acc);
+    pref_sum<SEQ_BLOCK>(a.side[k], b, from, to, threadIdx.x, acc);
     block_sum<2, SEQ_BLOCK>(acc, part);
     if (threadIdx.x == 0) {
         a.partials[2L * blockIdx.x] = acc[0];
@@ -436,42 +528,92 @@ __global__ void __launch_bounds__(SEQ_BLOCK) k_pref_sum(PrefArgs a)
     }
 }
 
-__global__ void __launch_bounds__(SEQ_BLOCK) k_pref_grad(PrefArgs a)
+// the margin of pair b from its chunks' sums: LANES neighbouring lanes together, each gets it
+template <int LANES> __device__ __forceinline__ Margin margin_of_chunks(const PrefArgs &a, long b, int lane)
 {
-    __shared__ double part[SEQ_BLOCK / 64][4];
-    const long b = blockIdx.x / (2 * a.chunks);
-    const int k = blockIdx.x / a.chunks % 2, c = blockIdx.x % a.chunks;
     double v[4] = {0.0, 0.0, 0.0, 0.0};
-    for (int i = threadIdx.x; i < a.chunks; i += SEQ_BLOCK) {
+    for (int i = lane; i < a.chunks; i += LANES) {
         const double *p = a.partials + 2 * (b * 2 * a.chunks + i);
         v[0] += p[0];
         v[1] += p[1];
         v[2] += p[2 * a.chunks];
         v[3] += p[2 * a.chunks + 1];
     }
-    block_sum<4, SEQ_BLOCK>(v, part);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[k] = wave_sum(v[k]);
     const double sum[2] = {v[0], v[2]}, count[2] = {v[1], v[3]};
-    const Pair p = pair_of(a, sum, count);
+    return margin_of(a, sum, count);
+}
+
+// the last workgroup makes the mean over the pairs, the others write the gradients of their chunks
+__global__ void __launch_bounds__(SEQ_BLOCK) k_pref_grad(PrefArgs a)
+{
+    const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
+    if (blockIdx.x == 2 * a.B * a.chunks) {
+        __shared__ double part[SEQ_BLOCK / 64][2];
+        double acc[2] = {0.0, 0.0};
+        for (long b = wid; b < a.B; b += SEQ_BLOCK / 64) {
+            const Margin m = margin_of_chunks<64>(a, b, lane);
+            if (lane == 0) {
+                acc[0] += pair_loss(a, m);
+                acc[1] += m.z > 0.0 ? 1.0 : 0.0;
+                pref_rewards(a, b, m);
+            }
+        }
+        block_sum<2, SEQ_BLOCK>(acc, part);
+        if (threadIdx.x == 0) pref_out(a, acc[0], acc[1]);
+        return;
+    }
+    const long b = blockIdx.x / (2 * a.chunks);
+    const int k = blockIdx.x / a.chunks % 2, c = blockIdx.x % a.chunks;
     long from, to;
     chunk_of(a, a.side[k].L, c, from, to);
-    pref_write<SEQ_BLOCK>(a.side[k], b, from, to, p.g[k]);
-    if (threadIdx.x == 0 && k == 0 && c == 0) pref_note(a, b, p);
+    const Ahead ahead = pref_ahead<SEQ_BLOCK>(a.side[k], b, from, to, threadIdx.x);
+    const float g = pair_grad(a, margin_of_chunks<64>(a, b, lane), k);   // (every wave for itself)
+    pref_write<SEQ_BLOCK>(a.side[k], b, from, to, threadIdx.x, ahead, g);
 }
 
-__global__ void __launch_bounds__(SEQ_BLOCK) k_pref_final(PrefArgs a)
+// everything in one workgroup, a wave a pair: a few thousand tokens, where launches are what costs
+__global__ void __launch_bounds__(ONE_BLOCK) k_pref_one(PrefArgs a)
 {
-    __shared__ double part[SEQ_BLOCK / 64][2];
-    pref_final<SEQ_BLOCK>(a, part);
+    __shared__ double part[ONE_BLOCK / 64][2];
+    const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
+    double tot[2] = {0.0, 0.0};
+    for (long b = wid; b < a.B; b += ONE_BLOCK / 64) {
+        double sum[2], count[2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            double acc[2];
+            pref_sum<64>(a.side[k], b, 0, a.side[k].L, lane, acc);
+            sum[k] = wave_sum(acc[0]);
+            count[k] = wave_sum(acc[1]);
+        }
+        const Margin m = margin_of(a, sum, count);
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+            pref_write<64>(a.side[k], b, 0, a.side[k].L, lane, pref_ahead<64>(a.side[k], b, 0, a.side[k].L, lane), pair_grad(a, m, k));
+        if (lane == 0) {
+            pref_rewards(a, b, m);
+            tot[0] += pair_loss(a, m);
+            tot[1] += m.z > 0.0 ? 1.0 : 0.0;
+        }
+    }
+    block_sum<2, ONE_BLOCK>(tot, part);
+    if (threadIdx.x == 0) pref_out(a, tot[0], tot[1]);
 }
 
-// chunks a row is cut into: 1 = a workgroup a pair
-int pref_chunks(long B, long L)
+bool one_workgroup(long batch, long length) { return batch <= ONE_ROWS && batch * ((length + 3) / 4) <= ONE_GROUPS; }
+
+// workgroups a row is cut into: 0 = one for everything, 1 = one a pair, otherwise about 512 in all, of 2048 tokens at least
+int pref_chunks(long B, long Lc, long Lr)
 {
-    if (B >= 256 || L <= 8192) return 1;
+    if (B <= 64 && B * (Lc + Lr) <= 32768) return 0;
+    const long L = Lc > Lr ? Lc : Lr;
+    if (B >= 256 || L <= 4096) return 1;
     long c = (512 + 2 * B - 1) / (2 * B);
-    const long most = (L + 4095) / 4096;
+    const long most = (L + 2047) / 2048;
     if (c > most) c = most;
-    return c < 1 ? 1 : (int)c;
+    return c < 2 ? 2 : (int)c;
 }
 
 bool rows_ok(const void *p, long B, long L, long stride)
@@ -483,9 +625,9 @@ bool rows_ok(const void *p, long B, long L, long stride)
 
 extern "C" {
 
-size_t ppo_policy_kl_loss_workspace_bytes(long batch)
+size_t ppo_policy_kl_loss_workspace_bytes(long batch, long length)
 {
-    return batch < 0 ? 0 : (size_t)SEQ_MAX_BLOCKS * NSUM * sizeof(double) + (size_t)COUNT_MAX_BLOCKS * 2 * sizeof(double) + (size_t)batch * sizeof(int);
+    return batch < 0 || one_workgroup(batch, length) ? 0 : (size_t)SEQ_MAX_BLOCKS * NSUM * sizeof(double) + (size_t)COUNT_MAX_BLOCKS * 2 * sizeof(double) + (size_t)batch * sizeof(int);
 }
 
 int ppo_policy_kl_loss(const float *log_probs, long lp_stride, const float *old_log_probs, long old_stride, const float *advantages,
@@ -501,7 +643,8 @@ int ppo_policy_kl_loss(const float *log_probs, long lp_stride, const float *old_
     PPO_REQUIRE(out6 && ppo_aligned(out6, 4) && ppo_aligned(g_log_probs, 4));
     PPO_REQUIRE(clip_low >= 0.0 && clip_low < 1.0 && clip_high >= 0.0 && clip_high <= 1e30 && kl_coef == kl_coef);
     PPO_REQUIRE(kl_kind == PPO_KL_K1 || kl_kind == PPO_KL_K2 || kl_kind == PPO_KL_K3);
-    PPO_REQUIRE(workspace && ppo_aligned(workspace, 8) && workspace_bytes >= ppo_policy_kl_loss_workspace_bytes(batch));
+    const bool one = one_workgroup(batch, length);
+    PPO_REQUIRE(one || (workspace && ppo_aligned(workspace, 8) && workspace_bytes >= ppo_policy_kl_loss_workspace_bytes(batch, length)));
     PolicyArgs a;
     a.lp = log_probs; a.old_lp = old_log_probs; a.adv = advantages; a.ref_lp = ref_log_probs; a.mask = mask;
     a.g = g_log_probs; a.out6 = out6;
@@ -515,7 +658,7 @@ int ppo_policy_kl_loss(const float *log_probs, long lp_stride, const float *old_
     a.kl = kl_kind; a.per_sequence = per_sequence; a.sequence_mean = sequence_mean;
     hipStream_t s = (hipStream_t)stream;
     const long groups = batch * ((length + 3) / 4);
-    if (groups <= 4096 && batch <= 256) {
+    if (one) {
         a.count_blocks = 0;
         hipLaunchKernelGGL(k_policy_one, dim3(1), dim3(ONE_BLOCK), 0, s, a);
         return ppo_launch_status();
@@ -536,9 +679,9 @@ int ppo_policy_kl_loss(const float *log_probs, long lp_stride, const float *old_
 
 size_t ppo_preference_loss_workspace_bytes(long pairs, long chosen_length, long rejected_length)
 {
-    if (pairs < 0) return 0;
-    const int chunks = pref_chunks(pairs, chosen_length > rejected_length ? chosen_length : rejected_length);
-    return (size_t)pairs * 2 * sizeof(double) + (size_t)pairs * 4 * chunks * sizeof(double);
+    if (pairs < 0 || chosen_length < 0 || rejected_length < 0) return 0;
+    const int chunks = pref_chunks(pairs, chosen_length, rejected_length);
+    return chunks == 0 ? 0 : chunks == 1 ? (size_t)pairs * 2 * sizeof(double) : (size_t)pairs * 4 * chunks * sizeof(double);
 }
 
 int ppo_preference_loss(const float *chosen, long chosen_stride, const float *ref_chosen, long ref_chosen_stride,
@@ -553,8 +696,9 @@ int ppo_preference_loss(const float *chosen, long chosen_stride, const float *re
     PPO_REQUIRE(kind == PPO_PREF_SIGMOID || kind == PPO_PREF_HINGE || kind == PPO_PREF_IPO);
     PPO_REQUIRE(beta > 0.0 && beta <= 1e30 && label_smoothing >= 0.0 && label_smoothing < 0.5);
     PPO_REQUIRE(out2 && rewards && ppo_aligned(out2, 4) && ppo_aligned(rewards, 4) && ppo_aligned(g_chosen, 4) && ppo_aligned(g_rejected, 4));
-    PPO_REQUIRE(workspace && ppo_aligned(workspace, 8) &&
-                workspace_bytes >= ppo_preference_loss_workspace_bytes(pairs, chosen_length, rejected_length));
+    const int chunks = pref_chunks(pairs, chosen_length, rejected_length);
+    PPO_REQUIRE(chunks == 0 || (workspace && ppo_aligned(workspace, 8) &&
+                                workspace_bytes >= ppo_preference_loss_workspace_bytes(pairs, chosen_length, rejected_length)));
     PrefArgs a;
     a.side[0] = PrefSide{chosen, ref_chosen, mask_chosen, g_chosen, chosen_length, chosen_stride, ref_chosen_stride, mask_chosen_stride};
     a.side[1] = PrefSide{rejected, ref_rejected, mask_rejected, g_rejected, rejected_length, rejected_stride, ref_rejected_stride, mask_rejected_stride};
@@ -563,22 +707,25 @@ int ppo_preference_loss(const float *chosen, long chosen_stride, const float *re
         PPO_REQUIRE(rows_ok(s.lp, pairs, s.L, s.lp_stride) && (!s.ref || rows_ok(s.ref, pairs, s.L, s.ref_stride)));
         PPO_REQUIRE(!s.mask || (s.mask_stride >= 0 && (__int128)(pairs - 1) * s.mask_stride + s.L < ((__int128)1 << 60)));
     }
-    a.pair = reinterpret_cast<double *>(workspace);
-    a.partials = a.pair + 2 * pairs;
-    a.out2 = out2; a.rewards = rewards; a.B = pairs; a.beta = beta; a.smoothing = label_smoothing; a.kind = kind; a.average = average;
-    a.chunks = pref_chunks(pairs, chosen_length > rejected_length ? chosen_length : rejected_length);
+    a.pair = a.partials = reinterpret_cast<double *>(workspace);
+    a.out2 = out2; a.rewards = rewards; a.B = pairs; a.inv_pairs = 1.0 / (double)pairs; a.beta = beta; a.smoothing = label_smoothing; a.kind = kind; a.average = average;
+    a.chunks = chunks;
     hipStream_t s = (hipStream_t)stream;
-    if (a.chunks == 1) {
+    if (chunks == 0) {
+        hipLaunchKernelGGL(k_pref_one, dim3(1), dim3(ONE_BLOCK), 0, s, a);
+        return ppo_launch_status();
+    }
+    if (chunks == 1) {
         hipLaunchKernelGGL(k_pref_pair, dim3((unsigned)pairs), dim3(SEQ_BLOCK), 0, s, a);
-    } else {
-        hipLaunchKernelGGL(k_pref_sum, dim3((unsigned)(2 * pairs * a.chunks)), dim3(SEQ_BLOCK), 0, s, a);
         const int rc = ppo_launch_status();
         if (rc) return rc;
-        hipLaunchKernelGGL(k_pref_grad, dim3((unsigned)(2 * pairs * a.chunks)), dim3(SEQ_BLOCK), 0, s, a);
+        hipLaunchKernelGGL(k_pref_final, dim3(1), dim3(SEQ_BLOCK), 0, s, a);
+    } else {
+        hipLaunchKernelGGL(k_pref_sum, dim3((unsigned)(2 * pairs * chunks)), dim3(SEQ_BLOCK), 0, s, a);
+        const int rc = ppo_launch_status();
+        if (rc) return rc;
+        hipLaunchKernelGGL(k_pref_grad, dim3((unsigned)(2 * pairs * chunks + 1)), dim3(SEQ_BLOCK), 0, s, a);
     }
-    const int rc = ppo_launch_status();
-    if (rc) return rc;
-    hipLaunchKernelGGL(k_pref_final, dim3(1), dim3(SEQ_BLOCK), 0, s, a);
     return ppo_launch_status();
 }
 

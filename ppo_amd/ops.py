@@ -691,49 +691,58 @@ KL_KINDS = {"k1": 1, "k2": 2, "k3": 3}                                 # PPO_KL_
 PREFERENCE_KINDS = {"sigmoid": 0, "hinge": 1, "ipo": 2}                # PPO_PREF_*
 
 
-def _need(cond, what: str):
-    if not cond:
-        raise _lib.PpoAmdError(what)
+def _refuse(what: str):
+    raise _lib.PpoAmdError(what)
 
 
 def _on_tensor_device(fn):
     """Launches go to the first tensor's device and that device's current stream."""
     @functools.wraps(fn)
     def call(first, *args, **kwargs):
-        _need(isinstance(first, torch.Tensor), f"{fn.__name__} takes tensors")
-        if first.is_cuda and first.get_device() != torch._C._cuda_getDevice():
-            with torch.cuda.device(first.device):
+        if not isinstance(first, torch.Tensor):
+            _refuse(f"{fn.__name__} takes tensors")
+        index = first.get_device()
+        if index >= 0 and index != torch._C._cuda_getDevice():
+            with torch.cuda.device(index):
                 return fn(first, *args, **kwargs)
         return fn(first, *args, **kwargs)
     return call
 
 
-def _device_tensors(name: str, *tensors):
-    dev = tensors[0].device
-    _need(dev.type == "cuda", f"{name} needs HIP device tensors; there is no CPU fallback")
-    for t in tensors[1:]:
-        _need(t is None or t.device == dev, f"{name}: every tensor has to be on {dev}")
+def _device_tensors(name: str, first, *others):
+    index = first.get_device()
+    if index < 0:
+        _refuse(f"{name} needs HIP device tensors; there is no CPU fallback")
+    for t in others:
+        if t is not None and t.get_device() != index:
+            _refuse(f"{name}: every tensor has to be on {first.device}")
 
 
 def _token_rows(name, logits, actions, temperature):
-    """(logits with contiguous actions, actions, [batch, length, batch stride, token stride])"""
-    _need(logits.dtype in _DTYPES, f"{name}: logits are float32, bfloat16 or float16, not {logits.dtype}")
-    _need(logits.dim() >= 1 and logits.shape[-1] >= 1, f"{name}: logits are [..., actions] with at least one action")
-    _need(isinstance(actions, torch.Tensor) and actions.dtype in (torch.int32, torch.int64), f"{name}: actions are int32 or int64")
-    _need(actions.shape == logits.shape[:-1], f"{name}: actions {tuple(actions.shape)} for logits {tuple(logits.shape)}")
-    _need(1e-6 <= float(temperature) <= 1e6, f"{name}: temperature {temperature} outside [1e-6, 1e6]")
+    """(logits with contiguous actions, actions, batch, length, batch stride, token stride)"""
+    if logits.dtype not in _DTYPES:
+        _refuse(f"{name}: logits are float32, bfloat16 or float16, not {logits.dtype}")
+    if logits.dim() < 1 or logits.shape[-1] < 1:
+        _refuse(f"{name}: logits are [..., actions] with at least one action")
+    if not isinstance(actions, torch.Tensor) or actions.dtype not in (torch.int32, torch.int64):
+        _refuse(f"{name}: actions are int32 or int64")
+    if actions.shape != logits.shape[:-1]:
+        _refuse(f"{name}: actions {tuple(actions.shape)} for logits {tuple(logits.shape)}")
+    if not 1e-6 <= temperature <= 1e6:
+        _refuse(f"{name}: temperature {temperature} outside [1e-6, 1e6]")
     _device_tensors(name, logits, actions)
     if logits.dim() > 3:
         logits = logits.reshape(-1, *logits.shape[-2:])
-    if logits.shape[-1] > 1 and logits.stride(-1) != 1:
+    strides = logits.stride()
+    if strides[-1] != 1 and logits.shape[-1] > 1:
         logits = logits.contiguous()
-    if logits.dim() == 3:
-        geometry = (logits.shape[0], logits.shape[1], logits.stride(0), logits.stride(1))
-    elif logits.dim() == 2:
-        geometry = (1, logits.shape[0], 0, logits.stride(0))
-    else:
-        geometry = (1, 1, 0, 0)
-    return logits, actions.contiguous(), geometry
+        strides = logits.stride()
+    actions = actions.contiguous()
+    if len(strides) == 3:
+        return logits, actions, logits.shape[0], logits.shape[1], strides[0], strides[1]
+    if len(strides) == 2:
+        return logits, actions, 1, logits.shape[0], 0, strides[0]
+    return logits, actions, 1, 1, 0, 0
 
 
 @_on_tensor_device
@@ -745,15 +754,16 @@ def token_logprobs_fwd(logits, actions, temperature=1.0, ignore_index=-100, want
     action is ignore_index gives 0; a row without a legal action gives log p -inf and entropy 0; an action out of range
     gives NaN.  stats [..., 2] is what token_logprobs_bwd needs."""
     lib = _lib.load()
-    lg, act, (batch, length, bs, ts) = _token_rows("token_logprobs", logits, actions, temperature)
-    shape, dev = actions.shape, lg.device
+    lg, act, batch, length, bs, ts = _token_rows("token_logprobs", logits, actions, temperature)
+    shape, dev = act.shape, lg.device
     logp = torch.empty(shape, dtype=torch.float32, device=dev)
     entropy = torch.empty(shape, dtype=torch.float32, device=dev) if want_entropy else None
     stats = torch.empty((*shape, 2), dtype=torch.float32, device=dev)
     rc = lib.ppo_token_logprobs_fwd(lg.data_ptr(), _DTYPES[lg.dtype], batch, length, lg.shape[-1], bs, ts, act.data_ptr(),
-                                    act.element_size(), float(temperature), int(ignore_index), logp.data_ptr(), _ptr(entropy),
+                                    act.element_size(), temperature, ignore_index, logp.data_ptr(), _ptr(entropy),
                                     stats.data_ptr(), _stream())
-    _lib.check(rc, "ppo_token_logprobs_fwd")
+    if rc:
+        _lib.check(rc, "ppo_token_logprobs_fwd")
     return logp, entropy, stats
 
 
@@ -763,20 +773,26 @@ def token_logprobs_bwd(logits, actions, stats, entropy, g_logp, g_entropy=None, 
     from the inputs and outputs of token_logprobs_fwd.  g_logp or g_entropy may be None."""
     lib = _lib.load()
     name = "token_logprobs_bwd"
-    lg, act, (batch, length, bs, ts) = _token_rows(name, logits, actions, temperature)
-    _need(g_logp is not None or g_entropy is not None, f"{name}: a gradient of log p or of the entropy is needed")
-    _need(g_entropy is None or entropy is not None, f"{name}: the entropy's gradient needs the entropy")
-    _need(stats.dtype == torch.float32 and stats.shape == (*actions.shape, 2) and stats.is_contiguous(), f"{name}: stats are those of the forward call")
+    lg, act, batch, length, bs, ts = _token_rows(name, logits, actions, temperature)
+    shape = act.shape
+    if g_logp is None and g_entropy is None:
+        _refuse(f"{name}: a gradient of log p or of the entropy is needed")
+    if g_entropy is not None and entropy is None:
+        _refuse(f"{name}: the entropy's gradient needs the entropy")
+    if stats.dtype != torch.float32 or stats.shape != (*shape, 2) or not stats.is_contiguous():
+        _refuse(f"{name}: stats are those of the forward call")
     rows = []
     for t in (entropy, g_logp, g_entropy):
-        _need(t is None or (t.dtype == torch.float32 and t.shape == actions.shape), f"{name}: entropy and gradients are float32 of the actions' shape")
+        if t is not None and (t.dtype != torch.float32 or t.shape != shape):
+            _refuse(f"{name}: entropy and gradients are float32 of the actions' shape")
         rows.append(None if t is None else t.contiguous())
     _device_tensors(name, lg, stats, *rows)
     g = torch.empty(logits.shape, dtype=lg.dtype, device=lg.device)
     rc = lib.ppo_token_logprobs_bwd(lg.data_ptr(), _DTYPES[lg.dtype], batch, length, lg.shape[-1], bs, ts, act.data_ptr(),
-                                    act.element_size(), stats.data_ptr(), *[_ptr(t) for t in rows], float(temperature),
-                                    int(ignore_index), g.data_ptr(), _stream())
-    _lib.check(rc, "ppo_token_logprobs_bwd")
+                                    act.element_size(), stats.data_ptr(), *[_ptr(t) for t in rows], temperature, ignore_index,
+                                    g.data_ptr(), _stream())
+    if rc:
+        _lib.check(rc, "ppo_token_logprobs_bwd")
     return g
 
 
@@ -805,18 +821,22 @@ def token_logprobs(logits, actions, temperature=1.0, ignore_index=-100):
     return token_logprobs_fwd(logits, actions, temperature, ignore_index)[:2]
 
 
-def _sequence_rows(name, what, t, shape, dtypes=(torch.float32,)):
-    """(tensor whose tokens are contiguous, its row stride); (None, 0) for None"""
+_MASK_TYPES = (torch.bool, torch.uint8)
+
+
+def _sequence_rows(name, what, t, shape, mask=False):
+    """(tensor whose tokens are contiguous, its row stride) of a [rows, tokens] or [rows] tensor; (None, 0) for None"""
     if t is None:
         return None, 0
-    _need(isinstance(t, torch.Tensor) and t.dtype in dtypes, f"{name}: {what} is {' or '.join(str(d) for d in dtypes)}")
-    _need(tuple(t.shape) == tuple(shape), f"{name}: {what} is {tuple(t.shape)}, not {tuple(shape)}")
-    if t.dim() == 2 and t.shape[1] > 1 and t.stride(1) != 1:
+    if not isinstance(t, torch.Tensor) or (t.dtype not in _MASK_TYPES if mask else t.dtype != torch.float32):
+        _refuse(f"{name}: {what} is a {'bool or uint8' if mask else 'float32'} tensor")
+    if t.shape != shape:
+        _refuse(f"{name}: {what} is {tuple(t.shape)}, not {tuple(shape)}")
+    strides = t.stride()
+    if len(strides) == 2 and strides[1] != 1 and shape[1] > 1:
         t = t.contiguous()
-    return t, t.stride(0)
-
-
-_MASK_TYPES = (torch.bool, torch.uint8)
+        strides = t.stride()
+    return t, strides[0]
 
 
 @_on_tensor_device
@@ -831,31 +851,35 @@ def policy_kl_loss_fwd_bwd(new_lp, old_lp, adv, mask=None, ref_lp=None, clip_low
     strided."""
     lib = _lib.load()
     name = "policy_kl_loss"
-    _need(new_lp.dim() == 2, f"{name}: log-probs are [sequences, tokens]")
-    _need(kl in KL_KINDS, f"{name}: kl is one of {sorted(KL_KINDS)}")
-    _need(reduction in ("token", "sequence"), f"{name}: reduction is 'token' or 'sequence'")
-    _need(0.0 <= float(clip_low) < 1.0 and 0.0 <= float(clip_high) <= 1e30, f"{name}: clip_low in [0, 1), clip_high >= 0")
-    _need(float(kl_coef) == float(kl_coef), f"{name}: kl_coef is NaN")
-    B, L = shape = tuple(new_lp.shape)
+    if new_lp.dim() != 2:
+        _refuse(f"{name}: log-probs are [sequences, tokens]")
+    if kl not in KL_KINDS or reduction not in ("token", "sequence"):
+        _refuse(f"{name}: kl is one of {sorted(KL_KINDS)}, reduction 'token' or 'sequence'")
+    if not (0.0 <= clip_low < 1.0 and 0.0 <= clip_high <= 1e30 and kl_coef == kl_coef):
+        _refuse(f"{name}: clip_low in [0, 1), clip_high >= 0, kl_coef a number")
+    if old_lp is None or adv is None:
+        _refuse(f"{name}: old_lp and adv are needed")
+    shape = new_lp.shape
+    B, L = shape
     new, new_s = _sequence_rows(name, "new_lp", new_lp, shape)
     old, old_s = _sequence_rows(name, "old_lp", old_lp, shape)
     ref, ref_s = _sequence_rows(name, "ref_lp", ref_lp, shape)
-    msk, msk_s = _sequence_rows(name, "mask", mask, shape, _MASK_TYPES)
+    msk, msk_s = _sequence_rows(name, "mask", mask, shape, True)
     per_sequence = isinstance(adv, torch.Tensor) and adv.dim() == 1
     a, a_s = _sequence_rows(name, "adv", adv, shape[:1] if per_sequence else shape)
-    _need(old is not None and a is not None, f"{name}: old_lp and adv are needed")
     _device_tensors(name, new, old, ref, msk, a)
     dev = new.device
     g = torch.empty(shape, dtype=torch.float32, device=dev) if want_grad else None
     if B == 0 or L == 0:
         return torch.zeros(6, dtype=torch.float32, device=dev), g
     out6 = torch.empty(6, dtype=torch.float32, device=dev)
-    nws = lib.ppo_policy_kl_loss_workspace_bytes(B)
-    ws = torch.empty(nws, dtype=torch.uint8, device=dev)
-    rc = lib.ppo_policy_kl_loss(new.data_ptr(), new_s, old.data_ptr(), old_s, a.data_ptr(), a_s, int(per_sequence), _ptr(ref),
-                                ref_s, _ptr(msk), msk_s, B, L, float(clip_low), float(clip_high), float(kl_coef), KL_KINDS[kl],
-                                int(reduction == "sequence"), out6.data_ptr(), _ptr(g), ws.data_ptr(), nws, _stream())
-    _lib.check(rc, "ppo_policy_kl_loss")
+    nws = lib.ppo_policy_kl_loss_workspace_bytes(B, L)
+    ws = torch.empty(nws, dtype=torch.uint8, device=dev) if nws else None
+    rc = lib.ppo_policy_kl_loss(new.data_ptr(), new_s, old.data_ptr(), old_s, a.data_ptr(), a_s, per_sequence, _ptr(ref),
+                                ref_s, _ptr(msk), msk_s, B, L, clip_low, clip_high, kl_coef, KL_KINDS[kl], reduction == "sequence",
+                                out6.data_ptr(), _ptr(g), _ptr(ws), nws, _stream())
+    if rc:
+        _lib.check(rc, "ppo_policy_kl_loss")
     return out6, g
 
 
@@ -881,33 +905,36 @@ def preference_loss_fwd_bwd(chosen_lp, rejected_lp, ref_chosen_lp=None, ref_reje
     [pairs, 2] = beta times the two sums, g_chosen, g_rejected)."""
     lib = _lib.load()
     name = "preference_loss"
-    _need(chosen_lp.dim() == 2 and isinstance(rejected_lp, torch.Tensor) and rejected_lp.dim() == 2 and rejected_lp.shape[0] == chosen_lp.shape[0],
-          f"{name}: log-probs are [pairs, tokens], as many pairs chosen as rejected")
-    _need(kind in PREFERENCE_KINDS, f"{name}: kind is one of {sorted(PREFERENCE_KINDS)}")
-    _need(0.0 < float(beta) <= 1e30, f"{name}: beta > 0")
-    _need(0.0 <= float(label_smoothing) < 0.5, f"{name}: label_smoothing in [0, 0.5)")
-    pairs = chosen_lp.shape[0]
-    sides, tensors, grads = [], [], []
-    for what, lp, ref, mask in (("chosen", chosen_lp, ref_chosen_lp, chosen_mask), ("rejected", rejected_lp, ref_rejected_lp, rejected_mask)):
-        x, xs = _sequence_rows(name, what + "_lp", lp, lp.shape)
-        r, rs = _sequence_rows(name, f"ref_{what}_lp", ref, lp.shape)
-        m, ms = _sequence_rows(name, what + "_mask", mask, lp.shape, _MASK_TYPES)
-        tensors += [x, r, m]
-        sides += [x.data_ptr(), xs, _ptr(r), rs, _ptr(m), ms, lp.shape[1]]
-    _device_tensors(name, *tensors)
-    dev = chosen_lp.device
-    for lp in (chosen_lp, rejected_lp):
-        grads.append(torch.empty(lp.shape, dtype=torch.float32, device=dev) if want_grad else None)
+    if chosen_lp.dim() != 2 or not isinstance(rejected_lp, torch.Tensor) or rejected_lp.dim() != 2 or rejected_lp.shape[0] != chosen_lp.shape[0]:
+        _refuse(f"{name}: log-probs are [pairs, tokens], as many pairs chosen as rejected")
+    if kind not in PREFERENCE_KINDS:
+        _refuse(f"{name}: kind is one of {sorted(PREFERENCE_KINDS)}")
+    if not (0.0 < beta <= 1e30 and 0.0 <= label_smoothing < 0.5):
+        _refuse(f"{name}: beta > 0, label_smoothing in [0, 0.5)")
+    cs, rs = chosen_lp.shape, rejected_lp.shape
+    pairs = cs[0]
+    c, c_s = _sequence_rows(name, "chosen_lp", chosen_lp, cs)
+    rc_, rc_s = _sequence_rows(name, "ref_chosen_lp", ref_chosen_lp, cs)
+    mc, mc_s = _sequence_rows(name, "chosen_mask", chosen_mask, cs, True)
+    r, r_s = _sequence_rows(name, "rejected_lp", rejected_lp, rs)
+    rr, rr_s = _sequence_rows(name, "ref_rejected_lp", ref_rejected_lp, rs)
+    mr, mr_s = _sequence_rows(name, "rejected_mask", rejected_mask, rs, True)
+    _device_tensors(name, c, rc_, mc, r, rr, mr)
+    dev = c.device
+    g_c = torch.empty(cs, dtype=torch.float32, device=dev) if want_grad else None
+    g_r = torch.empty(rs, dtype=torch.float32, device=dev) if want_grad else None
     rewards = torch.empty((pairs, 2), dtype=torch.float32, device=dev)
     if pairs == 0:
-        return torch.zeros(2, dtype=torch.float32, device=dev), rewards, *grads
+        return torch.zeros(2, dtype=torch.float32, device=dev), rewards, g_c, g_r
     out2 = torch.empty(2, dtype=torch.float32, device=dev)
-    nws = lib.ppo_preference_loss_workspace_bytes(pairs, chosen_lp.shape[1], rejected_lp.shape[1])
-    ws = torch.empty(nws, dtype=torch.uint8, device=dev)
-    rc = lib.ppo_preference_loss(*sides, pairs, PREFERENCE_KINDS[kind], float(beta), float(label_smoothing), int(bool(average)),
-                                 out2.data_ptr(), rewards.data_ptr(), _ptr(grads[0]), _ptr(grads[1]), ws.data_ptr(), nws, _stream())
-    _lib.check(rc, "ppo_preference_loss")
-    return out2, rewards, *grads
+    nws = lib.ppo_preference_loss_workspace_bytes(pairs, cs[1], rs[1])
+    ws = torch.empty(nws, dtype=torch.uint8, device=dev) if nws else None
+    rc = lib.ppo_preference_loss(c.data_ptr(), c_s, _ptr(rc_), rc_s, _ptr(mc), mc_s, cs[1], r.data_ptr(), r_s, _ptr(rr), rr_s,
+                                 _ptr(mr), mr_s, rs[1], pairs, PREFERENCE_KINDS[kind], beta, label_smoothing, bool(average),
+                                 out2.data_ptr(), rewards.data_ptr(), _ptr(g_c), _ptr(g_r), _ptr(ws), nws, _stream())
+    if rc:
+        _lib.check(rc, "ppo_preference_loss")
+    return out2, rewards, g_c, g_r
 
 
 class _PairLoss(torch.autograd.Function):
@@ -947,27 +974,34 @@ def _deriv_dtype(dtype):
 
 
 def _matrix(t):
-    """(rows, matrix whose rows are contiguous and do not overlap, its row stride) of [..., columns]"""
+    """(matrix whose rows are contiguous and do not overlap, its row stride) of [..., columns]"""
     m = t if t.dim() == 2 else t.reshape(-1, t.shape[-1])
-    if (m.shape[1] > 1 and m.stride(1) != 1) or (m.shape[0] > 1 and m.stride(0) < m.shape[1]):
+    rows, cols = m.shape
+    s0, s1 = m.stride()
+    if (s1 != 1 and cols > 1) or (s0 < cols and rows > 1):
         m = m.contiguous()
-    return m.shape[0], m, max(m.stride(0), m.shape[1])
+        s0 = m.stride(0)
+    return m, s0 if s0 > cols else cols
 
 
-def _linear_inputs(name, x, weight, others):
-    _need(x.dtype in _DTYPES, f"{name}: x is float32, bfloat16 or float16, not {x.dtype}")
-    _need(isinstance(weight, torch.Tensor) and weight.dim() == 2 and x.dim() >= 1 and x.shape[-1] == weight.shape[1],
-          f"{name}: x [..., inputs] and weight [outputs, inputs]")
-    _need(weight.shape[0] >= 1 and weight.shape[1] >= 1, f"{name}: at least one input and one output")
+def _linear_inputs(name, x, weight):
+    """(rows, inputs, outputs)"""
+    if x.dtype not in _DTYPES:
+        _refuse(f"{name}: x is float32, bfloat16 or float16, not {x.dtype}")
+    if not isinstance(weight, torch.Tensor) or weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1] or weight.dtype != x.dtype:
+        _refuse(f"{name}: x [..., inputs] and weight [outputs, inputs] of one type")
     n, k = weight.shape
-    for what, t, shape in others:
-        _need(t is None or (isinstance(t, torch.Tensor) and tuple(t.shape) == tuple(shape)), f"{name}: {what} is not {tuple(shape)}")
-    for what, t in [("weight", weight)] + [(what, t) for what, t, _ in others]:
-        dtype = _deriv_dtype(x.dtype) if what == "deriv" else x.dtype
-        _need(t is None or t.dtype == dtype, f"{name}: {what} is {dtype} where x is {x.dtype}")
+    if n < 1 or k < 1:
+        _refuse(f"{name}: at least one input and one output")
     rows = x.numel() // k
-    _need(max(rows, n, k) <= _LINEAR_MOST and max(rows * n, rows * k, n * k) < 1 << 38, f"{name}: sizes beyond {_LINEAR_MOST} or 2^38 elements")
-    _device_tensors(name, x, weight, *[t for _, t, _ in others])
+    if max(rows, n, k) > _LINEAR_MOST or max(rows * n, rows * k, n * k) >= 1 << 38:
+        _refuse(f"{name}: sizes beyond {_LINEAR_MOST} or 2^38 elements")
+    return rows, k, n
+
+
+def _linear_operand(name, what, t, shape, dtype):
+    if t is not None and (not isinstance(t, torch.Tensor) or t.shape != shape or t.dtype != dtype):
+        _refuse(f"{name}: {what} is {dtype} of shape {tuple(shape)}")
 
 
 @_on_tensor_device
@@ -977,27 +1011,30 @@ def linear_act_fwd(x, weight, bias=None, activation="none", residual=None, want_
     f32.  deriv (want_deriv, and an activation) is act'(z) for linear_act_bwd, f16 for bf16 layers and f32 for others, else None."""
     lib = _lib.load()
     name = "linear_act"
-    _need(activation in ACTIVATIONS, f"{name}: activation is one of {sorted(ACTIVATIONS)}")
-    _need(isinstance(weight, torch.Tensor) and weight.dim() == 2, f"{name}: weight is [outputs, inputs]")
-    n, k = weight.shape
-    shape = (*x.shape[:-1], n)
-    _linear_inputs(name, x, weight, [("bias", bias, (n,)), ("residual", residual, shape)])
-    rows, xm, xs = _matrix(x)
-    _, wm, ws_ = _matrix(weight)
-    bias = None if bias is None else bias.contiguous()
-    rm, rs = None, 0
-    if residual is not None:
-        _, rm, rs = _matrix(residual)
-    y = torch.empty(shape, dtype=x.dtype, device=x.device)
-    deriv = torch.empty(shape, dtype=_deriv_dtype(x.dtype), device=x.device) if want_deriv and activation != "none" else None
+    if activation not in ACTIVATIONS:
+        _refuse(f"{name}: activation is one of {sorted(ACTIVATIONS)}")
+    rows, k, n = _linear_inputs(name, x, weight)
+    dtype, shape = x.dtype, (*x.shape[:-1], n)
+    _linear_operand(name, "bias", bias, (n,), dtype)
+    _linear_operand(name, "residual", residual, shape, dtype)
+    _device_tensors(name, x, weight, bias, residual)
+    dev = x.device
+    y = torch.empty(shape, dtype=dtype, device=dev)
+    deriv = torch.empty(shape, dtype=_deriv_dtype(dtype), device=dev) if want_deriv and activation != "none" else None
     if rows == 0:
         return y, deriv
-    dt = _DTYPES[x.dtype]
+    xm, xs = _matrix(x)
+    wm, ws_ = _matrix(weight)
+    rm, rs = (None, 0) if residual is None else _matrix(residual)
+    if bias is not None:
+        bias = bias.contiguous()
+    dt = _DTYPES[dtype]
     nws = lib.ppo_linear_act_fwd_workspace_bytes(rows, k, n, dt)
-    ws = torch.empty(nws, dtype=torch.uint8, device=x.device) if nws else None
+    ws = torch.empty(nws, dtype=torch.uint8, device=dev) if nws else None
     rc = lib.ppo_linear_act_fwd(xm.data_ptr(), xs, wm.data_ptr(), ws_, _ptr(bias), _ptr(rm), rs, dt, rows, k, n, ACTIVATIONS[activation],
                                 y.data_ptr(), _ptr(deriv), _ptr(ws), nws, _stream())
-    _lib.check(rc, "ppo_linear_act_fwd")
+    if rc:
+        _lib.check(rc, "ppo_linear_act_fwd")
     return y, deriv
 
 
@@ -1008,25 +1045,30 @@ def linear_act_bwd(g, x, weight, deriv=None, want_input=True, want_weight=True, 
     is g itself.)"""
     lib = _lib.load()
     name = "linear_act_bwd"
-    _need(isinstance(x, torch.Tensor) and isinstance(weight, torch.Tensor) and weight.dim() == 2, f"{name}: x [..., inputs] and weight [outputs, inputs]")
-    n, k = weight.shape
-    shape = (*x.shape[:-1], n)
-    _linear_inputs(name, x, weight, [("g", g, shape), ("deriv", deriv, shape)])
-    rows, gm, gs = _matrix(g)
-    _, xm, xs = _matrix(x)
-    _, wm, ws_ = _matrix(weight)
-    make = lambda want, s: torch.empty(s, dtype=x.dtype, device=x.device) if want else None  # noqa: E731
-    g_x, g_w, g_b = make(want_input, x.shape), make(want_weight, (n, k)), make(want_bias, (n,))
+    if not isinstance(x, torch.Tensor):
+        _refuse(f"{name}: x [..., inputs] and weight [outputs, inputs] of one type")
+    rows, k, n = _linear_inputs(name, x, weight)
+    dtype, shape, dev = x.dtype, (*x.shape[:-1], n), x.device
+    _linear_operand(name, "g", g, shape, dtype)
+    _linear_operand(name, "deriv", deriv, shape, _deriv_dtype(dtype))
+    _device_tensors(name, x, weight, g, deriv)
+    g_x = torch.empty(x.shape, dtype=dtype, device=dev) if want_input else None
+    g_w = torch.empty((n, k), dtype=dtype, device=dev) if want_weight else None
+    g_b = torch.empty((n,), dtype=dtype, device=dev) if want_bias else None
     if rows == 0:
         return g_x, None if g_w is None else g_w.zero_(), None if g_b is None else g_b.zero_()
+    gm, gs = _matrix(g)
+    xm, xs = _matrix(x)
+    wm, ws_ = _matrix(weight)
     if deriv is not None:
         deriv = deriv.contiguous()
-    dt = _DTYPES[x.dtype]
+    dt = _DTYPES[dtype]
     nws = lib.ppo_linear_act_bwd_workspace_bytes(rows, k, n, dt)
-    ws = torch.empty(nws, dtype=torch.uint8, device=x.device)
+    ws = torch.empty(nws, dtype=torch.uint8, device=dev)
     rc = lib.ppo_linear_act_bwd(gm.data_ptr(), gs, xm.data_ptr(), xs, wm.data_ptr(), ws_, _ptr(deriv), dt, rows, k, n, _ptr(g_x), _ptr(g_w),
                                 _ptr(g_b), ws.data_ptr(), nws, _stream())
-    _lib.check(rc, "ppo_linear_act_bwd")
+    if rc:
+        _lib.check(rc, "ppo_linear_act_bwd")
     return g_x, g_w, g_b
 
 

@@ -66,15 +66,17 @@ def test_c_entries_refuse():
     assert bwd(b=0) == 0
     for kw in ({"st": None}, {"H": None}, {"gl": None, "gh": None}, {"g": None}, {"g": p + 2}, {"A": 0}, {"t": -1.0}, {"A": 1 << 40, "b": 1 << 20}):
         assert bwd(**kw) == INVALID, kw
-    n = lib.ppo_policy_kl_loss_workspace_bytes(2)
-    pol = lambda lp=p, s=4, adv=p, mask=p, b=2, n_=4, lo=0.2, hi=0.2, c=0.1, kl=3, out=p, g=p, ws=p, nws=n: lib.ppo_policy_kl_loss(  # noqa: E731
+    assert lib.ppo_policy_kl_loss_workspace_bytes(2, 4) == 0
+    n = lib.ppo_policy_kl_loss_workspace_bytes(2, 1 << 16)
+    pol = lambda lp=p, s=1 << 16, adv=p, mask=p, b=2, n_=1 << 16, lo=0.2, hi=0.2, c=0.1, kl=3, out=p, g=p, ws=p, nws=n: lib.ppo_policy_kl_loss(  # noqa: E731
         lp, s, p, 4, adv, 4, 0, p, 4, mask, 4, b, n_, lo, hi, c, kl, 0, out, g, ws, nws, None)
     for kw in ({"lp": None}, {"lp": p + 2}, {"s": -1}, {"adv": None}, {"b": 0}, {"n_": 0}, {"b": 1 << 32}, {"n_": 1 << 31}, {"lo": 1.0}, {"lo": -0.5}, {"hi": -1.0},
                {"hi": float("inf")}, {"c": float("nan")}, {"kl": 0}, {"kl": 4}, {"out": None}, {"g": p + 1}, {"ws": None}, {"nws": n - 1}, {"ws": p + 4}):
         assert pol(**kw) == INVALID, kw
-    n = lib.ppo_preference_loss_workspace_bytes(2, 4, 4)
-    pref = lambda c=p, s=4, L=4, b=2, kind=0, beta=0.1, eps=0.0, out=p, rew=p, ws=p, nws=n: lib.ppo_preference_loss(  # noqa: E731
-        c, s, p, 4, p, 4, L, p, 4, p, 4, p, 4, 4, b, kind, beta, eps, 0, out, rew, p, p, ws, nws, None)
+    assert lib.ppo_preference_loss_workspace_bytes(2, 4, 4) == 0
+    n = lib.ppo_preference_loss_workspace_bytes(2, 1 << 16, 1 << 16)
+    pref = lambda c=p, s=1 << 16, L=1 << 16, b=2, kind=0, beta=0.1, eps=0.0, out=p, rew=p, ws=p, nws=n: lib.ppo_preference_loss(  # noqa: E731
+        c, s, p, 4, p, 4, L, p, 4, p, 4, p, 4, 1 << 16, b, kind, beta, eps, 0, out, rew, p, p, ws, nws, None)
     for kw in ({"c": None}, {"c": p + 2}, {"s": -1}, {"L": -1}, {"b": 0}, {"b": 1 << 29}, {"kind": 3}, {"beta": 0.0}, {"beta": float("nan")}, {"eps": 0.5},
                {"out": None}, {"rew": None}, {"ws": None}, {"nws": n - 1}):
         assert pref(**kw) == INVALID, kw
