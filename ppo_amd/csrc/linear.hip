@@ -229,18 +229,25 @@ template <class T> __global__ void __launch_bounds__(256) k_prep(PrepArgs a)
     }
 }
 
-template <class T> __global__ void __launch_bounds__(256) k_bias_grad(const float *sums, long tiles, long C, typename T::raw *out)
+// 64 columns a workgroup, its 16 waves share the tiles of rows
+template <class T> __global__ void __launch_bounds__(1024) k_bias_grad(const float *sums, long tiles, long C, typename T::raw *out)
 {
-    // 64 columns a workgroup, four waves share the tiles of rows
-    __shared__ float part[4][64];
-    const long c = (long)blockIdx.x * 64 + (threadIdx.x & 63);
-    const int w = threadIdx.x >> 6;
+    __shared__ float part[16][64];
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    const long c = (long)blockIdx.x * 64 + lane;
     float s = 0.0f;
-    if (c < C)
-        for (long t = w; t < tiles; t += 4) s += sums[t * C + c];
-    part[w][threadIdx.x & 63] = s;
+    if (c < C) {
+#pragma unroll 4
+        for (long t = w; t < tiles; t += 16) s += sums[t * C + c];
+    }
+    part[w][lane] = s;
     __syncthreads();
-    if (w == 0 && c < C) out[c] = T::store((part[0][threadIdx.x] + part[1][threadIdx.x]) + (part[2][threadIdx.x] + part[3][threadIdx.x]));
+    if (w == 0 && c < C) {
+        s = 0.0f;
+#pragma unroll
+        for (int k = 0; k < 16; ++k) s += part[k][lane];
+        out[c] = T::store(s);
+    }
 }
 
 // ---- the product -----------------------------------------------------------------------------------------------------
@@ -264,31 +271,26 @@ template <class T> __device__ __forceinline__ void finish(const GemmArgs &g, lon
     if (g.residual) y += T::load(reinterpret_cast<const raw *>(g.residual)[m * g.res_ld + n]);
 }
 
-// CNT (at most 16) neighbouring results of row m
-template <class T, int CNT> __device__ __forceinline__ void epilogue(const GemmArgs &g, long m, long n, const float (&z)[CNT])
+// 16 bytes of neighbouring results of row m; `bias` is theirs
+template <class T> __device__ __forceinline__ void epilogue(const GemmArgs &g, long m, long n, const float (&z)[16 / T::BYTES], const float (&bias)[16 / T::BYTES])
 {
     using raw = typename T::raw;
     constexpr int E = 16 / T::BYTES;
-    if (m >= g.M || n >= g.N) return;
     raw *out = reinterpret_cast<raw *>(g.out) + m * g.N + n;
     typename D<T>::raw *der = g.deriv ? reinterpret_cast<typename D<T>::raw *>(g.deriv) + m * g.N + n : nullptr;
-    if (n + CNT <= g.N) {
+    if (n + E <= g.N) {
+        float r[E], y[E], d[E];
+        if (g.residual) load16<T>(reinterpret_cast<const raw *>(g.residual) + m * g.res_ld + n, r);
 #pragma unroll
-        for (int q = 0; q < CNT; q += E) {
-            float b[E], r[E], y[E], d[E];
-            if (g.bias) load16<T>(reinterpret_cast<const raw *>(g.bias) + n + q, b);
-            if (g.residual) load16<T>(reinterpret_cast<const raw *>(g.residual) + m * g.res_ld + n + q, r);
-#pragma unroll
-            for (int j = 0; j < E; ++j) {
-                activate<T::BYTES == 2>(g.act, g.bias ? z[q + j] + b[j] : z[q + j], y[j], d[j]);
-                if (g.residual) y[j] += r[j];
-            }
-            store16<T>(out + q, y);
-            if (der) store_n<D<T>, E>(der + q, d);
+        for (int j = 0; j < E; ++j) {
+            activate<T::BYTES == 2>(g.act, z[j] + bias[j], y[j], d[j]);
+            if (g.residual) y[j] += r[j];
         }
+        store16<T>(out, y);
+        if (der) store_n<D<T>, E>(der, d);
     } else {
 #pragma unroll
-        for (int j = 0; j < CNT; ++j) {
+        for (int j = 0; j < E; ++j) {
             if (n + j < g.N) {
                 float y, d;
                 finish<T>(g, m, n + j, z[j], y, d);
@@ -297,6 +299,14 @@ template <class T, int CNT> __device__ __forceinline__ void epilogue(const GemmA
             }
         }
     }
+}
+
+template <class T> __device__ __forceinline__ void load_bias(const GemmArgs &g, long n, float (&bias)[16 / T::BYTES])
+{
+    constexpr int E = 16 / T::BYTES;
+    const typename T::raw *p = reinterpret_cast<const typename T::raw *>(g.bias);
+#pragma unroll
+    for (int j = 0; j < E; ++j) bias[j] = p && n + j < g.N ? T::load(p[n + j]) : 0.0f;
 }
 
 // Swizzles: piece c (16 bytes) of a row of 128 bytes lies at c ^ f(row) in LDS.  A ds_read_b128 is served 16 lanes a cycle
@@ -526,34 +536,48 @@ __global__ void __launch_bounds__(64 * WAVES_M * WAVES_N) k_gemm(GemmArgs g)
         }
     }
 
-    // acc[i][j][e] is C[m0 + wm WM + 16 i + q][n0 + wn WN + 16 kg + 4 j + e].  One row of products at a time in a loop, the
-    // others moving down a place: unrolled, the activations' code would be there MI times (90 KB of it)
-    const long n1 = n0 + wn * WN + kg * 16;
-    long m = m0 + wm * WM + q;
+    // acc[i][j][e] is C[m0 + wm WM + 16 i + q][n0 + wn WN + 16 kg + 4 j + e].  The results go through LDS, PI rows of
+    // products of every wave at a time, so that a wave finishes and stores whole rows: from the accumulators' layout a
+    // store touched 32 cache lines, and each residual and derivative as many again.  (A pad of 16 bytes a row puts the 16
+    // rows of a write into different banks.)
+    constexpr int E = 16 / T::BYTES, PI = 4, ROWS = WAVES_M * 16 * PI, LD = BN * 4 + 16, LANES = BN / E, STEP = 64 * WAVES / LANES;
+    static_assert(MI % PI == 0 && ROWS * LD <= 3 * A_STAGE + 2 * B_STAGE, "the results' rows fit");
+    const int col = threadIdx.x % LANES * E, row0 = threadIdx.x / LANES;
+    const long nn = n0 + col;
+    float bias[E];
+    load_bias<T>(g, nn, bias);
+#pragma unroll
+    for (int pass = 0; pass < MI / PI; ++pass) {
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < PI; ++i)
+#pragma unroll
+            for (int j = 0; j < NI; ++j)
+                *reinterpret_cast<f32x4 *>(lds + ((wm * PI + i) * 16 + q) * LD + (wn * WN + kg * 16 + j * 4) * 4) = acc[pass * PI + i][j];
+        __syncthreads();
 #pragma clang loop unroll(disable)
-    for (int i = 0; i < MI; ++i, m += 16) {
-        float z[16];
+        for (int r = row0; r < ROWS; r += STEP) {
+            const long m = m0 + r / (16 * PI) * WM + pass * 16 * PI + r % (16 * PI);
+            if (m >= g.M || nn >= g.N) continue;
+            float z[E];
 #pragma unroll
-        for (int j = 0; j < NI; ++j)
+            for (int j = 0; j < E; j += 4) {
+                const f32x4 v = *reinterpret_cast<const f32x4 *>(lds + r * LD + (col + j) * 4);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) z[j * 4 + e] = acc[0][j][e];
-#pragma unroll
-        for (int k = 0; k + 1 < MI; ++k)
-#pragma unroll
-            for (int j = 0; j < NI; ++j) acc[k][j] = acc[k + 1][j];
-        if (g.partial) {
-            if (m < g.M && n1 < g.N) {
-                float *p = g.partial + ((long)blockIdx.y * g.M + m) * g.N + n1;
-                if (n1 + 16 <= g.N) {
-                    store_n<F32, 16>(p, z);
+                for (int e = 0; e < 4; ++e) z[j + e] = v[e];
+            }
+            if (g.partial) {
+                float *p = g.partial + ((long)blockIdx.y * g.M + m) * g.N + nn;
+                if (nn + E <= g.N) {
+                    store_n<F32, E>(p, z);
                 } else {
 #pragma unroll
-                    for (int e = 0; e < 16; ++e)
-                        if (n1 + e < g.N) p[e] = z[e];
+                    for (int e = 0; e < E; ++e)
+                        if (nn + e < g.N) p[e] = z[e];
                 }
+            } else {
+                epilogue<T>(g, m, nn, z, bias);
             }
-        } else {
-            epilogue<T, 16>(g, m, n1, z);
         }
     }
 }
@@ -585,7 +609,9 @@ template <class T> __global__ void __launch_bounds__(256) k_join(GemmArgs g, int
                 if (j < have) z[j] += p[j];
         }
     }
-    epilogue<T, E>(g, m, n, z);
+    float bias[E];
+    load_bias<T>(g, n, bias);
+    epilogue<T>(g, m, n, z, bias);
 }
 
 // ---- few rows: the weights are read once, by the vector units --------------------------------------------------------
@@ -824,7 +850,7 @@ int ppo_linear_act_bwd(const void *g_y, long g_stride, const void *x, long x_str
             rc = prep<T>(g_y, g_stride, deriv, rows, outputs, want_rows ? u : nullptr, g_weight ? ut : nullptr, g_bias ? sums : nullptr, s);
         if (!rc && g_bias) {
             const long tiles = ((g_weight ? Mp : rows) + 63) / 64;
-            hipLaunchKernelGGL(k_bias_grad<T>, dim3((unsigned)((outputs + 63) / 64)), dim3(256), 0, s, sums, tiles, outputs,
+            hipLaunchKernelGGL(k_bias_grad<T>, dim3((unsigned)((outputs + 63) / 64)), dim3(1024), 0, s, sums, tiles, outputs,
                                reinterpret_cast<typename T::raw *>(g_bias));
             rc = ppo_launch_status();
         }
