@@ -152,12 +152,14 @@ template <class T, int N> __device__ __forceinline__ void store_n(typename T::ra
 
 // ---- operand preparation: pad, multiply by d, transpose, sum columns -----------------------------------------------
 // src [R, C] of T with row stride ld (times mul [R, C] of D<T>, contiguous) -> rows [R, Cp] and / or cols [C, Rp] of T, Cp and Rp
-// the next multiples of a k step, zero-filled; sums [tiles of 64 rows][C] f32 = column sums of a tile.
+// the next multiples of a k step, zero-filled; sums [tiles of 64 rows][C] f32 = column sums of a tile.  pad_rows: `rows`
+// gets Rp of them, for use along k.
 struct PrepArgs {
     const void *src, *mul;
     void *rows, *cols;
     float *sums;
     long R, C, ld, Rp, Cp;
+    int pad_rows;
 };
 
 template <class T> __global__ void __launch_bounds__(256) k_prep(PrepArgs a)
@@ -198,7 +200,7 @@ template <class T> __global__ void __launch_bounds__(256) k_prep(PrepArgs a)
         }
 #pragma unroll
         for (int j = 0; j < E; ++j) sum[j] += v[j];
-        if (a.rows && gr < a.R && gc < a.Cp) store16<T>(reinterpret_cast<raw *>(a.rows) + gr * a.Cp + gc, v);
+        if (a.rows && gr < (a.pad_rows ? a.Rp : a.R) && gc < a.Cp) store16<T>(reinterpret_cast<raw *>(a.rows) + gr * a.Cp + gc, v);
         if (a.cols) {
 #pragma unroll
             for (int j = 0; j < E; ++j) tile[r][tc + j] = T::store(v[j]);
@@ -337,9 +339,12 @@ __device__ __forceinline__ u32x4 buffer_of(const void *p, long bytes)
                  (uint32_t)__builtin_amdgcn_readfirstlane((int)n), 0x00027000u};
 }
 
-template <class T, int BM, int BN, int WAVES_M, int WAVES_N>
+// KA, KB: that operand lies [k, M] (or [k, N]) with its rows along k (f32 only: the 16-bit fragments' eight k would have to
+// be gathered in 2-byte reads)
+template <class T, int BM, int BN, int WAVES_M, int WAVES_N, bool KA, bool KB>
 __global__ void __launch_bounds__(64 * WAVES_M * WAVES_N) k_gemm(GemmArgs g)
 {
+    static_assert((!KA && !KB) || T::BYTES == 4, "f32 only");
     constexpr int WAVES = WAVES_M * WAVES_N, WM = BM / WAVES_M, WN = BN / WAVES_N, MI = WM / 16, NI = 4;
     static_assert(WN == 64 && MI * 16 * WAVES_M == BM, "a lane's 16 neighbouring n need 64 columns a wave");
     constexpr int LA = BM / 8 / WAVES, LB = BN / 8 / WAVES;          // loads a wave and stage (8 rows each)
@@ -362,23 +367,50 @@ __global__ void __launch_bounds__(64 * WAVES_M * WAVES_N) k_gemm(GemmArgs g)
 
     const long kbytes = (long)g.steps * 128;
     const long rows_a = g.M - m0 < BM ? g.M - m0 : BM, rows_b = g.N - n0 < BN ? g.N - n0 : BN;
-    const u32x4 ra = buffer_of(reinterpret_cast<const char *>(g.A) + m0 * g.lda, (rows_a - 1) * g.lda + kbytes);
-    const u32x4 rb = buffer_of(reinterpret_cast<const char *>(g.B) + n0 * g.ldb, (rows_b - 1) * g.ldb + kbytes);
+    const char *pa0 = reinterpret_cast<const char *>(g.A) + (KA ? m0 * 4 : m0 * g.lda), *pb0 = reinterpret_cast<const char *>(g.B) + (KB ? n0 * 4 : n0 * g.ldb);
+    const u32x4 ra = buffer_of(pa0, KA ? 0 : (rows_a - 1) * g.lda + kbytes), rb = buffer_of(pb0, KB ? 0 : (rows_b - 1) * g.ldb + kbytes);
     uint32_t va[LA], vb[LB];           // (256 rows of less than 2^24 bytes: below 2^32)
 #pragma unroll
     for (int i = 0; i < LA; ++i) {
-        const int row = (i * WAVES + wave) * 8 + lane / 8, have = row < rows_a ? row : (int)rows_a - 1;   // rows past the end repeat the last
-        va[i] = (uint32_t)have * (uint32_t)g.lda + ((lane % 8) ^ swizzle_a<T::BYTES>(row)) * 16;
+        if constexpr (KA) {
+            // a row of LDS is one k: BM floats, whose 16-byte pieces are moved by 4 (k / 8), so that the four k groups of a
+            // fragment read fall into different banks
+            constexpr int PIECES = BM / 4;
+            const int k = (i * WAVES + wave) * (64 / PIECES) + lane / PIECES;
+            va[i] = (uint32_t)k * (uint32_t)g.lda + ((lane % PIECES) ^ (k >> 3) * 4) * 16;
+        } else {
+            const int row = (i * WAVES + wave) * 8 + lane / 8, have = row < rows_a ? row : (int)rows_a - 1;   // rows past the end repeat the last
+            va[i] = (uint32_t)have * (uint32_t)g.lda + ((lane % 8) ^ swizzle_a<T::BYTES>(row)) * 16;
+        }
     }
 #pragma unroll
     for (int i = 0; i < LB; ++i) {
-        const int row = (i * WAVES + wave) * 8 + lane / 8, have = row < rows_b ? row : (int)rows_b - 1;
-        vb[i] = (uint32_t)have * (uint32_t)g.ldb + ((lane % 8) ^ swizzle_b<T::BYTES>(row)) * 16;
+        if constexpr (KB) {
+            constexpr int PIECES = BN / 4;             // (B's rows are read 4 neighbours at a time, 16 apart: moved by k / 8)
+            const int k = (i * WAVES + wave) * (64 / PIECES) + lane / PIECES;
+            vb[i] = (uint32_t)k * (uint32_t)g.ldb + ((lane % PIECES) ^ (k >> 3)) * 16;
+        } else {
+            const int row = (i * WAVES + wave) * 8 + lane / 8, have = row < rows_b ? row : (int)rows_b - 1;
+            vb[i] = (uint32_t)have * (uint32_t)g.ldb + ((lane % 8) ^ swizzle_b<T::BYTES>(row)) * 16;
+        }
     }
     const uint32_t base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds;
-    // load i of a stage's A or B to the place that begins at `to`
-    auto load_a = [&](int s, int to, int i) { load_lds(ra, va[i], s * 128, base + wave * 1024 + to + i * WAVES * 1024); };
-    auto load_b = [&](int s, int to, int i) { load_lds(rb, vb[i], s * 128, base + wave * 1024 + B_AT + to + i * WAVES * 1024); };
+    // load i of a stage's A or B to the place that begins at `to`.  Along k a stage is 32 rows of the matrix; what is read
+    // past its last column is the next row's beginning, or nothing behind the last row, and reaches no result that is kept.
+    auto load_a = [&](int s, int to, int i) {
+        const uint32_t at = base + wave * 1024 + to + i * WAVES * 1024;
+        if constexpr (KA)
+            load_lds(buffer_of(pa0 + s * 32L * g.lda, (g.steps * 32L - s * 32L - 1) * g.lda + (g.M - m0) * 4), va[i], 0, at);
+        else
+            load_lds(ra, va[i], s * 128, at);
+    };
+    auto load_b = [&](int s, int to, int i) {
+        const uint32_t at = base + wave * 1024 + B_AT + to + i * WAVES * 1024;
+        if constexpr (KB)
+            load_lds(buffer_of(pb0 + s * 32L * g.ldb, (g.steps * 32L - s * 32L - 1) * g.ldb + (g.N - n0) * 4), vb[i], 0, at);
+        else
+            load_lds(rb, vb[i], s * 128, at);
+    };
     auto stage_a = [&](int s, int to) {
 #pragma unroll
         for (int i = 0; i < LA; ++i) load_a(s, to, i);
@@ -507,8 +539,7 @@ __global__ void __launch_bounds__(64 * WAVES_M * WAVES_N) k_gemm(GemmArgs g)
                 stage_b(s + 1, (now ^ 1) * B_STAGE);
             }
             const char *at_a = lds + now * A_STAGE, *at_b = lds + now * B_STAGE;
-            auto split = [&](const char *p0, const char *p1, u32x4(&f)[3]) {
-                const f32x4 lo = *reinterpret_cast<const f32x4 *>(p0), hi = *reinterpret_cast<const f32x4 *>(p1);
+            auto split = [&](f32x4 lo, f32x4 hi, u32x4(&f)[3]) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     uint32_t w0, w1, w2;
@@ -519,13 +550,46 @@ __global__ void __launch_bounds__(64 * WAVES_M * WAVES_N) k_gemm(GemmArgs g)
                 }
             };
             const int c = 2 * kg, ca0 = (c ^ xa) * 16, ca1 = ((c + 1) ^ xa) * 16, cb0 = (c ^ xb) * 16, cb1 = ((c + 1) ^ xb) * 16;
+            // eight k of one row: two pieces of it, or a float of each of eight rows of k
+            auto read_a = [&](int i, f32x4 &lo, f32x4 &hi) {
+                if constexpr (KA) {
+                    const char *p = at_a + kg * 8 * (BM * 4) + ((row_a + i * 16) ^ kg * 16) * 4;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        lo[e] = *reinterpret_cast<const float *>(p + e * (BM * 4));
+                        hi[e] = *reinterpret_cast<const float *>(p + (e + 4) * (BM * 4));
+                    }
+                } else {
+                    lo = *reinterpret_cast<const f32x4 *>(at_a + pa + i * 2048 + ca0);
+                    hi = *reinterpret_cast<const f32x4 *>(at_a + pa + i * 2048 + ca1);
+                }
+            };
+            auto read_b = [&](int j, f32x4 &lo, f32x4 &hi) {
+                if constexpr (KB) {
+                    const char *p = at_b + B_AT + kg * 8 * (BN * 4) + ((row_b + j * 4) ^ kg * 4) * 4;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        lo[e] = *reinterpret_cast<const float *>(p + e * (BN * 4));
+                        hi[e] = *reinterpret_cast<const float *>(p + (e + 4) * (BN * 4));
+                    }
+                } else {
+                    lo = *reinterpret_cast<const f32x4 *>(at_b + pb + j * 512 + cb0);
+                    hi = *reinterpret_cast<const f32x4 *>(at_b + pb + j * 512 + cb1);
+                }
+            };
             u32x4 fb[NI][3];
 #pragma unroll
-            for (int j = 0; j < NI; ++j) split(at_b + pb + j * 512 + cb0, at_b + pb + j * 512 + cb1, fb[j]);
+            for (int j = 0; j < NI; ++j) {
+                f32x4 lo, hi;
+                read_b(j, lo, hi);
+                split(lo, hi, fb[j]);
+            }
 #pragma unroll
             for (int i = 0; i < MI; ++i) {
+                f32x4 lo, hi;
                 u32x4 fa[3];
-                split(at_a + pa + i * 2048 + ca0, at_a + pa + i * 2048 + ca1, fa);
+                read_a(i, lo, hi);
+                split(lo, hi, fa);
 #pragma unroll
                 for (int t = 0; t < 6; ++t) {
                     constexpr int PA[6] = {0, 2, 1, 0, 1, 0}, PB[6] = {2, 0, 1, 1, 0, 0};   // small terms first
@@ -713,18 +777,19 @@ size_t partial_bytes(const Plan &p, long M, long N) { return p.splits > 1 ? roun
 
 bool in_place(const void *p, long ld, long K, long e) { return ppo_aligned(p, 16) && ld * e % 16 == 0 && K * e % 128 == 0 && ld <= MOST_K; }
 
-template <class T> int prep(const void *src, long ld, const void *mul, long R, long C, void *rows, void *cols, float *sums, hipStream_t s)
+template <class T>
+int prep(const void *src, long ld, const void *mul, long R, long C, void *rows, void *cols, float *sums, hipStream_t s, bool pad_rows = false)
 {
     constexpr long e = T::BYTES;
-    PrepArgs a{src, mul, rows, cols, sums, R, C, ld, k_padded(R, e), k_padded(C, e)};
+    PrepArgs a{src, mul, rows, cols, sums, R, C, ld, k_padded(R, e), k_padded(C, e), pad_rows};
     // whole k steps in both directions: what lies past the matrix becomes zero
-    const long gr = cols ? (a.Rp + 63) / 64 : (R + 63) / 64, gc = rows ? (a.Cp + 63) / 64 : (C + 63) / 64;
+    const long gr = cols || pad_rows ? (a.Rp + 63) / 64 : (R + 63) / 64, gc = rows ? (a.Cp + 63) / 64 : (C + 63) / 64;
     PPO_REQUIRE(gr < 65536 && gc < (1L << 31));
     hipLaunchKernelGGL(k_prep<T>, dim3((unsigned)gc, (unsigned)gr), dim3(256), 0, s, a);
     return ppo_launch_status();
 }
 
-template <class T> int gemm(GemmArgs g, const Plan &p, hipStream_t s)
+template <class T, bool KA, bool KB> int gemm(GemmArgs g, const Plan &p, hipStream_t s)
 {
     g.steps = p.steps;
     g.steps_per_split = p.per_split;
@@ -733,9 +798,9 @@ template <class T> int gemm(GemmArgs g, const Plan &p, hipStream_t s)
     if (p.splits == 1) g.partial = nullptr;
     const dim3 grid((unsigned)(p.tiles_m * p.tiles_n), (unsigned)p.splits);
     if (p.large)
-        hipLaunchKernelGGL((k_gemm<T, 256, 256, 2, 4>), grid, dim3(512), 0, s, g);
+        hipLaunchKernelGGL((k_gemm<T, 256, 256, 2, 4, KA, KB>), grid, dim3(512), 0, s, g);
     else
-        hipLaunchKernelGGL((k_gemm<T, 128, 128, 2, 2>), grid, dim3(256), 0, s, g);
+        hipLaunchKernelGGL((k_gemm<T, 128, 128, 2, 2, KA, KB>), grid, dim3(256), 0, s, g);
     int rc = ppo_launch_status();
     if (rc || p.splits == 1) return rc;
     constexpr long E = 16 / T::BYTES;
@@ -743,6 +808,9 @@ template <class T> int gemm(GemmArgs g, const Plan &p, hipStream_t s)
     hipLaunchKernelGGL(k_join<T>, dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, s, g, p.splits);
     return ppo_launch_status();
 }
+
+// an operand whose rows go along k: padded to whole k steps unless it is whole already
+bool in_place_along_k(const void *p, long ld, long R, long e) { return ppo_aligned(p, 16) && ld * e % 16 == 0 && R * e % 128 == 0 && ld <= MOST_K; }
 
 bool sizes_ok(long rows, long inputs, long outputs, int dtype)
 {
@@ -811,7 +879,7 @@ int ppo_linear_act_fwd(const void *x, long x_stride, const void *weight, long we
         }
         ws += round256((size_t)outputs * Kp * e);
         g.partial = reinterpret_cast<float *>(ws);
-        return gemm<T>(g, plan_of(rows, outputs, inputs, e), s);
+        return gemm<T, false, false>(g, plan_of(rows, outputs, inputs, e), s);
     });
 }
 
@@ -820,8 +888,10 @@ size_t ppo_linear_act_bwd_workspace_bytes(long rows, long inputs, long outputs, 
     if (!sizes_ok(rows, inputs, outputs, dtype)) return 0;
     const long e = dtype_bytes(dtype), Mp = k_padded(rows, e), Np = k_padded(outputs, e);
     const size_t px = partial_bytes(plan_of(rows, inputs, outputs, e), rows, inputs), pw = partial_bytes(plan_of(outputs, inputs, rows, e), outputs, inputs);
-    return round256((size_t)rows * Np * e) + round256((size_t)outputs * Mp * e) + round256((size_t)inputs * Np * e) +
-           round256((size_t)inputs * Mp * e) + round256((size_t)((Mp + 63) / 64) * outputs * 4) + (px > pw ? px : pw);
+    const long Kp = k_padded(inputs, e);
+    const size_t ut = e == 2 ? round256((size_t)outputs * Mp * e) : 0;
+    return round256((size_t)Mp * Np * e) + ut + round256((size_t)Kp * Np * e) + round256((size_t)Kp * Mp * e) +
+           round256((size_t)((Mp + 63) / 64) * outputs * 4) + (px > pw ? px : pw);
 }
 
 int ppo_linear_act_bwd(const void *g_y, long g_stride, const void *x, long x_stride, const void *weight, long weight_stride,
@@ -837,36 +907,68 @@ int ppo_linear_act_bwd(const void *g_y, long g_stride, const void *x, long x_str
     hipStream_t s = (hipStream_t)stream;
     return by_dtype(dtype, [&](auto t) {
         using T = decltype(t);
-        const long Mp = k_padded(rows, e), Np = k_padded(outputs, e);
+        const long Mp = k_padded(rows, e), Np = k_padded(outputs, e), Kp = k_padded(inputs, e);
         char *ws = reinterpret_cast<char *>(workspace);
         auto take = [&](size_t n) { char *p = ws; ws += round256(n); return p; };
-        char *u = take((size_t)rows * Np * e), *ut = take((size_t)outputs * Mp * e), *wt = take((size_t)inputs * Np * e), *xt = take((size_t)inputs * Mp * e);
+        char *u = take((size_t)Mp * Np * e), *ut = e == 2 ? take((size_t)outputs * Mp * e) : nullptr, *wt = take((size_t)Kp * Np * e), *xt = take((size_t)Kp * Mp * e);
         float *sums = reinterpret_cast<float *>(take((size_t)((Mp + 63) / 64) * outputs * 4));
         float *partial = reinterpret_cast<float *>(ws);
-        const bool as_is = !deriv && in_place(g_y, g_stride, outputs, e);
-        const bool want_rows = g_x && !as_is;
+        GemmArgs gx{}, gw{};
+        gx.M = rows; gx.N = inputs; gx.out = g_x; gx.act = PPO_ACT_NONE; gx.partial = partial;
+        gw.M = outputs; gw.N = inputs; gw.out = g_weight; gw.act = PPO_ACT_NONE; gw.partial = partial;
+        const Plan plan_x = plan_of(rows, inputs, outputs, e), plan_w = plan_of(outputs, inputs, rows, e);
+        const bool row_in_place = !deriv && in_place(g_y, g_stride, outputs, e);   // g_x's A
         int rc = 0;
-        if (want_rows || g_weight || g_bias)
-            rc = prep<T>(g_y, g_stride, deriv, rows, outputs, want_rows ? u : nullptr, g_weight ? ut : nullptr, g_bias ? sums : nullptr, s);
-        if (!rc && g_bias) {
-            const long tiles = ((g_weight ? Mp : rows) + 63) / 64;
-            hipLaunchKernelGGL(k_bias_grad<T>, dim3((unsigned)((outputs + 63) / 64)), dim3(1024), 0, s, sums, tiles, outputs,
-                               reinterpret_cast<typename T::raw *>(g_bias));
-            rc = ppo_launch_status();
-        }
-        if (!rc && g_x) {
-            rc = prep<T>(weight, weight_stride, nullptr, outputs, inputs, nullptr, wt, nullptr, s);
-            GemmArgs g{};
-            g.A = as_is ? g_y : u; g.lda = (as_is ? g_stride : Np) * e; g.B = wt; g.ldb = Np * e;
-            g.M = rows; g.N = inputs; g.out = g_x; g.act = PPO_ACT_NONE; g.partial = partial;
-            if (!rc) rc = gemm<T>(g, plan_of(rows, inputs, outputs, e), s);
-        }
-        if (!rc && g_weight) {
-            rc = prep<T>(x, x_stride, nullptr, rows, inputs, nullptr, xt, nullptr, s);
-            GemmArgs g{};
-            g.A = ut; g.lda = Mp * e; g.B = xt; g.ldb = Mp * e;
-            g.M = outputs; g.N = inputs; g.out = g_weight; g.act = PPO_ACT_NONE; g.partial = partial;
-            if (!rc) rc = gemm<T>(g, plan_of(outputs, inputs, rows, e), s);
+        if constexpr (T::BYTES == 4) {
+            // u and W and x are read along k as they lie
+            const bool col_in_place = !deriv && in_place_along_k(g_y, g_stride, rows, e);
+            const bool write_u = (g_x && !row_in_place) || (g_weight && !col_in_place);
+            if (write_u || g_bias)
+                rc = prep<T>(g_y, g_stride, deriv, rows, outputs, write_u ? u : nullptr, nullptr, g_bias ? sums : nullptr, s, write_u);
+            if (!rc && g_bias) {
+                const long tiles = ((write_u ? Mp : rows) + 63) / 64;
+                hipLaunchKernelGGL(k_bias_grad<T>, dim3((unsigned)((outputs + 63) / 64)), dim3(1024), 0, s, sums, tiles, outputs,
+                                   reinterpret_cast<typename T::raw *>(g_bias));
+                rc = ppo_launch_status();
+            }
+            if (!rc && g_x) {
+                gx.A = row_in_place ? g_y : u; gx.lda = (row_in_place ? g_stride : Np) * e;
+                gx.B = weight; gx.ldb = weight_stride * e;
+                if (!in_place_along_k(weight, weight_stride, outputs, e)) {
+                    rc = prep<T>(weight, weight_stride, nullptr, outputs, inputs, wt, nullptr, nullptr, s, true);
+                    gx.B = wt; gx.ldb = Kp * e;
+                }
+                if (!rc) rc = gemm<T, false, true>(gx, plan_x, s);
+            }
+            if (!rc && g_weight) {
+                gw.A = col_in_place ? g_y : u; gw.lda = (col_in_place ? g_stride : Np) * e;
+                gw.B = x; gw.ldb = x_stride * e;
+                if (!in_place_along_k(x, x_stride, rows, e)) {
+                    rc = prep<T>(x, x_stride, nullptr, rows, inputs, xt, nullptr, nullptr, s, true);
+                    gw.B = xt; gw.ldb = Kp * e;
+                }
+                if (!rc) rc = gemm<T, true, true>(gw, plan_w, s);
+            }
+        } else {
+            const bool want_rows = g_x && !row_in_place;
+            if (want_rows || g_weight || g_bias)
+                rc = prep<T>(g_y, g_stride, deriv, rows, outputs, want_rows ? u : nullptr, g_weight ? ut : nullptr, g_bias ? sums : nullptr, s);
+            if (!rc && g_bias) {
+                const long tiles = ((g_weight ? Mp : rows) + 63) / 64;
+                hipLaunchKernelGGL(k_bias_grad<T>, dim3((unsigned)((outputs + 63) / 64)), dim3(1024), 0, s, sums, tiles, outputs,
+                                   reinterpret_cast<typename T::raw *>(g_bias));
+                rc = ppo_launch_status();
+            }
+            if (!rc && g_x) {
+                rc = prep<T>(weight, weight_stride, nullptr, outputs, inputs, nullptr, wt, nullptr, s);
+                gx.A = row_in_place ? g_y : u; gx.lda = (row_in_place ? g_stride : Np) * e; gx.B = wt; gx.ldb = Np * e;
+                if (!rc) rc = gemm<T, false, false>(gx, plan_x, s);
+            }
+            if (!rc && g_weight) {
+                rc = prep<T>(x, x_stride, nullptr, rows, inputs, nullptr, xt, nullptr, s);
+                gw.A = ut; gw.lda = Mp * e; gw.B = xt; gw.ldb = Mp * e;
+                if (!rc) rc = gemm<T, false, false>(gw, plan_w, s);
+            }
         }
         return rc;
     });

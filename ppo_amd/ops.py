@@ -755,10 +755,9 @@ def token_logprobs_fwd(logits, actions, temperature=1.0, ignore_index=-100, want
     gives NaN.  stats [..., 2] is what token_logprobs_bwd needs."""
     lib = _lib.load()
     lg, act, batch, length, bs, ts = _token_rows("token_logprobs", logits, actions, temperature)
-    shape, dev = act.shape, lg.device
-    logp = torch.empty(shape, dtype=torch.float32, device=dev)
-    entropy = torch.empty(shape, dtype=torch.float32, device=dev) if want_entropy else None
-    stats = torch.empty((*shape, 2), dtype=torch.float32, device=dev)
+    logp = torch.empty_like(act, dtype=torch.float32)      # (act is contiguous; the _like and new_ forms cost half of torch.empty)
+    entropy = torch.empty_like(logp) if want_entropy else None
+    stats = logp.new_empty(*act.shape, 2)
     rc = lib.ppo_token_logprobs_fwd(lg.data_ptr(), _DTYPES[lg.dtype], batch, length, lg.shape[-1], bs, ts, act.data_ptr(),
                                     act.element_size(), temperature, ignore_index, logp.data_ptr(), _ptr(entropy),
                                     stats.data_ptr(), _stream())
@@ -787,7 +786,7 @@ def token_logprobs_bwd(logits, actions, stats, entropy, g_logp, g_entropy=None, 
             _refuse(f"{name}: entropy and gradients are float32 of the actions' shape")
         rows.append(None if t is None else t.contiguous())
     _device_tensors(name, lg, stats, *rows)
-    g = torch.empty(logits.shape, dtype=lg.dtype, device=lg.device)
+    g = torch.empty_like(logits, memory_format=torch.contiguous_format)
     rc = lib.ppo_token_logprobs_bwd(lg.data_ptr(), _DTYPES[lg.dtype], batch, length, lg.shape[-1], bs, ts, act.data_ptr(),
                                     act.element_size(), stats.data_ptr(), *[_ptr(t) for t in rows], temperature, ignore_index,
                                     g.data_ptr(), _stream())
@@ -868,13 +867,12 @@ def policy_kl_loss_fwd_bwd(new_lp, old_lp, adv, mask=None, ref_lp=None, clip_low
     per_sequence = isinstance(adv, torch.Tensor) and adv.dim() == 1
     a, a_s = _sequence_rows(name, "adv", adv, shape[:1] if per_sequence else shape)
     _device_tensors(name, new, old, ref, msk, a)
-    dev = new.device
-    g = torch.empty(shape, dtype=torch.float32, device=dev) if want_grad else None
+    g = torch.empty_like(new, memory_format=torch.contiguous_format) if want_grad else None
     if B == 0 or L == 0:
-        return torch.zeros(6, dtype=torch.float32, device=dev), g
-    out6 = torch.empty(6, dtype=torch.float32, device=dev)
+        return new.new_zeros(6), g
+    out6 = new.new_empty(6)
     nws = lib.ppo_policy_kl_loss_workspace_bytes(B, L)
-    ws = torch.empty(nws, dtype=torch.uint8, device=dev) if nws else None
+    ws = new.new_empty((nws + 3) // 4) if nws else None
     rc = lib.ppo_policy_kl_loss(new.data_ptr(), new_s, old.data_ptr(), old_s, a.data_ptr(), a_s, per_sequence, _ptr(ref),
                                 ref_s, _ptr(msk), msk_s, B, L, clip_low, clip_high, kl_coef, KL_KINDS[kl], reduction == "sequence",
                                 out6.data_ptr(), _ptr(g), _ptr(ws), nws, _stream())
@@ -920,15 +918,14 @@ def preference_loss_fwd_bwd(chosen_lp, rejected_lp, ref_chosen_lp=None, ref_reje
     rr, rr_s = _sequence_rows(name, "ref_rejected_lp", ref_rejected_lp, rs)
     mr, mr_s = _sequence_rows(name, "rejected_mask", rejected_mask, rs, True)
     _device_tensors(name, c, rc_, mc, r, rr, mr)
-    dev = c.device
-    g_c = torch.empty(cs, dtype=torch.float32, device=dev) if want_grad else None
-    g_r = torch.empty(rs, dtype=torch.float32, device=dev) if want_grad else None
-    rewards = torch.empty((pairs, 2), dtype=torch.float32, device=dev)
+    g_c = torch.empty_like(c, memory_format=torch.contiguous_format) if want_grad else None
+    g_r = torch.empty_like(r, memory_format=torch.contiguous_format) if want_grad else None
+    rewards = c.new_empty(pairs, 2)
     if pairs == 0:
-        return torch.zeros(2, dtype=torch.float32, device=dev), rewards, g_c, g_r
-    out2 = torch.empty(2, dtype=torch.float32, device=dev)
+        return c.new_zeros(2), rewards, g_c, g_r
+    out2 = c.new_empty(2)
     nws = lib.ppo_preference_loss_workspace_bytes(pairs, cs[1], rs[1])
-    ws = torch.empty(nws, dtype=torch.uint8, device=dev) if nws else None
+    ws = c.new_empty((nws + 3) // 4) if nws else None
     rc = lib.ppo_preference_loss(c.data_ptr(), c_s, _ptr(rc_), rc_s, _ptr(mc), mc_s, cs[1], r.data_ptr(), r_s, _ptr(rr), rr_s,
                                  _ptr(mr), mr_s, rs[1], pairs, PREFERENCE_KINDS[kind], beta, label_smoothing, bool(average),
                                  out2.data_ptr(), rewards.data_ptr(), _ptr(g_c), _ptr(g_r), _ptr(ws), nws, _stream())
@@ -1018,9 +1015,8 @@ def linear_act_fwd(x, weight, bias=None, activation="none", residual=None, want_
     _linear_operand(name, "bias", bias, (n,), dtype)
     _linear_operand(name, "residual", residual, shape, dtype)
     _device_tensors(name, x, weight, bias, residual)
-    dev = x.device
-    y = torch.empty(shape, dtype=dtype, device=dev)
-    deriv = torch.empty(shape, dtype=_deriv_dtype(dtype), device=dev) if want_deriv and activation != "none" else None
+    y = x.new_empty(*shape)
+    deriv = torch.empty_like(y, dtype=_deriv_dtype(dtype)) if want_deriv and activation != "none" else None
     if rows == 0:
         return y, deriv
     xm, xs = _matrix(x)
@@ -1030,7 +1026,7 @@ def linear_act_fwd(x, weight, bias=None, activation="none", residual=None, want_
         bias = bias.contiguous()
     dt = _DTYPES[dtype]
     nws = lib.ppo_linear_act_fwd_workspace_bytes(rows, k, n, dt)
-    ws = torch.empty(nws, dtype=torch.uint8, device=dev) if nws else None
+    ws = x.new_empty((nws + 3) // x.element_size()) if nws else None
     rc = lib.ppo_linear_act_fwd(xm.data_ptr(), xs, wm.data_ptr(), ws_, _ptr(bias), _ptr(rm), rs, dt, rows, k, n, ACTIVATIONS[activation],
                                 y.data_ptr(), _ptr(deriv), _ptr(ws), nws, _stream())
     if rc:
@@ -1048,13 +1044,13 @@ def linear_act_bwd(g, x, weight, deriv=None, want_input=True, want_weight=True, 
     if not isinstance(x, torch.Tensor):
         _refuse(f"{name}: x [..., inputs] and weight [outputs, inputs] of one type")
     rows, k, n = _linear_inputs(name, x, weight)
-    dtype, shape, dev = x.dtype, (*x.shape[:-1], n), x.device
+    dtype, shape = x.dtype, (*x.shape[:-1], n)
     _linear_operand(name, "g", g, shape, dtype)
     _linear_operand(name, "deriv", deriv, shape, _deriv_dtype(dtype))
     _device_tensors(name, x, weight, g, deriv)
-    g_x = torch.empty(x.shape, dtype=dtype, device=dev) if want_input else None
-    g_w = torch.empty((n, k), dtype=dtype, device=dev) if want_weight else None
-    g_b = torch.empty((n,), dtype=dtype, device=dev) if want_bias else None
+    g_x = torch.empty_like(x, memory_format=torch.contiguous_format) if want_input else None
+    g_w = x.new_empty(n, k) if want_weight else None
+    g_b = x.new_empty(n) if want_bias else None
     if rows == 0:
         return g_x, None if g_w is None else g_w.zero_(), None if g_b is None else g_b.zero_()
     gm, gs = _matrix(g)
@@ -1064,7 +1060,7 @@ def linear_act_bwd(g, x, weight, deriv=None, want_input=True, want_weight=True, 
         deriv = deriv.contiguous()
     dt = _DTYPES[dtype]
     nws = lib.ppo_linear_act_bwd_workspace_bytes(rows, k, n, dt)
-    ws = torch.empty(nws, dtype=torch.uint8, device=dev)
+    ws = x.new_empty((nws + 3) // x.element_size())
     rc = lib.ppo_linear_act_bwd(gm.data_ptr(), gs, xm.data_ptr(), xs, wm.data_ptr(), ws_, _ptr(deriv), dt, rows, k, n, _ptr(g_x), _ptr(g_w),
                                 _ptr(g_b), ws.data_ptr(), nws, _stream())
     if rc:
