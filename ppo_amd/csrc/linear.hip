@@ -754,21 +754,36 @@ struct Plan {
     int tiles_m, tiles_n, steps, per_split, splits;
 };
 
+// Tiles of 256 x 256 or 128 x 128, and how many workgroups share a tile's k: the cheapest by a model of the 256 CUs fitted
+// to measurements (us; 16-bit / f32).  A round of large tiles, one a CU: 19 + 1.4 / 4.6 a stage.  Of small ones: 10 + 0.57 / 1.43
+// a stage alone on a CU, 10 + 0.9 / 2.6 for two together.  Joining splits: 3 + 8 bytes a partial result at 4.5 TB/s.
+// Measured, large against small tiles, best splits of each: bf16 4096 x 4096 x 4096 108 against 135 us, 4096 x 4096 x 1024 44 / 49,
+// 6000 x 3000 x 512 58 / 43, 2048 x 2048 x 2048 41 / 28, 1024 x 1024 x 8192 44 (8 splits) / 34 (4; unsplit 74), 64 x 16384 x 4096
+// 38 (4) / 29 (2; unsplit 40); f32 16384 x 3136 x 512 368 / 302, 16384 x 512 x 3136 289 (2) / 264, 512 x 3136 x 16384 311 (8) / 281 (5;
+// unsplit 741).
 Plan plan_of(long M, long N, long K, long e)
 {
-    Plan p;
+    Plan p{};
     p.steps = (int)(k_padded(K, e) * e / 128);
-    const long big = ((M + 255) / 256) * ((N + 255) / 256);
-    p.large = big >= 192;
-    const long b = p.large ? 256 : 128;
-    p.tiles_m = (int)((M + b - 1) / b);
-    p.tiles_n = (int)((N + b - 1) / b);
-    const long tiles = (long)p.tiles_m * p.tiles_n;
-    long splits = p.large ? 1 : 512 / tiles;
-    if (splits > p.steps / 8) splits = p.steps / 8;
-    if (splits < 1) splits = 1;
-    p.per_split = (int)((p.steps + splits - 1) / splits);
-    p.splits = (p.steps + p.per_split - 1) / p.per_split;
+    const double t_large = e == 2 ? 1.4 : 4.6, t_two = e == 2 ? 0.9 : 2.6, t_one = e == 2 ? 0.57 : 1.43;
+    double best = 0.0;
+    for (int large = 0; large < 2; ++large) {
+        const long b = large ? 256 : 128, tm = (M + b - 1) / b, tn = (N + b - 1) / b;
+        for (int splits : {1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 24, 32}) {
+            if (splits > 1 && (p.steps < 4 * splits || (double)splits * M * N > 2.5e8)) break;
+            const int per = (p.steps + splits - 1) / splits;
+            const long rounds = (tm * tn * splits + 255) / 256;
+            double us = large ? rounds * (19.0 + t_large * per) : rounds / 2 * (10.0 + t_two * per) + rounds % 2 * (10.0 + t_one * per);
+            if (splits > 1) us += 3.0 + (double)splits * M * N * 8.0 / 4.5e6;
+            if (best != 0.0 && us >= best) continue;
+            best = us;
+            p.large = large;
+            p.tiles_m = (int)tm;
+            p.tiles_n = (int)tn;
+            p.per_split = per;
+            p.splits = (p.steps + per - 1) / per;
+        }
+    }
     return p;
 }
 
