@@ -539,8 +539,8 @@ int ppo_clip_adam_step(int n_tensors, float *const *params, float *const *exp_av
  * Categorical(logits).log_prob / .entropy (src/ppo.py:186-189, :212-214) for any number of actions.
  *   logits   [batch, length, num_actions] of `dtype`, actions contiguous, strides in elements (>= 0) of the other two axes;
  *            -inf marks an illegal action
- *   actions  [batch * length] i32 or i64 (action_bytes 4 / 8).  ignore_index: the row is not read, its outputs and its
- *            gradient are 0.  Any other value outside [0, num_actions): the row's outputs and gradient are NaN.
+ *   actions  [batch * length] i32 or i64 (action_bytes 4 / 8).  ignore_index: what the row holds is not used, its
+ *            outputs and its gradient are 0.  Any other value outside [0, num_actions): the row's outputs and gradient are NaN.
  *   logp     [batch * length] f32; entropy the same or NULL; stats [batch * length, 2] f32 {max logit, ln sum} for the
  *            backward call.  A row without a legal action: logp -inf, entropy 0.  NaN or +inf in a row: NaN.
  *   temperature in [1e-6, 1e6].
@@ -607,7 +607,7 @@ int ppo_preference_loss(const float *chosen, long chosen_stride, const float *re
  *   y [rows, outputs] contiguous; deriv the same or NULL: act'(z) for the backward call, f16 for PPO_DTYPE_BF16, f32 for
  *   the other types.
  * Sums are f32: 16-bit inputs on the 16-bit matrix cores; f32 inputs as three bf16 pieces each (PPO_NET_BF16X3), f32-grade,
- * except that magnitudes above 3.38e38 and infinities give NaN where more than 8 rows make the matrix cores worth while.
+ * except that magnitudes above 3.38e38 and infinities may give NaN where the rows are enough for the matrix cores.
  * ppo_linear_act_bwd: with u = g_y * deriv (deriv NULL: u = g_y), rounded to `dtype`:
  *   g_x [rows, inputs] = u W, g_weight [outputs, inputs] = u^T x, g_bias [outputs] = column sums of the unrounded u; each
  *   contiguous, of `dtype`, or NULL.  The residual's gradient is g_y.

@@ -744,7 +744,15 @@ template <class T, int ROWS, int COLS> __global__ void __launch_bounds__(256) k_
 }
 
 // ---- host: how a product is cut -------------------------------------------------------------------------------------
-constexpr long FEW_ROWS = 8;           // at most so many rows go to k_few_rows
+// Which calls go to k_few_rows.  Measured, that against the matrix cores, us: weights of a few MB, which stay in L2 when
+// they are read once for every 8 rows, 1000 x 1024 and 32 rows 9.7 / 14 in bf16, 10.7 / 15 in f32 (64 rows 12.5 / 13.5); 134 MB of
+// bf16 and 8 rows 46 / 32 (4 rows 30), the same not in place, where the matrix cores need a padded copy of the weights
+// first, 12 rows 98 / 87 (8 rows 54); 268 MB of f32 and 16 rows 109 / 104 (12 rows 106 / 109), not in place and 32 rows 178 / 196.
+bool few_rows(long rows, long N, long K, long e, bool in_place)
+{
+    if (N * K * e <= 4L << 20) return rows <= 32;
+    return rows <= (e == 2 ? (in_place ? 4 : 10) : (in_place ? 12 : 32));
+}
 constexpr long MOST_K = (1L << 22) - 128;   // 256 padded rows of so many floats still have 32-bit offsets
 
 long k_padded(long k, long e) { return (k * e + 127) / 128 * 128 / e; }
@@ -843,8 +851,8 @@ extern "C" {
 
 size_t ppo_linear_act_fwd_workspace_bytes(long rows, long inputs, long outputs, int dtype)
 {
-    if (!sizes_ok(rows, inputs, outputs, dtype) || rows <= FEW_ROWS) return 0;
     const long e = dtype_bytes(dtype), Kp = k_padded(inputs, e);
+    if (!sizes_ok(rows, inputs, outputs, dtype) || few_rows(rows, outputs, inputs, e, true)) return 0;
     return round256((size_t)rows * Kp * e) + round256((size_t)outputs * Kp * e) + partial_bytes(plan_of(rows, outputs, inputs, e), rows, outputs);
 }
 
@@ -858,17 +866,18 @@ int ppo_linear_act_fwd(const void *x, long x_stride, const void *weight, long we
     PPO_REQUIRE(matrix_ok(x, x_stride, inputs, e) && matrix_ok(weight, weight_stride, inputs, e));
     PPO_REQUIRE(!residual || matrix_ok(residual, residual_stride, outputs, e));
     PPO_REQUIRE(y && ppo_aligned(y, e) && ppo_aligned(deriv, dtype == PPO_DTYPE_BF16 ? 2 : 4) && ppo_aligned(bias, e) && activation >= PPO_ACT_NONE && activation <= PPO_ACT_SILU);
-    PPO_REQUIRE(workspace_bytes >= ppo_linear_act_fwd_workspace_bytes(rows, inputs, outputs, dtype));
-    PPO_REQUIRE(rows <= FEW_ROWS || (workspace && ppo_aligned(workspace, 16)));
+    const bool w_in_place = in_place(weight, weight_stride, inputs, e), few = few_rows(rows, outputs, inputs, e, w_in_place);
+    const size_t need = ppo_linear_act_fwd_workspace_bytes(rows, inputs, outputs, dtype);
+    PPO_REQUIRE(need == 0 || (workspace && ppo_aligned(workspace, 16) && workspace_bytes >= need));
     hipStream_t s = (hipStream_t)stream;
     return by_dtype(dtype, [&](auto t) {
         using T = decltype(t);
         GemmArgs g{};
         g.A = x; g.B = weight; g.M = rows; g.N = outputs; g.lda = x_stride * e; g.ldb = weight_stride * e;
         g.bias = bias; g.residual = residual; g.res_ld = residual_stride; g.out = y; g.deriv = deriv; g.act = activation;
-        if (rows <= FEW_ROWS) {
+        if (few) {
             constexpr int COLS = 4;
-            const dim3 grid((unsigned)((outputs + 4 * COLS - 1) / (4 * COLS)));
+            const dim3 grid((unsigned)((outputs + 4 * COLS - 1) / (4 * COLS)), (unsigned)((rows + 7) / 8));
             if (rows == 1)
                 hipLaunchKernelGGL((k_few_rows<T, 1, COLS>), grid, dim3(256), 0, s, g, inputs);
             else if (rows <= 4)
@@ -886,7 +895,7 @@ int ppo_linear_act_fwd(const void *x, long x_stride, const void *weight, long we
             g.lda = Kp * e;
         }
         ws += round256((size_t)rows * Kp * e);
-        if (!in_place(weight, weight_stride, inputs, e)) {
+        if (!w_in_place) {
             const int rc = prep<T>(weight, weight_stride, nullptr, outputs, inputs, ws, nullptr, nullptr, s);
             if (rc) return rc;
             g.B = ws;

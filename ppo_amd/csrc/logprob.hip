@@ -58,7 +58,7 @@ template <int N> __device__ __forceinline__ void row_add(Row &r, const float (&x
         const float t = (x[i] - base) * c;
         const float e = __builtin_amdgcn_exp2f(t);     // NaN stays in s
         s += e;
-        u += e * fmaxf(t, LOWEST);
+        u = __builtin_fmaf(e, fmaxf(t, LOWEST), u);
     }
     r.s += s;
     r.u += u;
@@ -121,26 +121,38 @@ template <class T> __device__ __forceinline__ void write_row(const FwdArgs &a, l
     a.stats[2 * row + 1] = lns;
 }
 
-// G lanes a row, one element a lane and turn: rows of a few dozen actions
+// G lanes a row, at most four elements a lane, all in registers: the lanes find the row's maximum first and then only
+// add, where joining running sums would take two exponentials a step
 template <class T, int G> __global__ void __launch_bounds__(256) k_logprobs_short(FwdArgs a)
 {
     const long row = (long)blockIdx.x * (256 / G) + threadIdx.x / G;
-    const int l = threadIdx.x % G;
+    const int l = threadIdx.x % G, A = (int)a.A;
     if (row >= a.rows) return;
+    const typename T::raw *x = reinterpret_cast<const typename T::raw *>(a.logits) + row_offset(row, a.rows, a.length, a.batch_stride, a.token_stride);
+    float v[4];                                        // (on their way while the action, which may be the ignored one, is)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = l + i * G < A ? T::load(x[l + i * G]) : -INFINITY;
     const long act = action_of(a.actions, a.action_bytes, row);
     if (act == a.ignore) {
         if (l == 0) write_ignored(a, row);
         return;
     }
-    const typename T::raw *x = reinterpret_cast<const typename T::raw *>(a.logits) + row_offset(row, a.rows, a.length, a.batch_stride, a.token_stride);
-    Row r = row_none();
-    for (long k = l; k < a.A; k += 4 * G) {
-        float v[4];
+    float m = fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3]));
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = k + i * G < a.A ? T::load(x[k + i * G]) : -INFINITY;
-        row_add<4>(r, v, a.c);
+    for (int off = G / 2; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor(m, off, 64));
+    const float base = m == -INFINITY ? 0.0f : m;
+    Row r = {m, 0.0f, 0.0f};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float t = (v[i] - base) * a.c, e = __builtin_amdgcn_exp2f(t);
+        r.s += e;
+        r.u = __builtin_fmaf(e, fmaxf(t, LOWEST), r.u);
     }
-    r = row_lanes<G>(r, a.c);
+#pragma unroll
+    for (int off = G / 2; off > 0; off >>= 1) {
+        r.s += __shfl_xor(r.s, off, 64);
+        r.u += __shfl_xor(r.u, off, 64);
+    }
     if (l == 0) write_row<T>(a, row, x, act, r);
 }
 
@@ -214,16 +226,11 @@ __device__ __forceinline__ Grad grad_of(const BwdArgs &a, long row)
 {
     Grad g;
     g.act = action_of(a.actions, a.action_bytes, row);
-    g.live = g.act != a.ignore;
-    g.base = g.lns2 = g.ga = g.gb = g.gl = 0.0f;
-    if (!g.live) return g;
     const float m = a.stats[2 * row], lns = a.stats[2 * row + 1];
-    if (m == -INFINITY && lns == 0.0f) {               // no legal action: no gradient
-        g.live = false;
-        return g;
-    }
     const float glp = a.g_logp ? a.g_logp[row] : 0.0f, gh = a.g_entropy ? a.g_entropy[row] : 0.0f;
     const float H = a.g_entropy ? a.entropy[row] : 0.0f;
+    // an ignored token and a row without a legal action have no gradient
+    g.live = g.act != a.ignore && !(m == -INFINITY && lns == 0.0f);
     g.base = m;
     g.lns2 = lns * LOG2E;
     g.gl = glp * a.inv_t;
@@ -234,23 +241,28 @@ __device__ __forceinline__ Grad grad_of(const BwdArgs &a, long row)
 
 __device__ __forceinline__ float grad_at(const Grad &g, float x, float c)
 {
-    const float t = (x - g.base) * c - g.lns2;         // log2 p
+    const float t = __builtin_fmaf(x - g.base, c, -g.lns2);   // log2 p
     const float p = __builtin_amdgcn_exp2f(t);
-    return -p * (g.ga + g.gb * fmaxf(t, LOWEST));
+    return -p * __builtin_fmaf(g.gb, fmaxf(t, LOWEST), g.ga);
 }
 
 template <class T, int G> __global__ void __launch_bounds__(256) k_logprobs_bwd_short(BwdArgs a)
 {
     const long row = (long)blockIdx.x * (256 / G) + threadIdx.x / G;
-    const int l = threadIdx.x % G;
+    const int l = threadIdx.x % G, A = (int)a.A;
     if (row >= a.rows) return;
-    const Grad g = grad_of(a, row);
     const typename T::raw *x = reinterpret_cast<const typename T::raw *>(a.logits) + row_offset(row, a.rows, a.length, a.batch_stride, a.token_stride);
     typename T::raw *o = reinterpret_cast<typename T::raw *>(a.g) + row * a.A;
-    for (long k = l; k < a.A; k += G) {
-        float v = 0.0f;
-        if (g.live) v = grad_at(g, T::load(x[k]), a.c) + (k == g.act ? g.gl : 0.0f);
-        o[k] = T::store(v);
+    const Grad g = grad_of(a, row);
+    for (int k = l; k < A; k += 4 * G) {
+        float v[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = k + i * G < A ? T::load(x[k + i * G]) : 0.0f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int at = k + i * G;
+            if (at < A) o[at] = T::store(g.live ? grad_at(g, v[i], a.c) + (at == g.act ? g.gl : 0.0f) : 0.0f);
+        }
     }
 }
 

@@ -18,7 +18,7 @@ using namespace ppo_token;
 
 namespace {
 
-constexpr int SEQ_BLOCK = 256, SEQ_MAX_BLOCKS = 2048, COUNT_MAX_BLOCKS = 512;
+constexpr int SEQ_BLOCK = 256, SEQ_MAX_BLOCKS = 2048, COUNT_MAX_BLOCKS = 1024;
 constexpr int NSUM = 4;                        // policy term, KL, clipped, drift r - 1 - ln r
 
 template <int NV, int THREADS> __device__ __forceinline__ void block_sum(double (&acc)[NV], double (*part)[NV])
@@ -81,6 +81,7 @@ __device__ __forceinline__ void count_rows(const PolicyArgs &a, int *row_counts,
         if (a.mask) {
             const uint8_t *m = a.mask + b * a.mask_stride;
             long t = lane * 16L;
+#pragma unroll 4
             for (; t + 16 <= a.L; t += 64 * 16) {
                 const Bytes16 v = *reinterpret_cast<const Bytes16 *>(m + t);
 #pragma unroll
@@ -223,14 +224,15 @@ __device__ __forceinline__ void policy_out(const PolicyArgs &a, const double (&s
     a.out6[5] = (float)tokens;
 }
 
-__device__ __forceinline__ void totals(const PolicyArgs &a, double (*part)[2], double &tokens, double &rows)
+template <int THREADS> __device__ __forceinline__ void totals(const PolicyArgs &a, double (*part)[2], double &tokens, double &rows)
 {
     double tot[2] = {0.0, 0.0};
-    for (int i = threadIdx.x; i < a.count_blocks; i += SEQ_BLOCK) {
+#pragma unroll 4
+    for (int i = threadIdx.x; i < a.count_blocks; i += THREADS) {
         tot[0] += a.counts[2 * i];
         tot[1] += a.counts[2 * i + 1];
     }
-    block_sum<2, SEQ_BLOCK>(tot, part);
+    block_sum<2, THREADS>(tot, part);
     tokens = tot[0];
     rows = tot[1];
 }
@@ -240,7 +242,7 @@ __global__ void __launch_bounds__(SEQ_BLOCK) k_policy_main(PolicyArgs a)
     __shared__ double part2[SEQ_BLOCK / 64][2];
     __shared__ double part[SEQ_BLOCK / 64][NSUM];
     double tokens, rows, acc[NSUM] = {0.0, 0.0, 0.0, 0.0};
-    totals(a, part2, tokens, rows);
+    totals<SEQ_BLOCK>(a, part2, tokens, rows);
     policy_groups(a, a.row_counts, tokens, rows, (long)blockIdx.x * SEQ_BLOCK + threadIdx.x, (long)gridDim.x * SEQ_BLOCK, acc);
     block_sum<NSUM, SEQ_BLOCK>(acc, part);
     if (threadIdx.x == 0) {
@@ -249,17 +251,19 @@ __global__ void __launch_bounds__(SEQ_BLOCK) k_policy_main(PolicyArgs a)
     }
 }
 
-__global__ void __launch_bounds__(SEQ_BLOCK) k_policy_final(PolicyArgs a, int blocks)
+constexpr int FINAL_BLOCK = 256;
+__global__ void __launch_bounds__(FINAL_BLOCK) k_policy_final(PolicyArgs a, int blocks)
 {
-    __shared__ double part2[SEQ_BLOCK / 64][2];
-    __shared__ double part[SEQ_BLOCK / 64][NSUM];
+    __shared__ double part2[FINAL_BLOCK / 64][2];
+    __shared__ double part[FINAL_BLOCK / 64][NSUM];
     double tokens, rows, acc[NSUM] = {0.0, 0.0, 0.0, 0.0};
-    totals(a, part2, tokens, rows);
-    for (int i = threadIdx.x; i < blocks; i += SEQ_BLOCK) {
+#pragma unroll 2
+    for (int i = threadIdx.x; i < blocks; i += FINAL_BLOCK) {
 #pragma unroll
         for (int k = 0; k < NSUM; ++k) acc[k] += a.partials[(long)i * NSUM + k];
     }
-    block_sum<NSUM, SEQ_BLOCK>(acc, part);
+    totals<FINAL_BLOCK>(a, part2, tokens, rows);
+    block_sum<NSUM, FINAL_BLOCK>(acc, part);
     if (threadIdx.x == 0) policy_out(a, acc, tokens, rows);
 }
 
@@ -673,7 +677,7 @@ int ppo_policy_kl_loss(const float *log_probs, long lp_stride, const float *old_
     hipLaunchKernelGGL(k_policy_main, dim3(blocks), dim3(SEQ_BLOCK), 0, s, a);
     rc = ppo_launch_status();
     if (rc) return rc;
-    hipLaunchKernelGGL(k_policy_final, dim3(1), dim3(SEQ_BLOCK), 0, s, a, blocks);
+    hipLaunchKernelGGL(k_policy_final, dim3(1), dim3(FINAL_BLOCK), 0, s, a, blocks);
     return ppo_launch_status();
 }
 

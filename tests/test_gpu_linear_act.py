@@ -92,6 +92,15 @@ def test_large_tiles(M, K, N, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows", [4, 5, 10, 11, 12, 13, 32, 33])
+def test_few_rows_of_large_weights(rows, dtype):
+    """Both sides of each border between the vector units and the matrix cores, weights in place and not (4.2 and 8.4 MB)."""
+    for K in (1024, 1025):
+        x, w, b, r, g = _make(rows, rows, K, 2100, dtype)
+        _check(x, w, b, r, g, "gelu")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_long_sums(dtype):
     """Long inner dimensions: splits and their joining."""
     for M, K, N in ((130, 20000, 70), (20011, 40, 33), (12, 9000, 16)):

@@ -104,9 +104,9 @@ def test_linear_c_entries_refuse():
     lib = _lib.load()
     buf = (ctypes.c_char * 4096)()
     p = (ctypes.addressof(buf) + 63) // 64 * 64
-    n = lib.ppo_linear_act_fwd_workspace_bytes(16, 8, 8, 0)
+    n = lib.ppo_linear_act_fwd_workspace_bytes(64, 8, 8, 0)
     assert lib.ppo_linear_act_fwd_workspace_bytes(8, 8, 8, 0) == 0 and n > 0
-    fwd = lambda x=p, xs=8, w=p, ws_=8, b=p, r=p, rs=8, dt=0, M=16, K=8, N=8, act=1, y=p, d=p, ws=p, nws=n: lib.ppo_linear_act_fwd(  # noqa: E731
+    fwd = lambda x=p, xs=8, w=p, ws_=8, b=p, r=p, rs=8, dt=0, M=64, K=8, N=8, act=1, y=p, d=p, ws=p, nws=n: lib.ppo_linear_act_fwd(  # noqa: E731
         x, xs, w, ws_, b, r, rs, dt, M, K, N, act, y, d, ws, nws, None)
     assert fwd(M=0) == 0
     for kw in ({"x": None}, {"x": p + 2}, {"xs": 7}, {"w": None}, {"ws_": 7}, {"w": p + 1}, {"b": p + 2}, {"r": p + 2}, {"rs": 7}, {"dt": 3}, {"dt": -1}, {"M": -1},
