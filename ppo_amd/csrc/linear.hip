@@ -159,16 +159,26 @@ struct PrepArgs {
     void *rows, *cols;
     float *sums;
     long R, C, ld, Rp, Cp;
-    int pad_rows;
+    int pad_rows, tiles_x;                 // tiles of 64 x 64 a row of tiles
 };
 
-template <class T> __global__ void __launch_bounds__(256) k_prep(PrepArgs a)
+// up to three of them in one launch: tiles first[j] .. first[j + 1] - 1 are those of job[j]
+struct PrepJobs {
+    PrepArgs job[3];
+    unsigned first[4];
+};
+
+template <class T> __global__ void __launch_bounds__(256) k_prep(PrepJobs jobs)
 {
+    const int which = blockIdx.x < jobs.first[1] ? 0 : blockIdx.x < jobs.first[2] ? 1 : 2;
+    const PrepArgs a = which == 0 ? jobs.job[0] : which == 1 ? jobs.job[1] : jobs.job[2];
+    const unsigned id = blockIdx.x - (which == 0 ? 0u : which == 1 ? jobs.first[1] : jobs.first[2]);
+    const long tile_y = id / (unsigned)a.tiles_x, tile_x = id % (unsigned)a.tiles_x;
     constexpr int E = 16 / T::BYTES, TPR = 64 / E, RPP = 256 / TPR;   // threads a row of 64, rows a pass
     using raw = typename T::raw;
     __shared__ raw tile[64][64 + 4 / T::BYTES];
     __shared__ float colsum[RPP][64];
-    const long r0 = (long)blockIdx.y * 64, c0 = (long)blockIdx.x * 64;
+    const long r0 = tile_y * 64, c0 = tile_x * 64;
     const int tc = threadIdx.x % TPR * E, tr = threadIdx.x / TPR;
     const raw *src = reinterpret_cast<const raw *>(a.src);
     const typename D<T>::raw *mul = reinterpret_cast<const typename D<T>::raw *>(a.mul);
@@ -227,7 +237,7 @@ template <class T> __global__ void __launch_bounds__(256) k_prep(PrepArgs a)
     if (a.sums && threadIdx.x < 64 && c0 + threadIdx.x < a.C) {
         float s = 0.0f;
         for (int k = 0; k < RPP; ++k) s += colsum[k][threadIdx.x];
-        a.sums[(long)blockIdx.y * a.C + c0 + threadIdx.x] = s;
+        a.sums[tile_y * a.C + c0 + threadIdx.x] = s;
     }
 }
 
@@ -800,17 +810,33 @@ size_t partial_bytes(const Plan &p, long M, long N) { return p.splits > 1 ? roun
 
 bool in_place(const void *p, long ld, long K, long e) { return ppo_aligned(p, 16) && ld * e % 16 == 0 && K * e % 128 == 0 && ld <= MOST_K; }
 
-template <class T>
-int prep(const void *src, long ld, const void *mul, long R, long C, void *rows, void *cols, float *sums, hipStream_t s, bool pad_rows = false)
-{
-    constexpr long e = T::BYTES;
-    PrepArgs a{src, mul, rows, cols, sums, R, C, ld, k_padded(R, e), k_padded(C, e), pad_rows};
-    // whole k steps in both directions: what lies past the matrix becomes zero
-    const long gr = cols || pad_rows ? (a.Rp + 63) / 64 : (R + 63) / 64, gc = rows ? (a.Cp + 63) / 64 : (C + 63) / 64;
-    PPO_REQUIRE(gr < 65536 && gc < (1L << 31));
-    hipLaunchKernelGGL(k_prep<T>, dim3((unsigned)gc, (unsigned)gr), dim3(256), 0, s, a);
-    return ppo_launch_status();
-}
+// collects what a call has to prepare, for one launch
+template <class T> struct Prep {
+    PrepJobs jobs{};
+    int count = 0;
+    long tiles = 0;
+
+    void add(const void *src, long ld, const void *mul, long R, long C, void *rows, void *cols, float *sums, bool pad_rows = false)
+    {
+        constexpr long e = T::BYTES;
+        PrepArgs a{src, mul, rows, cols, sums, R, C, ld, k_padded(R, e), k_padded(C, e), pad_rows, 0};
+        // whole k steps in both directions: what lies past the matrix becomes zero
+        const long gr = cols || pad_rows ? (a.Rp + 63) / 64 : (R + 63) / 64, gc = rows ? (a.Cp + 63) / 64 : (C + 63) / 64;
+        a.tiles_x = (int)gc;
+        jobs.job[count] = a;
+        tiles += gr * gc;
+        jobs.first[++count] = (unsigned)tiles;
+    }
+
+    int launch(hipStream_t s)
+    {
+        if (count == 0) return 0;
+        PPO_REQUIRE(tiles < (1L << 31));
+        for (int j = count; j < 3; ++j) jobs.first[j + 1] = (unsigned)tiles;
+        hipLaunchKernelGGL(k_prep<T>, dim3((unsigned)tiles), dim3(256), 0, s, jobs);
+        return ppo_launch_status();
+    }
+};
 
 template <class T, bool KA, bool KB> int gemm(GemmArgs g, const Plan &p, hipStream_t s)
 {
@@ -888,20 +914,21 @@ int ppo_linear_act_fwd(const void *x, long x_stride, const void *weight, long we
         }
         char *ws = reinterpret_cast<char *>(workspace);
         const long Kp = k_padded(inputs, e);
+        Prep<T> prep;
         if (!in_place(x, x_stride, inputs, e)) {
-            const int rc = prep<T>(x, x_stride, nullptr, rows, inputs, ws, nullptr, nullptr, s);
-            if (rc) return rc;
+            prep.add(x, x_stride, nullptr, rows, inputs, ws, nullptr, nullptr);
             g.A = ws;
             g.lda = Kp * e;
         }
         ws += round256((size_t)rows * Kp * e);
         if (!w_in_place) {
-            const int rc = prep<T>(weight, weight_stride, nullptr, outputs, inputs, ws, nullptr, nullptr, s);
-            if (rc) return rc;
+            prep.add(weight, weight_stride, nullptr, outputs, inputs, ws, nullptr, nullptr);
             g.B = ws;
             g.ldb = Kp * e;
         }
         ws += round256((size_t)outputs * Kp * e);
+        const int rc = prep.launch(s);
+        if (rc) return rc;
         g.partial = reinterpret_cast<float *>(ws);
         return gemm<T, false, false>(g, plan_of(rows, outputs, inputs, e), s);
     });
@@ -942,58 +969,45 @@ int ppo_linear_act_bwd(const void *g_y, long g_stride, const void *x, long x_str
         gw.M = outputs; gw.N = inputs; gw.out = g_weight; gw.act = PPO_ACT_NONE; gw.partial = partial;
         const Plan plan_x = plan_of(rows, inputs, outputs, e), plan_w = plan_of(outputs, inputs, rows, e);
         const bool row_in_place = !deriv && in_place(g_y, g_stride, outputs, e);   // g_x's A
-        int rc = 0;
+        Prep<T> prep;
+        long tiles = 0;                    // of 64 rows of u, for its column sums
         if constexpr (T::BYTES == 4) {
             // u and W and x are read along k as they lie
             const bool col_in_place = !deriv && in_place_along_k(g_y, g_stride, rows, e);
             const bool write_u = (g_x && !row_in_place) || (g_weight && !col_in_place);
-            if (write_u || g_bias)
-                rc = prep<T>(g_y, g_stride, deriv, rows, outputs, write_u ? u : nullptr, nullptr, g_bias ? sums : nullptr, s, write_u);
-            if (!rc && g_bias) {
-                const long tiles = ((write_u ? Mp : rows) + 63) / 64;
-                hipLaunchKernelGGL(k_bias_grad<T>, dim3((unsigned)((outputs + 63) / 64)), dim3(1024), 0, s, sums, tiles, outputs,
-                                   reinterpret_cast<typename T::raw *>(g_bias));
-                rc = ppo_launch_status();
+            if (write_u || g_bias) prep.add(g_y, g_stride, deriv, rows, outputs, write_u ? u : nullptr, nullptr, g_bias ? sums : nullptr, write_u);
+            tiles = ((write_u ? Mp : rows) + 63) / 64;
+            gx.A = row_in_place ? g_y : u; gx.lda = (row_in_place ? g_stride : Np) * e;
+            gx.B = weight; gx.ldb = weight_stride * e;
+            if (g_x && !in_place_along_k(weight, weight_stride, outputs, e)) {
+                prep.add(weight, weight_stride, nullptr, outputs, inputs, wt, nullptr, nullptr, true);
+                gx.B = wt; gx.ldb = Kp * e;
             }
-            if (!rc && g_x) {
-                gx.A = row_in_place ? g_y : u; gx.lda = (row_in_place ? g_stride : Np) * e;
-                gx.B = weight; gx.ldb = weight_stride * e;
-                if (!in_place_along_k(weight, weight_stride, outputs, e)) {
-                    rc = prep<T>(weight, weight_stride, nullptr, outputs, inputs, wt, nullptr, nullptr, s, true);
-                    gx.B = wt; gx.ldb = Kp * e;
-                }
-                if (!rc) rc = gemm<T, false, true>(gx, plan_x, s);
-            }
-            if (!rc && g_weight) {
-                gw.A = col_in_place ? g_y : u; gw.lda = (col_in_place ? g_stride : Np) * e;
-                gw.B = x; gw.ldb = x_stride * e;
-                if (!in_place_along_k(x, x_stride, rows, e)) {
-                    rc = prep<T>(x, x_stride, nullptr, rows, inputs, xt, nullptr, nullptr, s, true);
-                    gw.B = xt; gw.ldb = Kp * e;
-                }
-                if (!rc) rc = gemm<T, true, true>(gw, plan_w, s);
+            gw.A = col_in_place ? g_y : u; gw.lda = (col_in_place ? g_stride : Np) * e;
+            gw.B = x; gw.ldb = x_stride * e;
+            if (g_weight && !in_place_along_k(x, x_stride, rows, e)) {
+                prep.add(x, x_stride, nullptr, rows, inputs, xt, nullptr, nullptr, true);
+                gw.B = xt; gw.ldb = Kp * e;
             }
         } else {
             const bool want_rows = g_x && !row_in_place;
             if (want_rows || g_weight || g_bias)
-                rc = prep<T>(g_y, g_stride, deriv, rows, outputs, want_rows ? u : nullptr, g_weight ? ut : nullptr, g_bias ? sums : nullptr, s);
-            if (!rc && g_bias) {
-                const long tiles = ((g_weight ? Mp : rows) + 63) / 64;
-                hipLaunchKernelGGL(k_bias_grad<T>, dim3((unsigned)((outputs + 63) / 64)), dim3(1024), 0, s, sums, tiles, outputs,
-                                   reinterpret_cast<typename T::raw *>(g_bias));
-                rc = ppo_launch_status();
-            }
-            if (!rc && g_x) {
-                rc = prep<T>(weight, weight_stride, nullptr, outputs, inputs, nullptr, wt, nullptr, s);
-                gx.A = row_in_place ? g_y : u; gx.lda = (row_in_place ? g_stride : Np) * e; gx.B = wt; gx.ldb = Np * e;
-                if (!rc) rc = gemm<T, false, false>(gx, plan_x, s);
-            }
-            if (!rc && g_weight) {
-                rc = prep<T>(x, x_stride, nullptr, rows, inputs, nullptr, xt, nullptr, s);
-                gw.A = ut; gw.lda = Mp * e; gw.B = xt; gw.ldb = Mp * e;
-                if (!rc) rc = gemm<T, false, false>(gw, plan_w, s);
-            }
+                prep.add(g_y, g_stride, deriv, rows, outputs, want_rows ? u : nullptr, g_weight ? ut : nullptr, g_bias ? sums : nullptr);
+            tiles = ((g_weight ? Mp : rows) + 63) / 64;
+            if (g_x) prep.add(weight, weight_stride, nullptr, outputs, inputs, nullptr, wt, nullptr);
+            gx.A = row_in_place ? g_y : u; gx.lda = (row_in_place ? g_stride : Np) * e; gx.B = wt; gx.ldb = Np * e;
+            if (g_weight) prep.add(x, x_stride, nullptr, rows, inputs, nullptr, xt, nullptr);
+            gw.A = ut; gw.lda = Mp * e; gw.B = xt; gw.ldb = Mp * e;
         }
+        int rc = prep.launch(s);
+        if (!rc && g_bias) {
+            hipLaunchKernelGGL(k_bias_grad<T>, dim3((unsigned)((outputs + 63) / 64)), dim3(1024), 0, s, sums, tiles, outputs,
+                               reinterpret_cast<typename T::raw *>(g_bias));
+            rc = ppo_launch_status();
+        }
+        constexpr bool ALONG = T::BYTES == 4;
+        if (!rc && g_x) rc = gemm<T, false, ALONG>(gx, plan_x, s);
+        if (!rc && g_weight) rc = gemm<T, ALONG, ALONG>(gw, plan_w, s);
         return rc;
     });
 }
