@@ -152,14 +152,13 @@ template <class T, int N> __device__ __forceinline__ void store_n(typename T::ra
 
 // ---- operand preparation: pad, multiply by d, transpose, sum columns -----------------------------------------------
 // src [R, C] of T with row stride ld (times mul [R, C] of D<T>, contiguous) -> rows [R, Cp] and / or cols [C, Rp] of T, Cp and Rp
-// the next multiples of a k step, zero-filled; sums [tiles of 64 rows][C] f32 = column sums of a tile.  pad_rows: `rows`
-// gets Rp of them, for use along k.
+// the next multiples of a k step, zero-filled; sums [tiles of 64 rows][C] f32 = column sums of a tile.
 struct PrepArgs {
     const void *src, *mul;
     void *rows, *cols;
     float *sums;
     long R, C, ld, Rp, Cp;
-    int pad_rows, tiles_x;                 // tiles of 64 x 64 a row of tiles
+    int tiles_x;                           // tiles of 64 x 64 a row of tiles
 };
 
 // up to three of them in one launch: tiles first[j] .. first[j + 1] - 1 are those of job[j]
@@ -210,7 +209,7 @@ template <class T> __global__ void __launch_bounds__(256) k_prep(PrepJobs jobs)
         }
 #pragma unroll
         for (int j = 0; j < E; ++j) sum[j] += v[j];
-        if (a.rows && gr < (a.pad_rows ? a.Rp : a.R) && gc < a.Cp) store16<T>(reinterpret_cast<raw *>(a.rows) + gr * a.Cp + gc, v);
+        if (a.rows && gr < a.R && gc < a.Cp) store16<T>(reinterpret_cast<raw *>(a.rows) + gr * a.Cp + gc, v);
         if (a.cols) {
 #pragma unroll
             for (int j = 0; j < E; ++j) tile[r][tc + j] = T::store(v[j]);
@@ -266,6 +265,7 @@ template <class T> __global__ void __launch_bounds__(1024) k_bias_grad(const flo
 struct GemmArgs {
     const void *A, *B;                 // [M, k], [N, k]; rows lda, ldb bytes apart
     long M, N, lda, ldb;
+    long K;                            // the last stage's elements from here on count as 0
     int steps, steps_per_split;        // steps of 128 bytes of k
     int tiles_m, tiles_n;
     float *partial;                    // [splits][M][N], or NULL: the epilogue below
@@ -375,7 +375,9 @@ __global__ void __launch_bounds__(64 * WAVES_M * WAVES_N) k_gemm(GemmArgs g)
     const long m0 = (long)(first + id % band % high) * BM, n0 = (long)(id % band / high) * BN;
     const int s0 = blockIdx.y * g.steps_per_split, s1 = s0 + g.steps_per_split < g.steps ? s0 + g.steps_per_split : g.steps;
 
-    const long kbytes = (long)g.steps * 128;
+    const long kbytes = g.K * T::BYTES;
+    constexpr int KS = 128 / T::BYTES;                               // elements of k a stage
+    const int tail = s1 == g.steps ? (int)(g.K - (g.steps - 1L) * KS) : KS;   // of the last one
     const long rows_a = g.M - m0 < BM ? g.M - m0 : BM, rows_b = g.N - n0 < BN ? g.N - n0 : BN;
     const char *pa0 = reinterpret_cast<const char *>(g.A) + (KA ? m0 * 4 : m0 * g.lda), *pb0 = reinterpret_cast<const char *>(g.B) + (KB ? n0 * 4 : n0 * g.ldb);
     const u32x4 ra = buffer_of(pa0, KA ? 0 : (rows_a - 1) * g.lda + kbytes), rb = buffer_of(pb0, KB ? 0 : (rows_b - 1) * g.ldb + kbytes);
@@ -405,19 +407,20 @@ __global__ void __launch_bounds__(64 * WAVES_M * WAVES_N) k_gemm(GemmArgs g)
         }
     }
     const uint32_t base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds;
-    // load i of a stage's A or B to the place that begins at `to`.  Along k a stage is 32 rows of the matrix; what is read
-    // past its last column is the next row's beginning, or nothing behind the last row, and reaches no result that is kept.
+    // load i of a stage's A or B to the place that begins at `to`.  What is read past a row's end is the next row's beginning,
+    // or nothing behind the last row: past K it is masked out of the last stage's fragments, and where the operand's rows go
+    // along k it belongs to columns whose results are not kept.
     auto load_a = [&](int s, int to, int i) {
         const uint32_t at = base + wave * 1024 + to + i * WAVES * 1024;
         if constexpr (KA)
-            load_lds(buffer_of(pa0 + s * 32L * g.lda, (g.steps * 32L - s * 32L - 1) * g.lda + (g.M - m0) * 4), va[i], 0, at);
+            load_lds(buffer_of(pa0 + s * 32L * g.lda, (g.K - s * 32L - 1) * g.lda + (g.M - m0) * 4), va[i], 0, at);
         else
             load_lds(ra, va[i], s * 128, at);
     };
     auto load_b = [&](int s, int to, int i) {
         const uint32_t at = base + wave * 1024 + B_AT + to + i * WAVES * 1024;
         if constexpr (KB)
-            load_lds(buffer_of(pb0 + s * 32L * g.ldb, (g.steps * 32L - s * 32L - 1) * g.ldb + (g.N - n0) * 4), vb[i], 0, at);
+            load_lds(buffer_of(pb0 + s * 32L * g.ldb, (g.K - s * 32L - 1) * g.ldb + (g.N - n0) * 4), vb[i], 0, at);
         else
             load_lds(rb, vb[i], s * 128, at);
     };
@@ -481,7 +484,21 @@ __global__ void __launch_bounds__(64 * WAVES_M * WAVES_N) k_gemm(GemmArgs g)
         static_assert(2 * R <= MI * NI, "room for the reads");
         const int n = s1 - s0;
         int a_now = 0, a_next = A_STAGE, b_now = 0, b_next = B_STAGE;
+        // what lies past K in the last stage is not of this row: 0.  (K is even: a pair of halves is in or out)
+        auto cut = [&](Half &h, int half) {
+            if (tail < KS) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const bool out = half * 32 + kg * 8 + 2 * e >= tail;
+#pragma unroll
+                    for (int j = 0; j < NI; ++j) h.b[j][e] = out ? 0u : h.b[j][e];
+#pragma unroll
+                    for (int i = 0; i < MI; ++i) h.a[i][e] = out ? 0u : h.a[i][e];
+                }
+            }
+        };
         auto turn = [&](int s, auto left) {                 // left: stages behind this one, 3 for three or more
+            if constexpr (left() == 0) cut(h0, 0);
             work(h0, [&](int p, int) {
                 if (p % 2 == 0 && p / 2 < R) fetch(a_now, b_now, 1, h1, p / 2);
             });
@@ -491,6 +508,7 @@ __global__ void __launch_bounds__(64 * WAVES_M * WAVES_N) k_gemm(GemmArgs g)
                 asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
             __builtin_amdgcn_s_barrier();
             asm volatile("" ::: "memory");
+            if constexpr (left() == 0) cut(h1, 1);
             __builtin_amdgcn_sched_barrier(0);
             work(h1, [&](int p, int P) {
                 constexpr int NL = LB + LA;
@@ -539,12 +557,12 @@ __global__ void __launch_bounds__(64 * WAVES_M * WAVES_N) k_gemm(GemmArgs g)
     } else {
         stage_a(s0, 0);
         stage_b(s0, 0);
-        for (int s = s0; s < s1; ++s) {
+        auto step = [&](int s, auto last) {
             asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
             __builtin_amdgcn_s_barrier();                   // stage s has landed for every wave, and nobody reads the other one
             asm volatile("" ::: "memory");
             const int now = (s - s0) & 1;
-            if (s + 1 < s1) {
+            if constexpr (!last()) {
                 stage_a(s + 1, (now ^ 1) * A_STAGE);
                 stage_b(s + 1, (now ^ 1) * B_STAGE);
             }
@@ -587,11 +605,21 @@ __global__ void __launch_bounds__(64 * WAVES_M * WAVES_N) k_gemm(GemmArgs g)
                     hi = *reinterpret_cast<const f32x4 *>(at_b + pb + j * 512 + cb1);
                 }
             };
+            auto cut = [&](f32x4 &lo, f32x4 &hi) {          // k past K are not of this row
+                if constexpr (last()) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        lo[e] = kg * 8 + e < tail ? lo[e] : 0.0f;
+                        hi[e] = kg * 8 + e + 4 < tail ? hi[e] : 0.0f;
+                    }
+                }
+            };
             u32x4 fb[NI][3];
 #pragma unroll
             for (int j = 0; j < NI; ++j) {
                 f32x4 lo, hi;
                 read_b(j, lo, hi);
+                cut(lo, hi);
                 split(lo, hi, fb[j]);
             }
 #pragma unroll
@@ -599,6 +627,7 @@ __global__ void __launch_bounds__(64 * WAVES_M * WAVES_N) k_gemm(GemmArgs g)
                 f32x4 lo, hi;
                 u32x4 fa[3];
                 read_a(i, lo, hi);
+                cut(lo, hi);
                 split(lo, hi, fa);
 #pragma unroll
                 for (int t = 0; t < 6; ++t) {
@@ -607,7 +636,9 @@ __global__ void __launch_bounds__(64 * WAVES_M * WAVES_N) k_gemm(GemmArgs g)
                     for (int j = 0; j < NI; ++j) acc[i][j] = mfma<BF16>(fb[j][PB[t]], fa[PA[t]], acc[i][j]);
                 }
             }
-        }
+        };
+        for (int s = s0; s + 1 < s1; ++s) step(s, std::false_type{});
+        step(s1 - 1, std::true_type{});
     }
 
     // acc[i][j][e] is C[m0 + wm WM + 16 i + q][n0 + wn WN + 16 kg + 4 j + e].  The results go through LDS, PI rows of
@@ -808,7 +839,15 @@ Plan plan_of(long M, long N, long K, long e)
 size_t round256(size_t n) { return (n + 255) / 256 * 256; }
 size_t partial_bytes(const Plan &p, long M, long N) { return p.splits > 1 ? round256((size_t)p.splits * M * N * 4) : 0; }
 
-bool in_place(const void *p, long ld, long K, long e) { return ppo_aligned(p, 16) && ld * e % 16 == 0 && K * e % 128 == 0 && ld <= MOST_K; }
+// The loads take 16 bytes from any multiple of 4, so f32 operands are read as they lie, and 16-bit ones whose rows hold and
+// are an even number of elements apart; the others are copied to padded rows first.
+bool in_place(const void *p, long ld, long K, long e)
+{
+    return ppo_aligned(p, 4) && (e == 4 || (ld % 2 == 0 && K % 2 == 0));
+}
+
+// k as the kernel counts it: an odd number of halves is in padded copies only, whose rest is 0
+long whole_k(long K, long e) { return e == 2 && K % 2 ? k_padded(K, e) : K; }
 
 // collects what a call has to prepare, for one launch
 template <class T> struct Prep {
@@ -816,12 +855,12 @@ template <class T> struct Prep {
     int count = 0;
     long tiles = 0;
 
-    void add(const void *src, long ld, const void *mul, long R, long C, void *rows, void *cols, float *sums, bool pad_rows = false)
+    void add(const void *src, long ld, const void *mul, long R, long C, void *rows, void *cols, float *sums)
     {
         constexpr long e = T::BYTES;
-        PrepArgs a{src, mul, rows, cols, sums, R, C, ld, k_padded(R, e), k_padded(C, e), pad_rows, 0};
+        PrepArgs a{src, mul, rows, cols, sums, R, C, ld, k_padded(R, e), k_padded(C, e), 0};
         // whole k steps in both directions: what lies past the matrix becomes zero
-        const long gr = cols || pad_rows ? (a.Rp + 63) / 64 : (R + 63) / 64, gc = rows ? (a.Cp + 63) / 64 : (C + 63) / 64;
+        const long gr = cols ? (a.Rp + 63) / 64 : (R + 63) / 64, gc = rows ? (a.Cp + 63) / 64 : (C + 63) / 64;
         a.tiles_x = (int)gc;
         jobs.job[count] = a;
         tiles += gr * gc;
@@ -838,8 +877,9 @@ template <class T> struct Prep {
     }
 };
 
-template <class T, bool KA, bool KB> int gemm(GemmArgs g, const Plan &p, hipStream_t s)
+template <class T, bool KA, bool KB> int gemm(GemmArgs g, long K, const Plan &p, hipStream_t s)
 {
+    g.K = K;
     g.steps = p.steps;
     g.steps_per_split = p.per_split;
     g.tiles_m = p.tiles_m;
@@ -858,9 +898,6 @@ template <class T, bool KA, bool KB> int gemm(GemmArgs g, const Plan &p, hipStre
     return ppo_launch_status();
 }
 
-// an operand whose rows go along k: padded to whole k steps unless it is whole already
-bool in_place_along_k(const void *p, long ld, long R, long e) { return ppo_aligned(p, 16) && ld * e % 16 == 0 && R * e % 128 == 0 && ld <= MOST_K; }
-
 bool sizes_ok(long rows, long inputs, long outputs, int dtype)
 {
     // 32-bit workgroup counts and offsets inside a tile; rows are also the k of the weight gradient
@@ -869,7 +906,7 @@ bool sizes_ok(long rows, long inputs, long outputs, int dtype)
            (__int128)inputs * outputs < ((__int128)1 << 38);
 }
 
-bool matrix_ok(const void *p, long ld, long cols, long e) { return p && ppo_aligned(p, e) && ld >= cols && ld <= (1L << 32); }
+bool matrix_ok(const void *p, long ld, long cols, long e) { return p && ppo_aligned(p, e) && ld >= cols && ld <= MOST_K; }
 
 }  // namespace
 
@@ -930,7 +967,7 @@ int ppo_linear_act_fwd(const void *x, long x_stride, const void *weight, long we
         const int rc = prep.launch(s);
         if (rc) return rc;
         g.partial = reinterpret_cast<float *>(ws);
-        return gemm<T, false, false>(g, plan_of(rows, outputs, inputs, e), s);
+        return gemm<T, false, false>(g, whole_k(inputs, e), plan_of(rows, outputs, inputs, e), s);
     });
 }
 
@@ -973,22 +1010,13 @@ int ppo_linear_act_bwd(const void *g_y, long g_stride, const void *x, long x_str
         long tiles = 0;                    // of 64 rows of u, for its column sums
         if constexpr (T::BYTES == 4) {
             // u and W and x are read along k as they lie
-            const bool col_in_place = !deriv && in_place_along_k(g_y, g_stride, rows, e);
-            const bool write_u = (g_x && !row_in_place) || (g_weight && !col_in_place);
-            if (write_u || g_bias) prep.add(g_y, g_stride, deriv, rows, outputs, write_u ? u : nullptr, nullptr, g_bias ? sums : nullptr, write_u);
-            tiles = ((write_u ? Mp : rows) + 63) / 64;
-            gx.A = row_in_place ? g_y : u; gx.lda = (row_in_place ? g_stride : Np) * e;
+            const bool write_u = (g_x || g_weight) && !row_in_place;
+            if (write_u || g_bias) prep.add(g_y, g_stride, deriv, rows, outputs, write_u ? u : nullptr, nullptr, g_bias ? sums : nullptr);
+            tiles = (rows + 63) / 64;
+            gx.A = gw.A = row_in_place ? g_y : u;
+            gx.lda = gw.lda = (row_in_place ? g_stride : Np) * e;
             gx.B = weight; gx.ldb = weight_stride * e;
-            if (g_x && !in_place_along_k(weight, weight_stride, outputs, e)) {
-                prep.add(weight, weight_stride, nullptr, outputs, inputs, wt, nullptr, nullptr, true);
-                gx.B = wt; gx.ldb = Kp * e;
-            }
-            gw.A = col_in_place ? g_y : u; gw.lda = (col_in_place ? g_stride : Np) * e;
             gw.B = x; gw.ldb = x_stride * e;
-            if (g_weight && !in_place_along_k(x, x_stride, rows, e)) {
-                prep.add(x, x_stride, nullptr, rows, inputs, xt, nullptr, nullptr, true);
-                gw.B = xt; gw.ldb = Kp * e;
-            }
         } else {
             const bool want_rows = g_x && !row_in_place;
             if (want_rows || g_weight || g_bias)
@@ -1006,8 +1034,8 @@ int ppo_linear_act_bwd(const void *g_y, long g_stride, const void *x, long x_str
             rc = ppo_launch_status();
         }
         constexpr bool ALONG = T::BYTES == 4;
-        if (!rc && g_x) rc = gemm<T, false, ALONG>(gx, plan_x, s);
-        if (!rc && g_weight) rc = gemm<T, ALONG, ALONG>(gw, plan_w, s);
+        if (!rc && g_x) rc = gemm<T, false, ALONG>(gx, whole_k(outputs, e), plan_x, s);
+        if (!rc && g_weight) rc = gemm<T, ALONG, ALONG>(gw, whole_k(rows, e), plan_w, s);
         return rc;
     });
 }

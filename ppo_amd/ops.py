@@ -975,10 +975,10 @@ def _matrix(t):
     m = t if t.dim() == 2 else t.reshape(-1, t.shape[-1])
     rows, cols = m.shape
     s0, s1 = m.stride()
-    if (s1 != 1 and cols > 1) or (s0 < cols and rows > 1):
+    if (s1 != 1 and cols > 1) or ((s0 < cols or s0 > _LINEAR_MOST) and rows > 1):
         m = m.contiguous()
         s0 = m.stride(0)
-    return m, s0 if s0 > cols else cols
+    return m, s0 if rows > 1 else cols
 
 
 def _linear_inputs(name, x, weight):

@@ -143,6 +143,35 @@ def test_views_and_leading_axes(M, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("M,K,N", [(3, 70, 40), (150, 37, 130), (150, 70, 130), (260, 100, 301), (300, 1031, 70)])
+def test_what_lies_beside_the_operands_is_not_used(M, K, N, dtype):
+    """Operands cut out of buffers that hold NaN everywhere else, at even and odd strides and offsets."""
+    from ppo_amd import ops
+    x, w, b, r, g = _make(M, M, K, N, dtype)
+
+    def inside(t, left, right):
+        if t.dim() == 1:
+            return inside(t.unsqueeze(0), left, right)[0]
+        big = torch.full((t.shape[0] + 2, t.shape[1] + left + right), math.nan, dtype=t.dtype, device="cuda")
+        big[1:-1, left:left + t.shape[1]] = t
+        return big[1:-1, left:left + t.shape[1]]
+
+    for left, right in ((2, 4), (1, 2), (0, 3), (8, 8)):
+        X, W, B, R, G = (inside(t, left, right) for t in (x, w, b, r, g))
+        y, d = ops.linear_act_fwd(X, W, B, "tanh", R, want_deriv=True)
+        want, dw = ops.linear_act_fwd(x, w, b, "tanh", r, want_deriv=True)
+        assert torch.allclose(y, want, rtol=8 * torch.finfo(dtype).eps, atol=8 * torch.finfo(dtype).eps)
+        got = ops.linear_act_bwd(G, X, W, d)
+        for p, q in zip(got, ops.linear_act_bwd(g, x, w, dw)):
+            assert bool(torch.isfinite(p).all())
+            assert float((p - q).float().abs().max()) <= 8 * torch.finfo(dtype).eps * float(q.float().abs().max())
+        # without an activation the gradient itself is read in place
+        for p, q in zip(ops.linear_act_bwd(G, X, W), ops.linear_act_bwd(g, x, w)):
+            assert bool(torch.isfinite(p).all())
+            assert float((p - q).float().abs().max()) <= 8 * torch.finfo(dtype).eps * float(q.float().abs().max())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_rows_do_not_reach_each_other(dtype):
     """A NaN or an infinity in a row of x stays in that row of y; one in a row of W in that column; nothing behind the
     outputs is written."""
