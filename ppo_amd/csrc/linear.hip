@@ -916,7 +916,8 @@ size_t ppo_linear_act_fwd_workspace_bytes(long rows, long inputs, long outputs, 
 {
     const long e = dtype_bytes(dtype), Kp = k_padded(inputs, e);
     if (!sizes_ok(rows, inputs, outputs, dtype) || few_rows(rows, outputs, inputs, e, true)) return 0;
-    return round256((size_t)rows * Kp * e) + round256((size_t)outputs * Kp * e) + partial_bytes(plan_of(rows, outputs, inputs, e), rows, outputs);
+    const size_t copies = e == 2 ? round256((size_t)rows * Kp * e) + round256((size_t)outputs * Kp * e) : 0;   // f32 is read as it lies
+    return copies + partial_bytes(plan_of(rows, outputs, inputs, e), rows, outputs);
 }
 
 int ppo_linear_act_fwd(const void *x, long x_stride, const void *weight, long weight_stride, const void *bias, const void *residual,
@@ -957,13 +958,13 @@ int ppo_linear_act_fwd(const void *x, long x_stride, const void *weight, long we
             g.A = ws;
             g.lda = Kp * e;
         }
-        ws += round256((size_t)rows * Kp * e);
+        if (e == 2) ws += round256((size_t)rows * Kp * e);
         if (!w_in_place) {
             prep.add(weight, weight_stride, nullptr, outputs, inputs, ws, nullptr, nullptr);
             g.B = ws;
             g.ldb = Kp * e;
         }
-        ws += round256((size_t)outputs * Kp * e);
+        if (e == 2) ws += round256((size_t)outputs * Kp * e);
         const int rc = prep.launch(s);
         if (rc) return rc;
         g.partial = reinterpret_cast<float *>(ws);
@@ -976,10 +977,8 @@ size_t ppo_linear_act_bwd_workspace_bytes(long rows, long inputs, long outputs, 
     if (!sizes_ok(rows, inputs, outputs, dtype)) return 0;
     const long e = dtype_bytes(dtype), Mp = k_padded(rows, e), Np = k_padded(outputs, e);
     const size_t px = partial_bytes(plan_of(rows, inputs, outputs, e), rows, inputs), pw = partial_bytes(plan_of(outputs, inputs, rows, e), outputs, inputs);
-    const long Kp = k_padded(inputs, e);
-    const size_t ut = e == 2 ? round256((size_t)outputs * Mp * e) : 0;
-    return round256((size_t)Mp * Np * e) + ut + round256((size_t)Kp * Np * e) + round256((size_t)Kp * Mp * e) +
-           round256((size_t)((Mp + 63) / 64) * outputs * 4) + (px > pw ? px : pw);
+    const size_t transposed = e == 2 ? round256((size_t)outputs * Mp * e) + round256((size_t)inputs * Np * e) + round256((size_t)inputs * Mp * e) : 0;
+    return round256((size_t)rows * Np * e) + transposed + round256((size_t)((Mp + 63) / 64) * outputs * 4) + (px > pw ? px : pw);
 }
 
 int ppo_linear_act_bwd(const void *g_y, long g_stride, const void *x, long x_stride, const void *weight, long weight_stride,
@@ -995,10 +994,15 @@ int ppo_linear_act_bwd(const void *g_y, long g_stride, const void *x, long x_str
     hipStream_t s = (hipStream_t)stream;
     return by_dtype(dtype, [&](auto t) {
         using T = decltype(t);
-        const long Mp = k_padded(rows, e), Np = k_padded(outputs, e), Kp = k_padded(inputs, e);
+        const long Mp = k_padded(rows, e), Np = k_padded(outputs, e);
         char *ws = reinterpret_cast<char *>(workspace);
         auto take = [&](size_t n) { char *p = ws; ws += round256(n); return p; };
-        char *u = take((size_t)Mp * Np * e), *ut = e == 2 ? take((size_t)outputs * Mp * e) : nullptr, *wt = take((size_t)Kp * Np * e), *xt = take((size_t)Kp * Mp * e);
+        char *u = take((size_t)rows * Np * e), *ut = nullptr, *wt = nullptr, *xt = nullptr;
+        if (e == 2) {
+            ut = take((size_t)outputs * Mp * e);
+            wt = take((size_t)inputs * Np * e);
+            xt = take((size_t)inputs * Mp * e);
+        }
         float *sums = reinterpret_cast<float *>(take((size_t)((Mp + 63) / 64) * outputs * 4));
         float *partial = reinterpret_cast<float *>(ws);
         GemmArgs gx{}, gw{};

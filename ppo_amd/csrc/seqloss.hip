@@ -71,18 +71,18 @@ struct PolicyArgs {
     int kl, per_sequence, sequence_mean, count_blocks;
 };
 
-// unmasked tokens of the rows that this workgroup visits, a wave a row
-__device__ __forceinline__ void count_rows(const PolicyArgs &a, int *row_counts, long first, long step, double (&tot)[2])
+// unmasked tokens of the rows that this workgroup visits, LANES lanes a row
+template <int LANES> __device__ __forceinline__ void count_rows(const PolicyArgs &a, int *row_counts, long first, long step, double (&tot)[2])
 {
-    const int lane = threadIdx.x & 63;
+    const int lane = threadIdx.x % LANES;
     tot[0] = tot[1] = 0.0;
-    for (long b = first + (threadIdx.x >> 6); b < a.B; b += step) {
+    for (long b = first + threadIdx.x / LANES; b < a.B; b += step) {
         int n = 0;
         if (a.mask) {
             const uint8_t *m = a.mask + b * a.mask_stride;
             long t = lane * 16L;
 #pragma unroll 4
-            for (; t + 16 <= a.L; t += 64 * 16) {
+            for (; t + 16 <= a.L; t += LANES * 16) {
                 const Bytes16 v = *reinterpret_cast<const Bytes16 *>(m + t);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
@@ -91,10 +91,9 @@ __device__ __forceinline__ void count_rows(const PolicyArgs &a, int *row_counts,
                     n += __popc((((w & 0x7f7f7f7fu) + 0x7f7f7f7fu) | w) & 0x80808080u);
                 }
             }
-            for (; t < a.L; t += 64 * 16)
-                for (long k = t; k < a.L && k < t + 16; ++k) n += m[k] != 0;
+            for (long k = t; k < a.L && k < t + 16; ++k) n += m[k] != 0;
 #pragma unroll
-            for (int off = 32; off > 0; off >>= 1) n += __shfl_xor(n, off, 64);
+            for (int off = LANES / 2; off > 0; off >>= 1) n += __shfl_xor(n, off, 64);
         } else {
             n = (int)a.L;
         }
@@ -110,7 +109,11 @@ __global__ void __launch_bounds__(SEQ_BLOCK) k_policy_count(PolicyArgs a)
 {
     __shared__ double part[SEQ_BLOCK / 64][2];
     double tot[2];
-    count_rows(a, a.row_counts, (long)blockIdx.x * (SEQ_BLOCK / 64), (long)gridDim.x * (SEQ_BLOCK / 64), tot);
+    // a wave a row, eight rows a wave where they are short
+    if (a.L > 256)
+        count_rows<64>(a, a.row_counts, (long)blockIdx.x * (SEQ_BLOCK / 64), (long)gridDim.x * (SEQ_BLOCK / 64), tot);
+    else
+        count_rows<8>(a, a.row_counts, (long)blockIdx.x * (SEQ_BLOCK / 8), (long)gridDim.x * (SEQ_BLOCK / 8), tot);
     block_sum<2, SEQ_BLOCK>(tot, part);
     if (threadIdx.x == 0) {
         a.counts[2 * blockIdx.x] = tot[0];
@@ -275,7 +278,7 @@ __global__ void __launch_bounds__(ONE_BLOCK) k_policy_one(PolicyArgs a)
     __shared__ double part[ONE_BLOCK / 64][NSUM];
     __shared__ int row_counts[ONE_ROWS];
     double tot[2], acc[NSUM] = {0.0, 0.0, 0.0, 0.0};
-    count_rows(a, row_counts, 0, ONE_BLOCK / 64, tot);
+    count_rows<64>(a, row_counts, 0, ONE_BLOCK / 64, tot);
     block_sum<2, ONE_BLOCK>(tot, part2);           // (its barriers are the row counts' too)
     policy_groups(a, row_counts, tot[0], tot[1], threadIdx.x, ONE_BLOCK, acc);
     block_sum<NSUM, ONE_BLOCK>(acc, part);
@@ -500,6 +503,7 @@ __global__ void __launch_bounds__(SEQ_BLOCK) k_pref_final(PrefArgs a)
 {
     __shared__ double part[SEQ_BLOCK / 64][2];
     double acc[2] = {0.0, 0.0};
+#pragma unroll 8
     for (long b = threadIdx.x; b < a.B; b += SEQ_BLOCK) {
         acc[0] += a.pair[2 * b];
         acc[1] += a.pair[2 * b + 1];
@@ -667,7 +671,7 @@ int ppo_policy_kl_loss(const float *log_probs, long lp_stride, const float *old_
         hipLaunchKernelGGL(k_policy_one, dim3(1), dim3(ONE_BLOCK), 0, s, a);
         return ppo_launch_status();
     }
-    const long cb = (batch + SEQ_BLOCK / 64 - 1) / (SEQ_BLOCK / 64);
+    const long at_once = length > 256 ? SEQ_BLOCK / 64 : SEQ_BLOCK / 8, cb = (batch + at_once - 1) / at_once;
     a.count_blocks = (int)(cb < COUNT_MAX_BLOCKS ? cb : COUNT_MAX_BLOCKS);
     hipLaunchKernelGGL(k_policy_count, dim3(a.count_blocks), dim3(SEQ_BLOCK), 0, s, a);
     int rc = ppo_launch_status();

@@ -76,7 +76,8 @@ def _check(x, w, b, r, g, act):
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("M,K,N", [(1, 1, 1), (1, 7, 5), (1, 64, 16), (1, 1000, 333), (2, 513, 17), (4, 100, 33), (5, 64, 64), (8, 4096, 100), (9, 1, 1),
                                    (9, 33, 15), (16, 128, 17), (100, 64, 130), (127, 65, 129), (128, 128, 128), (129, 127, 257), (255, 192, 64), (256, 256, 256),
-                                   (1000, 96, 40), (40, 2049, 300), (300, 1000, 31), (2047, 129, 65)])
+                                   (1000, 96, 40), (40, 2049, 300), (300, 1000, 31), (2047, 129, 65),
+                                   (40, 1, 33), (33, 2, 70), (200, 3, 5), (100, 50, 1), (65, 4000, 2), (500, 31, 513)])
 def test_sizes(M, K, N, dtype):
     for i, act in enumerate(ACTS if M * N < 40000 else ["none", "gelu"]):
         x, w, b, r, g = _make(M + K + N + i, M, K, N, dtype, bias=i != 1, residual=i != 2)

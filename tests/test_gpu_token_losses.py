@@ -202,7 +202,7 @@ def _check_policy(new, old, adv, mask, refp, kl, reduction, coef=0.3, lo=0.2, hi
 
 
 @pytest.mark.parametrize("mask_kind", ["none", "ragged", "random", "nothing"])
-@pytest.mark.parametrize("B,L", [(1, 1), (1, 3), (3, 4), (4, 17), (7, 129), (64, 64), (300, 5), (33, 1000), (2, 20001), (1000, 33)])
+@pytest.mark.parametrize("B,L", [(1, 1), (1, 3), (3, 4), (4, 17), (7, 129), (64, 64), (300, 5), (33, 1000), (2, 20001), (1000, 33), (5000, 256), (3000, 257), (70000, 3)])
 def test_policy_loss(B, L, mask_kind):
     for i, (kl, reduction) in enumerate((("k1", "token"), ("k2", "sequence"), ("k3", "token"), ("k3", "sequence"))):
         new, old, adv, mask, refp = _policy_case(_gen(B * L + i), B, L, mask_kind, per_sequence=i % 2 == 1)
@@ -277,7 +277,7 @@ def _pairs(gen, B, Lc, Lr, mask_kind):
 
 
 @pytest.mark.parametrize("mask_kind", ["none", "ragged", "random"])
-@pytest.mark.parametrize("B,Lc,Lr", [(1, 1, 1), (1, 5, 0), (0, 3, 4), (4, 33, 40), (300, 7, 130), (3, 9001, 8193), (2, 50001, 17), (17, 1000, 1001)])
+@pytest.mark.parametrize("B,Lc,Lr", [(1, 1, 1), (1, 5, 0), (0, 3, 4), (4, 33, 40), (300, 7, 130), (20000, 3, 5), (70, 600, 5), (3, 9001, 8193), (2, 50001, 17), (17, 1000, 1001)])
 def test_preference_loss(B, Lc, Lr, mask_kind):
     """Sums and the pair's loss are f64: what is left are a rounding of the loss, of a reward and of a gradient to f32."""
     from ppo_amd import ops

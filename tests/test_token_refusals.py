@@ -104,14 +104,14 @@ def test_linear_c_entries_refuse():
     lib = _lib.load()
     buf = (ctypes.c_char * 4096)()
     p = (ctypes.addressof(buf) + 63) // 64 * 64
-    n = lib.ppo_linear_act_fwd_workspace_bytes(64, 8, 8, 0)
+    n = lib.ppo_linear_act_fwd_workspace_bytes(64, 8, 8, 1)
     assert lib.ppo_linear_act_fwd_workspace_bytes(8, 8, 8, 0) == 0 and n > 0
-    fwd = lambda x=p, xs=8, w=p, ws_=8, b=p, r=p, rs=8, dt=0, M=64, K=8, N=8, act=1, y=p, d=p, ws=p, nws=n: lib.ppo_linear_act_fwd(  # noqa: E731
+    fwd = lambda x=p, xs=8, w=p, ws_=8, b=p, r=p, rs=8, dt=1, M=64, K=8, N=8, act=1, y=p, d=p, ws=p, nws=n: lib.ppo_linear_act_fwd(  # noqa: E731
         x, xs, w, ws_, b, r, rs, dt, M, K, N, act, y, d, ws, nws, None)
     assert fwd(M=0) == 0
-    for kw in ({"x": None}, {"x": p + 2}, {"xs": 7}, {"w": None}, {"ws_": 7}, {"w": p + 1}, {"b": p + 2}, {"r": p + 2}, {"rs": 7}, {"dt": 3}, {"dt": -1}, {"M": -1},
-               {"K": 0}, {"N": 0}, {"M": 1 << 22}, {"K": 1 << 22, "xs": 1 << 22, "ws_": 1 << 22}, {"N": 1 << 22}, {"act": 5}, {"act": -1}, {"y": None}, {"y": p + 2},
-               {"d": p + 2}, {"ws": None}, {"ws": p + 8}, {"nws": n - 1}):
+    for kw in ({"x": None}, {"x": p + 1}, {"xs": 7}, {"w": None}, {"ws_": 7}, {"w": p + 1}, {"b": p + 1}, {"r": p + 1}, {"rs": 7}, {"dt": 3}, {"dt": -1}, {"M": -1},
+               {"K": 0}, {"N": 0}, {"M": 1 << 22}, {"K": 1 << 22, "xs": 1 << 22, "ws_": 1 << 22}, {"N": 1 << 22}, {"act": 5}, {"act": -1}, {"y": None}, {"y": p + 1},
+               {"d": p + 1}, {"ws": None}, {"xs": 1 << 22}, {"ws_": 1 << 22}, {"ws": p + 8}, {"nws": n - 1}):
         assert fwd(**kw) == INVALID, kw
     n = lib.ppo_linear_act_bwd_workspace_bytes(16, 8, 8, 0)
     bwd = lambda g=p, gs=8, x=p, xs=8, w=p, ws_=8, d=p, dt=0, M=16, K=8, N=8, gx=p, gw=p, gb=p, ws=p, nws=n: lib.ppo_linear_act_bwd(  # noqa: E731
