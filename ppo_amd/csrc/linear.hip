@@ -8,8 +8,7 @@
 // layers (|d| < 1.2: 8 times finer than bf16) and in f32 for the others, so that the one rounding that counts beside the
 // outputs' own is that of u to the inputs' type, which the two products need; g_b sums u unrounded, in f32.
 //
-// One product, C[m, n] = sum_k A[m, k] B[n, k] with k contiguous in both, serves all three: backward, the operands whose
-// k is not contiguous are transposed by k_prep first (a pass over memory against M N K operations).
+// One product, C[m, n] = sum_k A[m, k] B[n, k], serves all three, each operand with its rows along m (n) or along k.
 //   * 16-bit inputs: v_mfma_f32_16x16x32_{bf16,f16}, f32 accumulators.
 //   * f32 inputs: every operand split in registers into three bf16 pieces that represent it exactly (mfma_split.h), six
 //     products of order <= 2 into one f32 accumulator: the three left out are below 2^-23 of the product.  f32 matrix
@@ -150,14 +149,14 @@ template <class T, int N> __device__ __forceinline__ void store_n(typename T::ra
     }
 }
 
-// ---- operand preparation: pad, multiply by d, transpose, sum columns -----------------------------------------------
-// src [R, C] of T with row stride ld (times mul [R, C] of D<T>, contiguous) -> rows [R, Cp] and / or cols [C, Rp] of T, Cp and Rp
-// the next multiples of a k step, zero-filled; sums [tiles of 64 rows][C] f32 = column sums of a tile.
+// ---- operand preparation: multiply by d, pad, sum columns ----------------------------------------------------------
+// src [R, C] of T with row stride ld (times mul [R, C] of D<T>, contiguous) -> rows [R, Cp] of T, Cp the next multiple of a
+// stage's k, zero-filled; sums [tiles of 64 rows][C] f32 = column sums of a tile.
 struct PrepArgs {
     const void *src, *mul;
-    void *rows, *cols;
+    void *rows;
     float *sums;
-    long R, C, ld, Rp, Cp;
+    long R, C, ld, Cp;
     int tiles_x;                           // tiles of 64 x 64 a row of tiles
 };
 
@@ -175,10 +174,9 @@ template <class T> __global__ void __launch_bounds__(256) k_prep(PrepJobs jobs)
     const long tile_y = id / (unsigned)a.tiles_x, tile_x = id % (unsigned)a.tiles_x;
     constexpr int E = 16 / T::BYTES, TPR = 64 / E, RPP = 256 / TPR;   // threads a row of 64, rows a pass
     using raw = typename T::raw;
-    __shared__ raw tile[64][64 + 4 / T::BYTES];
     __shared__ float colsum[RPP][64];
-    const long r0 = tile_y * 64, c0 = tile_x * 64;
     const int tc = threadIdx.x % TPR * E, tr = threadIdx.x / TPR;
+    const long gc = tile_x * 64 + tc;
     const raw *src = reinterpret_cast<const raw *>(a.src);
     const typename D<T>::raw *mul = reinterpret_cast<const typename D<T>::raw *>(a.mul);
     float sum[E];
@@ -186,8 +184,7 @@ template <class T> __global__ void __launch_bounds__(256) k_prep(PrepJobs jobs)
     for (int j = 0; j < E; ++j) sum[j] = 0.0f;
 #pragma unroll
     for (int p = 0; p < 64 / RPP; ++p) {
-        const int r = p * RPP + tr;
-        const long gr = r0 + r, gc = c0 + tc;
+        const long gr = tile_y * 64 + p * RPP + tr;
         float v[E];
         if (gr < a.R && gc + E <= a.C) {
             load16<T>(src + gr * a.ld + gc, v);
@@ -210,33 +207,15 @@ template <class T> __global__ void __launch_bounds__(256) k_prep(PrepJobs jobs)
 #pragma unroll
         for (int j = 0; j < E; ++j) sum[j] += v[j];
         if (a.rows && gr < a.R && gc < a.Cp) store16<T>(reinterpret_cast<raw *>(a.rows) + gr * a.Cp + gc, v);
-        if (a.cols) {
-#pragma unroll
-            for (int j = 0; j < E; ++j) tile[r][tc + j] = T::store(v[j]);
-        }
     }
-    if (a.sums) {
+    if (!a.sums) return;
 #pragma unroll
-        for (int j = 0; j < E; ++j) colsum[tr][tc + j] = sum[j];
-    }
+    for (int j = 0; j < E; ++j) colsum[tr][tc + j] = sum[j];
     __syncthreads();
-    if (a.cols) {
-#pragma unroll
-        for (int p = 0; p < 64 / RPP; ++p) {
-            const int c = p * RPP + tr;
-            const long gc = c0 + c, gr = r0 + tc;
-            if (gc < a.C && gr < a.Rp) {
-                raw v[E];
-#pragma unroll
-                for (int j = 0; j < E; ++j) v[j] = tile[tc + j][c];
-                *reinterpret_cast<u32x4 *>(reinterpret_cast<raw *>(a.cols) + gc * a.Rp + gr) = __builtin_bit_cast(u32x4, v);
-            }
-        }
-    }
-    if (a.sums && threadIdx.x < 64 && c0 + threadIdx.x < a.C) {
+    if (threadIdx.x < 64 && tile_x * 64 + threadIdx.x < a.C) {
         float s = 0.0f;
         for (int k = 0; k < RPP; ++k) s += colsum[k][threadIdx.x];
-        a.sums[tile_y * a.C + c0 + threadIdx.x] = s;
+        a.sums[tile_y * a.C + tile_x * 64 + threadIdx.x] = s;
     }
 }
 
@@ -321,18 +300,23 @@ template <class T> __device__ __forceinline__ void load_bias(const GemmArgs &g, 
     for (int j = 0; j < E; ++j) bias[j] = p && n + j < g.N ? T::load(p[n + j]) : 0.0f;
 }
 
-// Swizzles: piece c (16 bytes) of a row of 128 bytes lies at c ^ f(row) in LDS.  A ds_read_b128 is served 16 lanes a cycle
-// from 64 banks: lanes {0-3, 12-15, 20-23, 24-27}, {4-11, 16-19, 28-31} and these + 32.  In a fragment read lane l wants
-// piece l / 16 of the fragment's row l % 16, so with f = a r1 ^ b r2 ^ d r3 (r1 .. r3 the row's bits that are lane bits 1 .. 3)
-// the lanes of a group fall into different places (row & 1, c ^ f) if 0, b ^ d, 1 ^ b and 1 ^ d differ modulo a: (4, 2, 3).
-// The f32 fragments' pieces are two apart, which makes that 0, b ^ d, 2 ^ b, 2 ^ d: (4, 1, 3).  (f = row & 7 costs twice the
-// cycles a read.)
-template <int BYTES> __device__ __forceinline__ int swizzle(int r1, int r2, int r3)
+// Swizzles: piece c (16 bytes) of a row of 128 bytes of k lies at c ^ f(row) in LDS.  A ds_read_b128 is served 16 lanes a
+// cycle from 64 banks: lanes {0-3, 12-15, 20-23, 24-27}, {4-11, 16-19, 28-31} and these + 32.  In a fragment read lane l wants
+// piece l / 16 of the fragment's row l % 16, so with f = a r1 ^ b r2 ^ d r3 (r1 .. r3 the bits 1 .. 3 of the row) the lanes of a
+// group fall into different places (row & 1, c ^ f) if 0, b ^ d, 1 ^ b and 1 ^ d differ modulo a: (4, 2, 3).  The f32 fragments'
+// pieces are two apart, which makes that 0, b ^ d, 2 ^ b, 2 ^ d: (4, 1, 3).  (f = row & 7 costs twice the cycles a read.)
+template <int BYTES> __device__ __forceinline__ int swizzle(int row)
 {
-    return (r1 & 1) * 4 ^ (r2 & 1) * (BYTES == 2 ? 2 : 1) ^ (r3 & 1) * 3;
+    return (row >> 1 & 1) * 4 ^ (row >> 2 & 1) * (BYTES == 2 ? 2 : 1) ^ (row >> 3 & 1) * 3;
 }
-template <int BYTES> __device__ __forceinline__ int swizzle_a(int row) { return swizzle<BYTES>(row >> 1, row >> 2, row >> 3); }
-template <int BYTES> __device__ __forceinline__ int swizzle_b(int row) { return swizzle<BYTES>(row >> 1, row >> 4, row >> 5); }
+// Operands whose rows go along k lie in LDS as they come, a row a k.  An f32 fragment is eight reads of a float, one a k, and
+// a row's pieces are moved by 4 (k / 8) so that the four k groups of such a read fall into different banks; a 16-bit one is
+// two ds_read_b64_tr_b16, which hand lane i of 16 the column i of four rows of 16: 32 bytes of 16 rows a read, moved by 32
+// bytes times (k % 4, k / 8 % 2) so that 8 of them fill the banks.
+template <int BYTES> __device__ __forceinline__ int moved(int k)
+{
+    return BYTES == 4 ? (k >> 3) * 4 : ((k & 3) | (k >> 3 & 1) << 2) * 2;
+}
 
 // 64 lanes bring 16 bytes each from rsrc[voff + soff] to LDS at lds + 16 lane.  In asm because the compiler's own form of
 // this load makes every LDS read wait for all of them; it has no destination register, and the loop below waits itself.
@@ -349,14 +333,12 @@ __device__ __forceinline__ u32x4 buffer_of(const void *p, long bytes)
                  (uint32_t)__builtin_amdgcn_readfirstlane((int)n), 0x00027000u};
 }
 
-// KA, KB: that operand lies [k, M] (or [k, N]) with its rows along k (f32 only: the 16-bit fragments' eight k would have to
-// be gathered in 2-byte reads)
+// KA, KB: that operand lies [k, M] (or [k, N]), its rows along k
 template <class T, int BM, int BN, int WAVES_M, int WAVES_N, bool KA, bool KB>
 __global__ void __launch_bounds__(64 * WAVES_M * WAVES_N) k_gemm(GemmArgs g)
 {
-    static_assert((!KA && !KB) || T::BYTES == 4, "f32 only");
     constexpr int WAVES = WAVES_M * WAVES_N, WM = BM / WAVES_M, WN = BN / WAVES_N, MI = WM / 16, NI = 4;
-    static_assert(WN == 64 && MI * 16 * WAVES_M == BM, "a lane's 16 neighbouring n need 64 columns a wave");
+    static_assert(WN == 16 * NI && MI * 16 * WAVES_M == BM, "whole 16 x 16 products");
     constexpr int LA = BM / 8 / WAVES, LB = BN / 8 / WAVES;          // loads a wave and stage (8 rows each)
     constexpr int A_STAGE = BM * 128, B_STAGE = BN * 128, B_AT = 3 * A_STAGE;
     __shared__ __align__(1024) char lds[3 * A_STAGE + 2 * B_STAGE];
@@ -375,37 +357,28 @@ __global__ void __launch_bounds__(64 * WAVES_M * WAVES_N) k_gemm(GemmArgs g)
     const long m0 = (long)(first + id % band % high) * BM, n0 = (long)(id % band / high) * BN;
     const int s0 = blockIdx.y * g.steps_per_split, s1 = s0 + g.steps_per_split < g.steps ? s0 + g.steps_per_split : g.steps;
 
-    const long kbytes = g.K * T::BYTES;
-    constexpr int KS = 128 / T::BYTES;                               // elements of k a stage
+    constexpr int KS = 128 / T::BYTES, ROW_A = BM * T::BYTES, ROW_B = BN * T::BYTES;   // k a stage; bytes of a row along k
+    const long kbytes = (g.K * T::BYTES + 3) / 4 * 4;                // (whole dwords: the last may hold an element that is masked)
     const int tail = s1 == g.steps ? (int)(g.K - (g.steps - 1L) * KS) : KS;   // of the last one
     const long rows_a = g.M - m0 < BM ? g.M - m0 : BM, rows_b = g.N - n0 < BN ? g.N - n0 : BN;
-    const char *pa0 = reinterpret_cast<const char *>(g.A) + (KA ? m0 * 4 : m0 * g.lda), *pb0 = reinterpret_cast<const char *>(g.B) + (KB ? n0 * 4 : n0 * g.ldb);
+    const char *pa0 = reinterpret_cast<const char *>(g.A) + (KA ? m0 * T::BYTES : m0 * g.lda);
+    const char *pb0 = reinterpret_cast<const char *>(g.B) + (KB ? n0 * T::BYTES : n0 * g.ldb);
     const u32x4 ra = buffer_of(pa0, KA ? 0 : (rows_a - 1) * g.lda + kbytes), rb = buffer_of(pb0, KB ? 0 : (rows_b - 1) * g.ldb + kbytes);
-    uint32_t va[LA], vb[LB];           // (256 rows of less than 2^24 bytes: below 2^32)
-#pragma unroll
-    for (int i = 0; i < LA; ++i) {
-        if constexpr (KA) {
-            // a row of LDS is one k: BM floats, whose 16-byte pieces are moved by 4 (k / 8), so that the four k groups of a
-            // fragment read fall into different banks
-            constexpr int PIECES = BM / 4;
-            const int k = (i * WAVES + wave) * (64 / PIECES) + lane / PIECES;
-            va[i] = (uint32_t)k * (uint32_t)g.lda + ((lane % PIECES) ^ (k >> 3) * 4) * 16;
+    // where in the operand what this lane brings in load i lies (256 rows of less than 2^24 bytes: below 2^32)
+    auto offset = [&](auto along_k, int i, int row_bytes, long rows, long ld) {
+        if constexpr (along_k()) {
+            const int pieces = row_bytes / 16, k = (i * WAVES + wave) * (64 / pieces) + lane / pieces;
+            return (uint32_t)k * (uint32_t)ld + ((lane % pieces) ^ moved<T::BYTES>(k)) * 16;
         } else {
-            const int row = (i * WAVES + wave) * 8 + lane / 8, have = row < rows_a ? row : (int)rows_a - 1;   // rows past the end repeat the last
-            va[i] = (uint32_t)have * (uint32_t)g.lda + ((lane % 8) ^ swizzle_a<T::BYTES>(row)) * 16;
+            const int row = (i * WAVES + wave) * 8 + lane / 8, have = row < rows ? row : (int)rows - 1;   // rows past the end repeat the last
+            return (uint32_t)have * (uint32_t)ld + ((lane % 8) ^ swizzle<T::BYTES>(row)) * 16;
         }
-    }
+    };
+    uint32_t va[LA], vb[LB];
 #pragma unroll
-    for (int i = 0; i < LB; ++i) {
-        if constexpr (KB) {
-            constexpr int PIECES = BN / 4;             // (B's rows are read 4 neighbours at a time, 16 apart: moved by k / 8)
-            const int k = (i * WAVES + wave) * (64 / PIECES) + lane / PIECES;
-            vb[i] = (uint32_t)k * (uint32_t)g.ldb + ((lane % PIECES) ^ (k >> 3)) * 16;
-        } else {
-            const int row = (i * WAVES + wave) * 8 + lane / 8, have = row < rows_b ? row : (int)rows_b - 1;
-            vb[i] = (uint32_t)have * (uint32_t)g.ldb + ((lane % 8) ^ swizzle_b<T::BYTES>(row)) * 16;
-        }
-    }
+    for (int i = 0; i < LA; ++i) va[i] = offset(std::bool_constant<KA>{}, i, ROW_A, rows_a, g.lda);
+#pragma unroll
+    for (int i = 0; i < LB; ++i) vb[i] = offset(std::bool_constant<KB>{}, i, ROW_B, rows_b, g.ldb);
     const uint32_t base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds;
     // load i of a stage's A or B to the place that begins at `to`.  What is read past a row's end is the next row's beginning,
     // or nothing behind the last row: past K it is masked out of the last stage's fragments, and where the operand's rows go
@@ -413,14 +386,14 @@ __global__ void __launch_bounds__(64 * WAVES_M * WAVES_N) k_gemm(GemmArgs g)
     auto load_a = [&](int s, int to, int i) {
         const uint32_t at = base + wave * 1024 + to + i * WAVES * 1024;
         if constexpr (KA)
-            load_lds(buffer_of(pa0 + s * 32L * g.lda, (g.K - s * 32L - 1) * g.lda + (g.M - m0) * 4), va[i], 0, at);
+            load_lds(buffer_of(pa0 + (long)s * KS * g.lda, (g.K - (long)s * KS - 1) * g.lda + ((g.M - m0) * T::BYTES + 3) / 4 * 4), va[i], 0, at);
         else
             load_lds(ra, va[i], s * 128, at);
     };
     auto load_b = [&](int s, int to, int i) {
         const uint32_t at = base + wave * 1024 + B_AT + to + i * WAVES * 1024;
         if constexpr (KB)
-            load_lds(buffer_of(pb0 + s * 32L * g.ldb, (g.K - s * 32L - 1) * g.ldb + (g.N - n0) * 4), vb[i], 0, at);
+            load_lds(buffer_of(pb0 + (long)s * KS * g.ldb, (g.K - (long)s * KS - 1) * g.ldb + ((g.N - n0) * T::BYTES + 3) / 4 * 4), vb[i], 0, at);
         else
             load_lds(rb, vb[i], s * 128, at);
     };
@@ -433,11 +406,13 @@ __global__ void __launch_bounds__(64 * WAVES_M * WAVES_N) k_gemm(GemmArgs g)
         for (int i = 0; i < LB; ++i) load_b(s, to, i);
     };
 
-    // fragment reads: lane q = lane % 16 reads k piece lane / 16 of A's row q and of B's row n(q) = 16 (q / 4) + q % 4 (+ 4 j);
-    // a lane's results are those of B's fragment rows 4 (lane / 16) + e, e < 4, which n() makes 16 neighbours over the j
+    // fragment reads: lane q = lane % 16 reads k piece kg = lane / 16 of row q (+ 16 i or 16 j) of a wave's rows
     const int q = lane & 15, kg = lane >> 4;
-    const int row_a = wm * WM + q, row_b = wn * WN + (q >> 2) * 16 + (q & 3);
-    const int pa = row_a * 128, pb = B_AT + row_b * 128, xa = swizzle_a<T::BYTES>(row_a), xb = swizzle_b<T::BYTES>(row_b);
+    const int row_a = wm * WM + q, row_b = wn * WN + q;
+    const int pa = row_a * 128, pb = B_AT + row_b * 128, xa = swizzle<T::BYTES>(row_a), xb = swizzle<T::BYTES>(row_b);
+    // along k, 16 bits: the lane's four columns of row k of its group; column block i lies at ^ 32 i
+    const int tk = kg * 8 + (q >> 2), tm = moved<2>(tk) * 16;
+    const int ta = tk * ROW_A + ((wm * WM * 2 + (q & 3) * 8) ^ tm), tb = B_AT + tk * ROW_B + ((wn * WN * 2 + (q & 3) * 8) ^ tm);
 
     f32x4 acc[MI][NI];
 #pragma unroll
@@ -459,12 +434,27 @@ __global__ void __launch_bounds__(64 * WAVES_M * WAVES_N) k_gemm(GemmArgs g)
         struct Half { u32x4 a[MI], b[NI]; };
         Half h0, h1;
         // one read of a half's fragments, in the order in which its products want them
+        auto turned = [&](int at, int row_bytes) {
+            using s4 = __attribute__((ext_vector_type(4))) short;
+            using u2 = __attribute__((ext_vector_type(2))) uint32_t;
+            typedef __attribute__((address_space(3))) s4 *ptr;
+            const u2 lo = __builtin_bit_cast(u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((ptr)(lds + at)));
+            const u2 hi = __builtin_bit_cast(u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((ptr)(lds + at + 4 * row_bytes)));
+            return u32x4{lo[0], lo[1], hi[0], hi[1]};
+        };
         auto fetch = [&](int at_a, int at_b, int half, Half &h, int r) {
             const int c = half * 4 + kg;
-            if (r < NI)
-                h.b[r] = *reinterpret_cast<const u32x4 *>(lds + at_b + pb + r * 512 + (c ^ xb) * 16);
-            else
-                h.a[r - NI] = *reinterpret_cast<const u32x4 *>(lds + at_a + pa + (r - NI) * 2048 + (c ^ xa) * 16);
+            if (r < NI) {
+                if constexpr (KB)
+                    h.b[r] = turned(((at_b + tb) ^ r * 32) + half * 32 * ROW_B, ROW_B);
+                else
+                    h.b[r] = *reinterpret_cast<const u32x4 *>(lds + at_b + pb + r * 2048 + (c ^ xb) * 16);
+            } else {
+                if constexpr (KA)
+                    h.a[r - NI] = turned(((at_a + ta) ^ (r - NI) * 32) + half * 32 * ROW_A, ROW_A);
+                else
+                    h.a[r - NI] = *reinterpret_cast<const u32x4 *>(lds + at_a + pa + (r - NI) * 2048 + (c ^ xa) * 16);
+            }
         };
         // a half's products one by one, and between them, in this order, the reads of the next half and the loads: left to
         // itself the compiler sends all loads first, which blocks the wave, and with it its products, until the address
@@ -484,16 +474,17 @@ __global__ void __launch_bounds__(64 * WAVES_M * WAVES_N) k_gemm(GemmArgs g)
         static_assert(2 * R <= MI * NI, "room for the reads");
         const int n = s1 - s0;
         int a_now = 0, a_next = A_STAGE, b_now = 0, b_next = B_STAGE;
-        // what lies past K in the last stage is not of this row: 0.  (K is even: a pair of halves is in or out)
+        // what lies past K in the last stage is not of this row: 0
         auto cut = [&](Half &h, int half) {
             if (tail < KS) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const bool out = half * 32 + kg * 8 + 2 * e >= tail;
+                    const int in = tail - (half * 32 + kg * 8 + 2 * e);
+                    const uint32_t keep = in >= 2 ? 0xffffffffu : in == 1 ? 0xffffu : 0u;
 #pragma unroll
-                    for (int j = 0; j < NI; ++j) h.b[j][e] = out ? 0u : h.b[j][e];
+                    for (int j = 0; j < NI; ++j) h.b[j][e] &= keep;
 #pragma unroll
-                    for (int i = 0; i < MI; ++i) h.a[i][e] = out ? 0u : h.a[i][e];
+                    for (int i = 0; i < MI; ++i) h.a[i][e] &= keep;
                 }
             }
         };
@@ -581,11 +572,11 @@ __global__ void __launch_bounds__(64 * WAVES_M * WAVES_N) k_gemm(GemmArgs g)
             // eight k of one row: two pieces of it, or a float of each of eight rows of k
             auto read_a = [&](int i, f32x4 &lo, f32x4 &hi) {
                 if constexpr (KA) {
-                    const char *p = at_a + kg * 8 * (BM * 4) + ((row_a + i * 16) ^ kg * 16) * 4;
+                    const char *p = at_a + kg * 8 * ROW_A + ((row_a + i * 16) ^ kg * 16) * 4;
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        lo[e] = *reinterpret_cast<const float *>(p + e * (BM * 4));
-                        hi[e] = *reinterpret_cast<const float *>(p + (e + 4) * (BM * 4));
+                        lo[e] = *reinterpret_cast<const float *>(p + e * ROW_A);
+                        hi[e] = *reinterpret_cast<const float *>(p + (e + 4) * ROW_A);
                     }
                 } else {
                     lo = *reinterpret_cast<const f32x4 *>(at_a + pa + i * 2048 + ca0);
@@ -594,15 +585,15 @@ __global__ void __launch_bounds__(64 * WAVES_M * WAVES_N) k_gemm(GemmArgs g)
             };
             auto read_b = [&](int j, f32x4 &lo, f32x4 &hi) {
                 if constexpr (KB) {
-                    const char *p = at_b + B_AT + kg * 8 * (BN * 4) + ((row_b + j * 4) ^ kg * 4) * 4;
+                    const char *p = at_b + B_AT + kg * 8 * ROW_B + ((row_b + j * 16) ^ kg * 16) * 4;
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        lo[e] = *reinterpret_cast<const float *>(p + e * (BN * 4));
-                        hi[e] = *reinterpret_cast<const float *>(p + (e + 4) * (BN * 4));
+                        lo[e] = *reinterpret_cast<const float *>(p + e * ROW_B);
+                        hi[e] = *reinterpret_cast<const float *>(p + (e + 4) * ROW_B);
                     }
                 } else {
-                    lo = *reinterpret_cast<const f32x4 *>(at_b + pb + j * 512 + cb0);
-                    hi = *reinterpret_cast<const f32x4 *>(at_b + pb + j * 512 + cb1);
+                    lo = *reinterpret_cast<const f32x4 *>(at_b + pb + j * 2048 + cb0);
+                    hi = *reinterpret_cast<const f32x4 *>(at_b + pb + j * 2048 + cb1);
                 }
             };
             auto cut = [&](f32x4 &lo, f32x4 &hi) {          // k past K are not of this row
@@ -641,7 +632,7 @@ __global__ void __launch_bounds__(64 * WAVES_M * WAVES_N) k_gemm(GemmArgs g)
         step(s1 - 1, std::true_type{});
     }
 
-    // acc[i][j][e] is C[m0 + wm WM + 16 i + q][n0 + wn WN + 16 kg + 4 j + e].  The results go through LDS, PI rows of
+    // acc[i][j][e] is C[m0 + wm WM + 16 i + q][n0 + wn WN + 16 j + 4 kg + e].  The results go through LDS, PI rows of
     // products of every wave at a time, so that a wave finishes and stores whole rows: from the accumulators' layout a
     // store touched 32 cache lines, and each residual and derivative as many again.  (A pad of 16 bytes a row puts the 16
     // rows of a write into different banks.)
@@ -658,7 +649,7 @@ __global__ void __launch_bounds__(64 * WAVES_M * WAVES_N) k_gemm(GemmArgs g)
         for (int i = 0; i < PI; ++i)
 #pragma unroll
             for (int j = 0; j < NI; ++j)
-                *reinterpret_cast<f32x4 *>(lds + ((wm * PI + i) * 16 + q) * LD + (wn * WN + kg * 16 + j * 4) * 4) = acc[pass * PI + i][j];
+                *reinterpret_cast<f32x4 *>(lds + ((wm * PI + i) * 16 + q) * LD + (wn * WN + j * 16 + kg * 4) * 4) = acc[pass * PI + i][j];
         __syncthreads();
 #pragma clang loop unroll(disable)
         for (int r = row0; r < ROWS; r += STEP) {
@@ -839,15 +830,10 @@ Plan plan_of(long M, long N, long K, long e)
 size_t round256(size_t n) { return (n + 255) / 256 * 256; }
 size_t partial_bytes(const Plan &p, long M, long N) { return p.splits > 1 ? round256((size_t)p.splits * M * N * 4) : 0; }
 
-// The loads take 16 bytes from any multiple of 4, so f32 operands are read as they lie, and 16-bit ones whose rows hold and
-// are an even number of elements apart; the others are copied to padded rows first.
-bool in_place(const void *p, long ld, long K, long e)
-{
-    return ppo_aligned(p, 4) && (e == 4 || (ld % 2 == 0 && K % 2 == 0));
-}
-
-// k as the kernel counts it: an odd number of halves is in padded copies only, whose rest is 0
-long whole_k(long K, long e) { return e == 2 && K % 2 ? k_padded(K, e) : K; }
+// The loads take 16 bytes from any multiple of 4, so f32 operands are read as they lie, and 16-bit ones whose rows are an
+// even number of elements apart (and, along a row, hold an even number of k); the others are copied to padded rows first.
+bool in_place_along_k(const void *p, long ld, long e) { return ppo_aligned(p, 4) && (e == 4 || ld % 2 == 0); }
+bool in_place(const void *p, long ld, long K, long e) { return in_place_along_k(p, ld, e) && (e == 4 || K % 2 == 0); }
 
 // collects what a call has to prepare, for one launch
 template <class T> struct Prep {
@@ -855,12 +841,10 @@ template <class T> struct Prep {
     int count = 0;
     long tiles = 0;
 
-    void add(const void *src, long ld, const void *mul, long R, long C, void *rows, void *cols, float *sums)
+    void add(const void *src, long ld, const void *mul, long R, long C, void *rows, float *sums)
     {
-        constexpr long e = T::BYTES;
-        PrepArgs a{src, mul, rows, cols, sums, R, C, ld, k_padded(R, e), k_padded(C, e), 0};
-        // whole k steps in both directions: what lies past the matrix becomes zero
-        const long gr = cols ? (a.Rp + 63) / 64 : (R + 63) / 64, gc = rows ? (a.Cp + 63) / 64 : (C + 63) / 64;
+        PrepArgs a{src, mul, rows, sums, R, C, ld, k_padded(C, T::BYTES), 0};
+        const long gr = (R + 63) / 64, gc = ((rows ? a.Cp : C) + 63) / 64;   // what lies past a row's end becomes zero
         a.tiles_x = (int)gc;
         jobs.job[count] = a;
         tiles += gr * gc;
@@ -954,13 +938,13 @@ int ppo_linear_act_fwd(const void *x, long x_stride, const void *weight, long we
         const long Kp = k_padded(inputs, e);
         Prep<T> prep;
         if (!in_place(x, x_stride, inputs, e)) {
-            prep.add(x, x_stride, nullptr, rows, inputs, ws, nullptr, nullptr);
+            prep.add(x, x_stride, nullptr, rows, inputs, ws, nullptr);
             g.A = ws;
             g.lda = Kp * e;
         }
         if (e == 2) ws += round256((size_t)rows * Kp * e);
         if (!w_in_place) {
-            prep.add(weight, weight_stride, nullptr, outputs, inputs, ws, nullptr, nullptr);
+            prep.add(weight, weight_stride, nullptr, outputs, inputs, ws, nullptr);
             g.B = ws;
             g.ldb = Kp * e;
         }
@@ -968,17 +952,17 @@ int ppo_linear_act_fwd(const void *x, long x_stride, const void *weight, long we
         const int rc = prep.launch(s);
         if (rc) return rc;
         g.partial = reinterpret_cast<float *>(ws);
-        return gemm<T, false, false>(g, whole_k(inputs, e), plan_of(rows, outputs, inputs, e), s);
+        return gemm<T, false, false>(g, inputs, plan_of(rows, outputs, inputs, e), s);
     });
 }
 
 size_t ppo_linear_act_bwd_workspace_bytes(long rows, long inputs, long outputs, int dtype)
 {
     if (!sizes_ok(rows, inputs, outputs, dtype)) return 0;
-    const long e = dtype_bytes(dtype), Mp = k_padded(rows, e), Np = k_padded(outputs, e);
+    const long e = dtype_bytes(dtype), Np = k_padded(outputs, e), Kp = k_padded(inputs, e);
     const size_t px = partial_bytes(plan_of(rows, inputs, outputs, e), rows, inputs), pw = partial_bytes(plan_of(outputs, inputs, rows, e), outputs, inputs);
-    const size_t transposed = e == 2 ? round256((size_t)outputs * Mp * e) + round256((size_t)inputs * Np * e) + round256((size_t)inputs * Mp * e) : 0;
-    return round256((size_t)rows * Np * e) + transposed + round256((size_t)((Mp + 63) / 64) * outputs * 4) + (px > pw ? px : pw);
+    const size_t copies = e == 2 ? round256((size_t)outputs * Kp * e) + round256((size_t)rows * Kp * e) : 0;   // f32 is read as it lies
+    return round256((size_t)rows * Np * e) + copies + round256((size_t)((rows + 63) / 64) * outputs * 4) + (px > pw ? px : pw);
 }
 
 int ppo_linear_act_bwd(const void *g_y, long g_stride, const void *x, long x_stride, const void *weight, long weight_stride,
@@ -994,52 +978,38 @@ int ppo_linear_act_bwd(const void *g_y, long g_stride, const void *x, long x_str
     hipStream_t s = (hipStream_t)stream;
     return by_dtype(dtype, [&](auto t) {
         using T = decltype(t);
-        const long Mp = k_padded(rows, e), Np = k_padded(outputs, e);
+        const long Np = k_padded(outputs, e), Kp = k_padded(inputs, e);
         char *ws = reinterpret_cast<char *>(workspace);
         auto take = [&](size_t n) { char *p = ws; ws += round256(n); return p; };
-        char *u = take((size_t)rows * Np * e), *ut = nullptr, *wt = nullptr, *xt = nullptr;
-        if (e == 2) {
-            ut = take((size_t)outputs * Mp * e);
-            wt = take((size_t)inputs * Np * e);
-            xt = take((size_t)inputs * Mp * e);
-        }
-        float *sums = reinterpret_cast<float *>(take((size_t)((Mp + 63) / 64) * outputs * 4));
+        char *u = take((size_t)rows * Np * e), *wc = e == 2 ? take((size_t)outputs * Kp * e) : nullptr, *xc = e == 2 ? take((size_t)rows * Kp * e) : nullptr;
+        float *sums = reinterpret_cast<float *>(take((size_t)((rows + 63) / 64) * outputs * 4));
         float *partial = reinterpret_cast<float *>(ws);
-        GemmArgs gx{}, gw{};
+        GemmArgs gx{}, gw{};               // u W over the outputs, and u^T x over the rows: W, u and x are read along k as they lie
         gx.M = rows; gx.N = inputs; gx.out = g_x; gx.act = PPO_ACT_NONE; gx.partial = partial;
         gw.M = outputs; gw.N = inputs; gw.out = g_weight; gw.act = PPO_ACT_NONE; gw.partial = partial;
-        const Plan plan_x = plan_of(rows, inputs, outputs, e), plan_w = plan_of(outputs, inputs, rows, e);
-        const bool row_in_place = !deriv && in_place(g_y, g_stride, outputs, e);   // g_x's A
+        const bool u_in_place = !deriv && in_place(g_y, g_stride, outputs, e), write_u = (g_x || g_weight) && !u_in_place;
         Prep<T> prep;
-        long tiles = 0;                    // of 64 rows of u, for its column sums
-        if constexpr (T::BYTES == 4) {
-            // u and W and x are read along k as they lie
-            const bool write_u = (g_x || g_weight) && !row_in_place;
-            if (write_u || g_bias) prep.add(g_y, g_stride, deriv, rows, outputs, write_u ? u : nullptr, nullptr, g_bias ? sums : nullptr);
-            tiles = (rows + 63) / 64;
-            gx.A = gw.A = row_in_place ? g_y : u;
-            gx.lda = gw.lda = (row_in_place ? g_stride : Np) * e;
-            gx.B = weight; gx.ldb = weight_stride * e;
-            gw.B = x; gw.ldb = x_stride * e;
-        } else {
-            const bool want_rows = g_x && !row_in_place;
-            if (want_rows || g_weight || g_bias)
-                prep.add(g_y, g_stride, deriv, rows, outputs, want_rows ? u : nullptr, g_weight ? ut : nullptr, g_bias ? sums : nullptr);
-            tiles = ((g_weight ? Mp : rows) + 63) / 64;
-            if (g_x) prep.add(weight, weight_stride, nullptr, outputs, inputs, nullptr, wt, nullptr);
-            gx.A = row_in_place ? g_y : u; gx.lda = (row_in_place ? g_stride : Np) * e; gx.B = wt; gx.ldb = Np * e;
-            if (g_weight) prep.add(x, x_stride, nullptr, rows, inputs, nullptr, xt, nullptr);
-            gw.A = ut; gw.lda = Mp * e; gw.B = xt; gw.ldb = Mp * e;
+        if (write_u || g_bias) prep.add(g_y, g_stride, deriv, rows, outputs, write_u ? u : nullptr, g_bias ? sums : nullptr);
+        gx.A = gw.A = u_in_place ? g_y : u;
+        gx.lda = gw.lda = (u_in_place ? g_stride : Np) * e;
+        gx.B = weight; gx.ldb = weight_stride * e;
+        if (g_x && !in_place_along_k(weight, weight_stride, e)) {
+            prep.add(weight, weight_stride, nullptr, outputs, inputs, wc, nullptr);
+            gx.B = wc; gx.ldb = Kp * e;
+        }
+        gw.B = x; gw.ldb = x_stride * e;
+        if (g_weight && !in_place_along_k(x, x_stride, e)) {
+            prep.add(x, x_stride, nullptr, rows, inputs, xc, nullptr);
+            gw.B = xc; gw.ldb = Kp * e;
         }
         int rc = prep.launch(s);
         if (!rc && g_bias) {
-            hipLaunchKernelGGL(k_bias_grad<T>, dim3((unsigned)((outputs + 63) / 64)), dim3(1024), 0, s, sums, tiles, outputs,
+            hipLaunchKernelGGL(k_bias_grad<T>, dim3((unsigned)((outputs + 63) / 64)), dim3(1024), 0, s, sums, (rows + 63) / 64, outputs,
                                reinterpret_cast<typename T::raw *>(g_bias));
             rc = ppo_launch_status();
         }
-        constexpr bool ALONG = T::BYTES == 4;
-        if (!rc && g_x) rc = gemm<T, false, ALONG>(gx, whole_k(outputs, e), plan_x, s);
-        if (!rc && g_weight) rc = gemm<T, ALONG, ALONG>(gw, whole_k(rows, e), plan_w, s);
+        if (!rc && g_x) rc = gemm<T, false, true>(gx, outputs, plan_of(rows, inputs, outputs, e), s);
+        if (!rc && g_weight) rc = gemm<T, true, true>(gw, rows, plan_of(outputs, inputs, rows, e), s);
         return rc;
     });
 }
