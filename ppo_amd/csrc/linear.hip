@@ -13,12 +13,12 @@
 //   * f32 inputs: every operand split in registers into three bf16 pieces that represent it exactly (mfma_split.h), six
 //     products of order <= 2 into one f32 accumulator: the three left out are below 2^-23 of the product.  f32 matrix
 //     instructions run at 1/16 of the bf16 rate, so six of these are 2.7 times as fast.  An infinite operand gives NaN.
-// A workgroup of 8 waves computes 256 x 256 of C (4 waves: 128 x 128, where there would be too few of the larger ones),
-// a wave 128 x 64 (64 x 64) of it.  Rows of 128 bytes of k (64 halves, 32 floats) are brought straight into LDS, two
-// stages, the next one on its way while the matrix cores work on this one.  16-byte pieces are swizzled inside their row
-// so that the 16 rows a fragment read touches fall into different banks; A and B have their own swizzles because B's rows
-// are read in an order that gives a lane 16 neighbouring n of the result, i.e. whole 32- or 64-byte stores.
-// The operands of v_mfma are swapped (B first), so that a lane's accumulators run along n.
+// A workgroup of 8 waves computes 256 x 256 of C (4 waves: 128 x 128 where there would be too few of the larger ones, 128 x 64
+// or 64 x 128 where C has no more columns or rows), a wave 128 x 64, 64 x 64 or 32 x 64 of it.  Rows of 128 bytes of k (64
+// halves, 32 floats; where an operand's rows go along k, as many rows of the tile's width) are brought straight into LDS, the
+// next stages on their way while the matrix cores work on this one.  16-byte pieces are swizzled inside their row so that what
+// a fragment read touches falls into different banks.  The operands of v_mfma are swapped (B first), so that a lane's
+// accumulators run along n.
 #include "token_common.h"
 #include "mfma_split.h"
 
@@ -313,9 +313,10 @@ template <int BYTES> __device__ __forceinline__ int swizzle(int row)
 // a row's pieces are moved by 4 (k / 8) so that the four k groups of such a read fall into different banks; a 16-bit one is
 // two ds_read_b64_tr_b16, which hand lane i of 16 the column i of four rows of 16: 32 bytes of 16 rows a read, moved by 32
 // bytes times (k % 4, k / 8 % 2) so that 8 of them fill the banks.
-template <int BYTES> __device__ __forceinline__ int moved(int k)
+template <int BYTES, int ROW> __device__ __forceinline__ int moved(int k)
 {
-    return BYTES == 4 ? (k >> 3) * 4 : ((k & 3) | (k >> 3 & 1) << 2) * 2;
+    if constexpr (BYTES == 4) return (k >> 3) * 4;
+    return (ROW == 128 ? (k >> 1 & 1) | (k >> 3 & 1) << 1 : (k & 3) | (k >> 3 & 1) << 2) * 2;   // (rows of 128 bytes: k & 1 moves them already)
 }
 
 // 64 lanes bring 16 bytes each from rsrc[voff + soff] to LDS at lds + 16 lane.  In asm because the compiler's own form of
@@ -340,8 +341,10 @@ __global__ void __launch_bounds__(64 * WAVES_M * WAVES_N) k_gemm(GemmArgs g)
     constexpr int WAVES = WAVES_M * WAVES_N, WM = BM / WAVES_M, WN = BN / WAVES_N, MI = WM / 16, NI = 4;
     static_assert(WN == 16 * NI && MI * 16 * WAVES_M == BM, "whole 16 x 16 products");
     constexpr int LA = BM / 8 / WAVES, LB = BN / 8 / WAVES;          // loads a wave and stage (8 rows each)
-    constexpr int A_STAGE = BM * 128, B_STAGE = BN * 128, B_AT = 3 * A_STAGE;
-    __shared__ __align__(1024) char lds[3 * A_STAGE + 2 * B_STAGE];
+    constexpr int A_STAGE = BM * 128, B_STAGE = BN * 128, B_AT = (T::BYTES == 2 ? 3 : 2) * A_STAGE;
+    constexpr int PI = MI < 4 ? MI : 4, ROWS = WAVES_M * 16 * PI, LD = BN * 4 + 16;   // the results' way out, below
+    constexpr int STAGES = B_AT + 2 * B_STAGE;
+    __shared__ __align__(1024) char lds[STAGES > ROWS * LD ? STAGES : ROWS * LD];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave / WAVES_N, wn = wave % WAVES_N;
 
@@ -365,10 +368,11 @@ __global__ void __launch_bounds__(64 * WAVES_M * WAVES_N) k_gemm(GemmArgs g)
     const char *pb0 = reinterpret_cast<const char *>(g.B) + (KB ? n0 * T::BYTES : n0 * g.ldb);
     const u32x4 ra = buffer_of(pa0, KA ? 0 : (rows_a - 1) * g.lda + kbytes), rb = buffer_of(pb0, KB ? 0 : (rows_b - 1) * g.ldb + kbytes);
     // where in the operand what this lane brings in load i lies (256 rows of less than 2^24 bytes: below 2^32)
-    auto offset = [&](auto along_k, int i, int row_bytes, long rows, long ld) {
+    auto offset = [&](auto along_k, auto row_bytes, int i, long rows, long ld) {
         if constexpr (along_k()) {
-            const int pieces = row_bytes / 16, k = (i * WAVES + wave) * (64 / pieces) + lane / pieces;
-            return (uint32_t)k * (uint32_t)ld + ((lane % pieces) ^ moved<T::BYTES>(k)) * 16;
+            constexpr int pieces = row_bytes() / 16;
+            const int k = (i * WAVES + wave) * (64 / pieces) + lane / pieces;
+            return (uint32_t)k * (uint32_t)ld + ((lane % pieces) ^ moved<T::BYTES, row_bytes()>(k)) * 16;
         } else {
             const int row = (i * WAVES + wave) * 8 + lane / 8, have = row < rows ? row : (int)rows - 1;   // rows past the end repeat the last
             return (uint32_t)have * (uint32_t)ld + ((lane % 8) ^ swizzle<T::BYTES>(row)) * 16;
@@ -376,24 +380,41 @@ __global__ void __launch_bounds__(64 * WAVES_M * WAVES_N) k_gemm(GemmArgs g)
     };
     uint32_t va[LA], vb[LB];
 #pragma unroll
-    for (int i = 0; i < LA; ++i) va[i] = offset(std::bool_constant<KA>{}, i, ROW_A, rows_a, g.lda);
+    for (int i = 0; i < LA; ++i) va[i] = offset(std::bool_constant<KA>{}, std::integral_constant<int, ROW_A>{}, i, rows_a, g.lda);
 #pragma unroll
-    for (int i = 0; i < LB; ++i) vb[i] = offset(std::bool_constant<KB>{}, i, ROW_B, rows_b, g.ldb);
+    for (int i = 0; i < LB; ++i) vb[i] = offset(std::bool_constant<KB>{}, std::integral_constant<int, ROW_B>{}, i, rows_b, g.ldb);
     const uint32_t base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds;
     // load i of a stage's A or B to the place that begins at `to`.  What is read past a row's end is the next row's beginning,
     // or nothing behind the last row: past K it is masked out of the last stage's fragments, and where the operand's rows go
     // along k it belongs to columns whose results are not kept.
+    // Along k the descriptor begins at the stage's first row and goes on to the operand's end; stages are loaded one after the
+    // other.  (Worked out anew for each it takes 40 scalar instructions a stage, as long as a tile of 128 x 128's products.)
+    struct Along {
+        const char *p;
+        long left, step;
+        __device__ u32x4 take(bool last)
+        {
+            const u32x4 d = buffer_of(p, left);
+            if (last) {
+                p += step;
+                left -= step;
+            }
+            return d;
+        }
+    };
+    Along al{pa0 + (long)s0 * KS * g.lda, (g.K - (long)s0 * KS - 1) * g.lda + ((g.M - m0) * T::BYTES + 3) / 4 * 4, KS * g.lda};
+    Along bl{pb0 + (long)s0 * KS * g.ldb, (g.K - (long)s0 * KS - 1) * g.ldb + ((g.N - n0) * T::BYTES + 3) / 4 * 4, KS * g.ldb};
     auto load_a = [&](int s, int to, int i) {
         const uint32_t at = base + wave * 1024 + to + i * WAVES * 1024;
         if constexpr (KA)
-            load_lds(buffer_of(pa0 + (long)s * KS * g.lda, (g.K - (long)s * KS - 1) * g.lda + ((g.M - m0) * T::BYTES + 3) / 4 * 4), va[i], 0, at);
+            load_lds(al.take(i == LA - 1), va[i], 0, at);
         else
             load_lds(ra, va[i], s * 128, at);
     };
     auto load_b = [&](int s, int to, int i) {
         const uint32_t at = base + wave * 1024 + B_AT + to + i * WAVES * 1024;
         if constexpr (KB)
-            load_lds(buffer_of(pb0 + (long)s * KS * g.ldb, (g.K - (long)s * KS - 1) * g.ldb + ((g.N - n0) * T::BYTES + 3) / 4 * 4), vb[i], 0, at);
+            load_lds(bl.take(i == LB - 1), vb[i], 0, at);
         else
             load_lds(rb, vb[i], s * 128, at);
     };
@@ -411,8 +432,9 @@ __global__ void __launch_bounds__(64 * WAVES_M * WAVES_N) k_gemm(GemmArgs g)
     const int row_a = wm * WM + q, row_b = wn * WN + q;
     const int pa = row_a * 128, pb = B_AT + row_b * 128, xa = swizzle<T::BYTES>(row_a), xb = swizzle<T::BYTES>(row_b);
     // along k, 16 bits: the lane's four columns of row k of its group; column block i lies at ^ 32 i
-    const int tk = kg * 8 + (q >> 2), tm = moved<2>(tk) * 16;
-    const int ta = tk * ROW_A + ((wm * WM * 2 + (q & 3) * 8) ^ tm), tb = B_AT + tk * ROW_B + ((wn * WN * 2 + (q & 3) * 8) ^ tm);
+    const int tk = kg * 8 + (q >> 2);
+    const int ta = tk * ROW_A + ((wm * WM * 2 + (q & 3) * 8) ^ moved<2, ROW_A>(tk) * 16);
+    const int tb = B_AT + tk * ROW_B + ((wn * WN * 2 + (q & 3) * 8) ^ moved<2, ROW_B>(tk) * 16);
 
     f32x4 acc[MI][NI];
 #pragma unroll
@@ -470,8 +492,8 @@ __global__ void __launch_bounds__(64 * WAVES_M * WAVES_N) k_gemm(GemmArgs g)
                 __builtin_amdgcn_sched_barrier(0);
             }
         };
-        constexpr int R = MI + NI;                          // a read to every other product, the last few without
-        static_assert(2 * R <= MI * NI, "room for the reads");
+        constexpr int R = MI + NI, GAP = 2 * R <= MI * NI ? 2 : 1;   // a read to every other product where there are enough
+        static_assert(GAP * R <= MI * NI && LA + LB <= MI * NI, "room for the reads and loads");
         const int n = s1 - s0;
         int a_now = 0, a_next = A_STAGE, b_now = 0, b_next = B_STAGE;
         // what lies past K in the last stage is not of this row: 0
@@ -491,7 +513,7 @@ __global__ void __launch_bounds__(64 * WAVES_M * WAVES_N) k_gemm(GemmArgs g)
         auto turn = [&](int s, auto left) {                 // left: stages behind this one, 3 for three or more
             if constexpr (left() == 0) cut(h0, 0);
             work(h0, [&](int p, int) {
-                if (p % 2 == 0 && p / 2 < R) fetch(a_now, b_now, 1, h1, p / 2);
+                if (p % GAP == 0 && p / GAP < R) fetch(a_now, b_now, 1, h1, p / GAP);
             });
             if constexpr (left() >= 2)
                 asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(LA) : "memory");   // A of stage s + 2 may be on its way
@@ -513,7 +535,7 @@ __global__ void __launch_bounds__(64 * WAVES_M * WAVES_N) k_gemm(GemmArgs g)
                     }
                 }
                 if constexpr (left() >= 1) {
-                    if (p % 2 == 0 && p / 2 < R) fetch(a_next, b_next, 0, h0, p / 2);
+                    if (p % GAP == 0 && p / GAP < R) fetch(a_next, b_next, 0, h0, p / GAP);
                 }
             });
             const int was = b_now;
@@ -636,8 +658,8 @@ __global__ void __launch_bounds__(64 * WAVES_M * WAVES_N) k_gemm(GemmArgs g)
     // products of every wave at a time, so that a wave finishes and stores whole rows: from the accumulators' layout a
     // store touched 32 cache lines, and each residual and derivative as many again.  (A pad of 16 bytes a row puts the 16
     // rows of a write into different banks.)
-    constexpr int E = 16 / T::BYTES, PI = 4, ROWS = WAVES_M * 16 * PI, LD = BN * 4 + 16, LANES = BN / E, STEP = 64 * WAVES / LANES;
-    static_assert(MI % PI == 0 && ROWS * LD <= 3 * A_STAGE + 2 * B_STAGE, "the results' rows fit");
+    constexpr int E = 16 / T::BYTES, LANES = BN / E, STEP = 64 * WAVES / LANES;
+    static_assert(MI % PI == 0, "whole passes");
     const int col = threadIdx.x % LANES * E, row0 = threadIdx.x / LANES;
     const long nn = n0 + col;
     float bias[E];
@@ -678,33 +700,53 @@ __global__ void __launch_bounds__(64 * WAVES_M * WAVES_N) k_gemm(GemmArgs g)
     }
 }
 
-// sums the splits of a row's 16 / BYTES neighbouring results, in order, and finishes them
-template <class T> __global__ void __launch_bounds__(256) k_join(GemmArgs g, int splits)
+// sums the splits of a row's 16 / BYTES neighbouring results and finishes them.  PARTS threads share the splits, each adds
+// its run of them in order, and the first the runs: where there are many splits of few results one thread's loads take long.
+template <class T, int PARTS> __global__ void __launch_bounds__(256) k_join(GemmArgs g, int splits)
 {
-    constexpr int E = 16 / T::BYTES;
-    const long per_row = (g.N + E - 1) / E, id = (long)blockIdx.x * 256 + threadIdx.x;
+    constexpr int E = 16 / T::BYTES, THREADS = 256 / PARTS;
+    const int part = threadIdx.x / THREADS, at = threadIdx.x % THREADS;
+    const long per_row = (g.N + E - 1) / E, id = (long)blockIdx.x * THREADS + at;
     const long m = id / per_row, n = (id - m * per_row) * E;
-    if (m >= g.M) return;
+    const bool in = m < g.M;
     float z[E];
 #pragma unroll
     for (int j = 0; j < E; ++j) z[j] = 0.0f;
-    const int have = g.N - n < E ? (int)(g.N - n) : E;
-    for (int s = 0; s < splits; ++s) {
-        const float *p = g.partial + ((long)s * g.M + m) * g.N + n;
-        if (have == E) {
+    if (in) {
+        const int have = g.N - n < E ? (int)(g.N - n) : E;
+        const int s1 = (int)((long)splits * (part + 1) / PARTS);
+#pragma unroll 4
+        for (int s = (int)((long)splits * part / PARTS); s < s1; ++s) {
+            const float *p = g.partial + ((long)s * g.M + m) * g.N + n;
+            if (have == E) {
 #pragma unroll
-            for (int j = 0; j < E; j += 4) {
-                float w[4];
-                load16<F32>(p + j, w);
+                for (int j = 0; j < E; j += 4) {
+                    float w[4];
+                    load16<F32>(p + j, w);
 #pragma unroll
-                for (int k = 0; k < 4; ++k) z[j + k] += w[k];
+                    for (int k = 0; k < 4; ++k) z[j + k] += w[k];
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < E; ++j)
+                    if (j < have) z[j] += p[j];
             }
-        } else {
-#pragma unroll
-            for (int j = 0; j < E; ++j)
-                if (j < have) z[j] += p[j];
         }
     }
+    if constexpr (PARTS > 1) {
+        __shared__ float runs[PARTS - 1][THREADS][E + 1];
+        if (part > 0) {
+#pragma unroll
+            for (int j = 0; j < E; ++j) runs[part - 1][at][j] = z[j];
+        }
+        __syncthreads();
+        if (part > 0) return;
+        for (int k = 0; k < PARTS - 1; ++k) {
+#pragma unroll
+            for (int j = 0; j < E; ++j) z[j] += runs[k][at][j];
+        }
+    }
+    if (!in) return;
     float bias[E];
     load_bias<T>(g, n, bias);
     epilogue<T>(g, m, n, z, bias);
@@ -789,35 +831,42 @@ constexpr long MOST_K = (1L << 22) - 128;   // 256 padded rows of so many floats
 
 long k_padded(long k, long e) { return (k * e + 127) / 128 * 128 / e; }
 
+enum Shape { SMALL, LARGE, NARROW_N, NARROW_M };   // of a tile: 128 x 128, 256 x 256, 128 x 64, 64 x 128
+
 struct Plan {
-    bool large;
+    Shape shape;
     int tiles_m, tiles_n, steps, per_split, splits;
 };
 
-// Tiles of 256 x 256 or 128 x 128, and how many workgroups share a tile's k: the cheapest by a model of the 256 CUs fitted
-// to measurements (us; 16-bit / f32).  A round of large tiles, one a CU: 19 + 1.4 / 4.6 a stage.  Of small ones: 10 + 0.57 / 1.43
-// a stage alone on a CU, 10 + 0.9 / 2.6 for two together.  Joining splits: 3 + 8 bytes a partial result at 4.5 TB/s.
-// Measured, large against small tiles, best splits of each: bf16 4096 x 4096 x 4096 108 against 135 us, 4096 x 4096 x 1024 44 / 49,
-// 6000 x 3000 x 512 58 / 43, 2048 x 2048 x 2048 41 / 28, 1024 x 1024 x 8192 44 (8 splits) / 34 (4; unsplit 74), 64 x 16384 x 4096
-// 38 (4) / 29 (2; unsplit 40); f32 16384 x 3136 x 512 368 / 302, 16384 x 512 x 3136 289 (2) / 264, 512 x 3136 x 16384 311 (8) / 281 (5;
-// unsplit 741).
+// The tile, and how many workgroups share a tile's k: the cheapest by a model of the 256 CUs fitted to measurements (us; 16-bit /
+// f32).  A round of 256 x 256 tiles, one a CU: 19 + 1.4 / 4.6 a stage.  Of 128 x 128: 10 + 0.5 / 1.43 a stage alone on a CU, 10 +
+// 0.9 / 2.6 for two together; of the narrow ones 0.4 / 0.88 and 0.6 / 1.25.  Joining splits: 3 + 8 bytes a partial result at 4.5 TB/s.
+// Measured, large against small tiles, best splits of each: bf16 4096 x 4096 x 4096 111 against 124 us, 4096 x 4096 x 1024 45 / 49,
+// 6000 x 3000 x 512 61 / 45, 2048 x 2048 x 2048 45 / 28, 1024 x 1024 x 8192 45 (8 splits) / 34 (4; unsplit 60); f32 16384 x 512 x 3136
+// 303 (2) / 274, 512 x 3136 x 16384 319 (8) / 292 (5; unsplit 733).  Small against narrow tiles, at most 64 rows or columns: f32
+// 4020 x 33 x 6985 51 (16) / 36 (16), 16384 x 64 x 2048 54 (4) / 41 (2), 65536 x 64 x 64 20 / 14, 64 x 512 x 16384 26 (64) / 21 (64),
+// 64 x 64 x 65536 33 (256; unsplit 2877) / 28 (128); bf16 4020 x 33 x 6985 48 (16) / 46 (16), 16384 x 18 x 512 15 (2) / 12, 64 x 64 x
+// 65536 18 (64) / 15 (64), 64 x 16384 x 4096 29 (2) / 29 (2).
 Plan plan_of(long M, long N, long K, long e)
 {
     Plan p{};
     p.steps = (int)(k_padded(K, e) * e / 128);
-    const double t_large = e == 2 ? 1.4 : 4.6, t_two = e == 2 ? 0.9 : 2.6, t_one = e == 2 ? 0.57 : 1.43;
     double best = 0.0;
-    for (int large = 0; large < 2; ++large) {
-        const long b = large ? 256 : 128, tm = (M + b - 1) / b, tn = (N + b - 1) / b;
-        for (int splits : {1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 24, 32}) {
+    for (Shape shape : {SMALL, LARGE, NARROW_N, NARROW_M}) {
+        if ((shape == NARROW_N && N > 64) || (shape == NARROW_M && M > 64)) continue;
+        const long bm = shape == LARGE ? 256 : shape == NARROW_M ? 64 : 128, bn = shape == LARGE ? 256 : shape == NARROW_N ? 64 : 128;
+        const long tm = (M + bm - 1) / bm, tn = (N + bn - 1) / bn;
+        const double one = shape == LARGE ? (e == 2 ? 1.4 : 4.6) : shape == SMALL ? (e == 2 ? 0.5 : 1.43) : (e == 2 ? 0.4 : 0.88);
+        const double two = shape == SMALL ? (e == 2 ? 0.9 : 2.6) : (e == 2 ? 0.6 : 1.25);
+        for (int splits : {1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 24, 32, 48, 64, 96, 128, 192, 256}) {
             if (splits > 1 && (p.steps < 4 * splits || (double)splits * M * N > 2.5e8)) break;
             const int per = (p.steps + splits - 1) / splits;
             const long rounds = (tm * tn * splits + 255) / 256;
-            double us = large ? rounds * (19.0 + t_large * per) : rounds / 2 * (10.0 + t_two * per) + rounds % 2 * (10.0 + t_one * per);
+            double us = shape == LARGE ? rounds * (19.0 + one * per) : rounds / 2 * (10.0 + two * per) + rounds % 2 * (10.0 + one * per);
             if (splits > 1) us += 3.0 + (double)splits * M * N * 8.0 / 4.5e6;
             if (best != 0.0 && us >= best) continue;
             best = us;
-            p.large = large;
+            p.shape = shape;
             p.tiles_m = (int)tm;
             p.tiles_n = (int)tn;
             p.per_split = per;
@@ -870,15 +919,20 @@ template <class T, bool KA, bool KB> int gemm(GemmArgs g, long K, const Plan &p,
     g.tiles_n = p.tiles_n;
     if (p.splits == 1) g.partial = nullptr;
     const dim3 grid((unsigned)(p.tiles_m * p.tiles_n), (unsigned)p.splits);
-    if (p.large)
-        hipLaunchKernelGGL((k_gemm<T, 256, 256, 2, 4, KA, KB>), grid, dim3(512), 0, s, g);
-    else
-        hipLaunchKernelGGL((k_gemm<T, 128, 128, 2, 2, KA, KB>), grid, dim3(256), 0, s, g);
+    switch (p.shape) {
+    case LARGE: hipLaunchKernelGGL((k_gemm<T, 256, 256, 2, 4, KA, KB>), grid, dim3(512), 0, s, g); break;
+    case SMALL: hipLaunchKernelGGL((k_gemm<T, 128, 128, 2, 2, KA, KB>), grid, dim3(256), 0, s, g); break;
+    case NARROW_N: hipLaunchKernelGGL((k_gemm<T, 128, 64, 4, 1, KA, KB>), grid, dim3(256), 0, s, g); break;
+    case NARROW_M: hipLaunchKernelGGL((k_gemm<T, 64, 128, 2, 2, KA, KB>), grid, dim3(256), 0, s, g); break;
+    }
     int rc = ppo_launch_status();
     if (rc || p.splits == 1) return rc;
     constexpr long E = 16 / T::BYTES;
     const long threads = g.M * ((g.N + E - 1) / E);
-    hipLaunchKernelGGL(k_join<T>, dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, s, g, p.splits);
+    if (p.splits >= 16)
+        hipLaunchKernelGGL((k_join<T, 8>), dim3((unsigned)((threads + 31) / 32)), dim3(256), 0, s, g, p.splits);
+    else
+        hipLaunchKernelGGL((k_join<T, 1>), dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, s, g, p.splits);
     return ppo_launch_status();
 }
 

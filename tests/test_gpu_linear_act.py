@@ -93,6 +93,14 @@ def test_large_tiles(M, K, N, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("M,K,N", [(20000, 64, 40), (20001, 63, 64), (9001, 18, 65), (64, 8001, 128), (50, 130, 9000), (35, 4999, 64), (66, 6000, 3),
+                                   (70000, 33, 18)])
+def test_narrow_sizes(M, K, N, dtype):
+    """At most 64 of one dimension and, in one of the three products, many of k: tiles of their own and up to hundreds of sums a result."""
+    _check(*_make(M + K + N, M, K, N, dtype), "tanh")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("rows", [4, 5, 10, 11, 12, 13, 32, 33])
 def test_few_rows_of_large_weights(rows, dtype):
     """Both sides of each border between the vector units and the matrix cores, weights in place and not (4.2 and 8.4 MB)."""
