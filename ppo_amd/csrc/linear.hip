@@ -903,7 +903,7 @@ template <class T> struct Prep {
     int launch(hipStream_t s)
     {
         if (count == 0) return 0;
-        PPO_REQUIRE(tiles < (1L << 31));
+        PPO_REQUIRE(tiles < (1L << 24));     // fewer than 2^32 threads a launch
         for (int j = count; j < 3; ++j) jobs.first[j + 1] = (unsigned)tiles;
         hipLaunchKernelGGL(k_prep<T>, dim3((unsigned)tiles), dim3(256), 0, s, jobs);
         return ppo_launch_status();

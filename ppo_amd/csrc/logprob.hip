@@ -77,7 +77,7 @@ template <int G> __device__ __forceinline__ Row row_lanes(Row r, float c)
 struct FwdArgs {
     const void *logits, *actions;
     float *logp, *entropy, *stats;
-    long rows, length, A, batch_stride, token_stride, ignore;
+    long rows, length, A, batch_stride, token_stride, ignore, first;   // first: row of this launch
     float c, inv_t;
     int action_bytes;
 };
@@ -125,7 +125,7 @@ template <class T> __device__ __forceinline__ void write_row(const FwdArgs &a, l
 // add, where joining running sums would take two exponentials a step
 template <class T, int G> __global__ void __launch_bounds__(256) k_logprobs_short(FwdArgs a)
 {
-    const long row = (long)blockIdx.x * (256 / G) + threadIdx.x / G;
+    const long row = a.first + (long)blockIdx.x * (256 / G) + threadIdx.x / G;
     const int l = threadIdx.x % G, A = (int)a.A;
     if (row >= a.rows) return;
     const typename T::raw *x = reinterpret_cast<const typename T::raw *>(a.logits) + row_offset(row, a.rows, a.length, a.batch_stride, a.token_stride);
@@ -160,7 +160,7 @@ template <class T, int G> __global__ void __launch_bounds__(256) k_logprobs_shor
 template <class T, int THREADS> __global__ void __launch_bounds__(THREADS < 256 ? 256 : THREADS) k_logprobs_long(FwdArgs a)
 {
     constexpr int E = 16 / T::BYTES, CHUNK = 32, U = CHUNK / E;
-    const long row = THREADS == 64 ? (long)blockIdx.x * 4 + threadIdx.x / 64 : (long)blockIdx.x;
+    const long row = a.first + (THREADS == 64 ? (long)blockIdx.x * 4 + threadIdx.x / 64 : (long)blockIdx.x);
     const int tid = THREADS == 64 ? threadIdx.x % 64 : threadIdx.x;
     if (row >= a.rows) return;
     const long act = action_of(a.actions, a.action_bytes, row);
@@ -210,7 +210,7 @@ struct BwdArgs {
     const void *logits, *actions;
     const float *stats, *entropy, *g_logp, *g_entropy;
     void *g;
-    long rows, length, A, batch_stride, token_stride, ignore;
+    long rows, length, A, batch_stride, token_stride, ignore, first;   // first: row of this launch
     float c, inv_t;
     int action_bytes;
 };
@@ -248,7 +248,7 @@ __device__ __forceinline__ float grad_at(const Grad &g, float x, float c)
 
 template <class T, int G> __global__ void __launch_bounds__(256) k_logprobs_bwd_short(BwdArgs a)
 {
-    const long row = (long)blockIdx.x * (256 / G) + threadIdx.x / G;
+    const long row = a.first + (long)blockIdx.x * (256 / G) + threadIdx.x / G;
     const int l = threadIdx.x % G, A = (int)a.A;
     if (row >= a.rows) return;
     const typename T::raw *x = reinterpret_cast<const typename T::raw *>(a.logits) + row_offset(row, a.rows, a.length, a.batch_stride, a.token_stride);
@@ -270,7 +270,7 @@ template <class T, int G> __global__ void __launch_bounds__(256) k_logprobs_bwd_
 template <class T> __global__ void __launch_bounds__(256) k_logprobs_bwd_long(BwdArgs a, int chunks)
 {
     constexpr int E = 16 / T::BYTES, CHUNK = 32, U = CHUNK / E;
-    const long row = blockIdx.x / chunks;
+    const long row = a.first + blockIdx.x / chunks;
     const long at = (long)(blockIdx.x % chunks) * (256 * CHUNK);
     const Grad g = grad_of(a, row);
     const typename T::raw *x = reinterpret_cast<const typename T::raw *>(a.logits) + row_offset(row, a.rows, a.length, a.batch_stride, a.token_stride);
@@ -325,6 +325,20 @@ template <class Args> void even_rows(Args &a, long batch)
     if (batch == 1 || a.batch_stride == a.length * a.token_stride) a.length = a.rows;
 }
 
+// A launch has fewer than 2^32 threads: so many rows (of `threads` each, rounded up to whole workgroups) at a time.
+template <class Args, class Kernel, class... More>
+int launch_rows(Kernel kernel, Args a, long threads, int block, hipStream_t s, More... more)
+{
+    const long fit = (1L << 31) / threads, most = fit >= 32 ? fit / 32 * 32 : fit;   // (whole workgroups)
+    for (a.first = 0; a.first < a.rows; a.first += most) {
+        const long rows = a.rows - a.first < most ? a.rows - a.first : most;
+        hipLaunchKernelGGL(kernel, dim3((unsigned)((rows * threads + block - 1) / block)), dim3(block), 0, s, a, more...);
+        const int rc = ppo_launch_status();
+        if (rc) return rc;
+    }
+    return 0;
+}
+
 }  // namespace
 
 extern "C" {
@@ -346,18 +360,11 @@ int ppo_token_logprobs_fwd(const void *logits, int dtype, long batch, long lengt
     hipStream_t s = (hipStream_t)stream;
     return by_dtype(dtype, [&](auto t) {
         using T = decltype(t);
-        const unsigned rows = (unsigned)a.rows;
-        if (a.A <= 32)
-            hipLaunchKernelGGL((k_logprobs_short<T, 8>), dim3((rows + 31) / 32), dim3(256), 0, s, a);
-        else if (a.A <= 256)
-            hipLaunchKernelGGL((k_logprobs_short<T, 64>), dim3((rows + 3) / 4), dim3(256), 0, s, a);
-        else if (a.A <= 4096)
-            hipLaunchKernelGGL((k_logprobs_long<T, 64>), dim3((rows + 3) / 4), dim3(256), 0, s, a);
-        else if (a.rows >= 1024)
-            hipLaunchKernelGGL((k_logprobs_long<T, 256>), dim3(rows), dim3(256), 0, s, a);
-        else
-            hipLaunchKernelGGL((k_logprobs_long<T, 1024>), dim3(rows), dim3(1024), 0, s, a);
-        return ppo_launch_status();
+        if (a.A <= 32) return launch_rows(k_logprobs_short<T, 8>, a, 8, 256, s);
+        if (a.A <= 256) return launch_rows(k_logprobs_short<T, 64>, a, 64, 256, s);
+        if (a.A <= 4096) return launch_rows(k_logprobs_long<T, 64>, a, 64, 256, s);
+        if (a.rows >= 1024) return launch_rows(k_logprobs_long<T, 256>, a, 256, 256, s);
+        return launch_rows(k_logprobs_long<T, 1024>, a, 1024, 1024, s);
     });
 }
 
@@ -379,18 +386,13 @@ int ppo_token_logprobs_bwd(const void *logits, int dtype, long batch, long lengt
     a.c = (float)(1.4426950408889634 / temperature);
     even_rows(a, batch);
     const long chunks = (a.A + 256 * 32 - 1) / (256 * 32);
-    PPO_REQUIRE(a.A <= 1024 || chunks <= ((1L << 31) - 1) / a.rows);
+    PPO_REQUIRE(a.A <= 1024 || chunks < (1L << 23));   // a row's gradient is one launch at least
     hipStream_t s = (hipStream_t)stream;
     return by_dtype(dtype, [&](auto t) {
         using T = decltype(t);
-        const unsigned rows = (unsigned)a.rows;
-        if (a.A <= 32)
-            hipLaunchKernelGGL((k_logprobs_bwd_short<T, 8>), dim3((rows + 31) / 32), dim3(256), 0, s, a);
-        else if (a.A <= 1024)
-            hipLaunchKernelGGL((k_logprobs_bwd_short<T, 64>), dim3((rows + 3) / 4), dim3(256), 0, s, a);
-        else
-            hipLaunchKernelGGL((k_logprobs_bwd_long<T>), dim3((unsigned)(a.rows * chunks)), dim3(256), 0, s, a, (int)chunks);
-        return ppo_launch_status();
+        if (a.A <= 32) return launch_rows(k_logprobs_bwd_short<T, 8>, a, 8, 256, s);
+        if (a.A <= 1024) return launch_rows(k_logprobs_bwd_short<T, 64>, a, 64, 256, s);
+        return launch_rows(k_logprobs_bwd_long<T>, a, chunks * 256, 256, s, (int)chunks);
     });
 }
 

@@ -195,7 +195,7 @@ __device__ __forceinline__ void policy_groups(const PolicyArgs &a, const int *ro
                         dk = e - k;                    // 1 - e^-e
                     }
                     s_kl += k;
-                    dl = __builtin_fmaf(a.kl_coef_f, dk, dl);
+                    if (a.kl_coef_f != 0.0f) dl = __builtin_fmaf(a.kl_coef_f, dk, dl);   // (only reported: an infinite one is no 0 * inf)
                 }
                 g[i] = gw * dl;
             }
@@ -219,7 +219,7 @@ __device__ __forceinline__ void policy_out(const PolicyArgs &a, const double (&s
 {
     const double whole = a.sequence_mean ? (rows > 0 ? 1.0 / rows : 1.0) : (tokens > 0 ? 1.0 / tokens : 1.0);
     const double pg = s[0] * whole, kl = s[1] * whole;
-    a.out6[0] = (float)(a.ref_lp ? pg + a.kl_coef * kl : pg);
+    a.out6[0] = (float)(a.ref_lp && a.kl_coef != 0.0 ? pg + a.kl_coef * kl : pg);
     a.out6[1] = (float)pg;
     a.out6[2] = (float)kl;
     a.out6[3] = (float)(s[2] * whole);
@@ -419,7 +419,8 @@ __device__ __forceinline__ double pair_loss(const PrefArgs &a, const Margin &m)
     if (a.kind == PPO_PREF_SIGMOID) {
         const double sp = log1p_unit(exp_minus(fabs(m.z)));           // softplus(-|z|)
         const double loss_pos = (m.z < 0.0 ? -m.z : 0.0) + sp, loss_neg = (m.z > 0.0 ? m.z : 0.0) + sp;   // -ln s(z), -ln s(-z)
-        return m.z != m.z ? m.z : (1.0 - a.smoothing) * loss_pos + a.smoothing * loss_neg;
+        const double smooth = a.smoothing > 0.0 ? a.smoothing * loss_neg : 0.0;   // (z = inf: 0, not 0 * inf)
+        return m.z != m.z ? m.z : (1.0 - a.smoothing) * loss_pos + smooth;
     }
     if (a.kind == PPO_PREF_HINGE) return m.z < 1.0 ? 1.0 - m.z : (m.z != m.z ? m.z : 0.0);
     const double off = m.delta - 0.5 / a.beta;
@@ -480,22 +481,23 @@ __device__ __forceinline__ void pref_out(const PrefArgs &a, double loss, double 
 __global__ void __launch_bounds__(SEQ_BLOCK) k_pref_pair(PrefArgs a)
 {
     __shared__ double part[SEQ_BLOCK / 64][4];
-    const long b = blockIdx.x;
-    double v[4], acc[2];
-    pref_sum<SEQ_BLOCK>(a.side[0], b, 0, a.side[0].L, threadIdx.x, acc);
-    v[0] = acc[0]; v[1] = acc[1];
-    pref_sum<SEQ_BLOCK>(a.side[1], b, 0, a.side[1].L, threadIdx.x, acc);
-    v[2] = acc[0]; v[3] = acc[1];
-    const Ahead ahead[2] = {pref_ahead<SEQ_BLOCK>(a.side[0], b, 0, a.side[0].L, threadIdx.x), pref_ahead<SEQ_BLOCK>(a.side[1], b, 0, a.side[1].L, threadIdx.x)};
-    block_sum<4, SEQ_BLOCK>(v, part);
-    const double sum[2] = {v[0], v[2]}, count[2] = {v[1], v[3]};
-    const Margin m = margin_of(a, sum, count);
+    for (long b = blockIdx.x; b < a.B; b += gridDim.x) {
+        double v[4], acc[2];
+        pref_sum<SEQ_BLOCK>(a.side[0], b, 0, a.side[0].L, threadIdx.x, acc);
+        v[0] = acc[0]; v[1] = acc[1];
+        pref_sum<SEQ_BLOCK>(a.side[1], b, 0, a.side[1].L, threadIdx.x, acc);
+        v[2] = acc[0]; v[3] = acc[1];
+        const Ahead ahead[2] = {pref_ahead<SEQ_BLOCK>(a.side[0], b, 0, a.side[0].L, threadIdx.x), pref_ahead<SEQ_BLOCK>(a.side[1], b, 0, a.side[1].L, threadIdx.x)};
+        block_sum<4, SEQ_BLOCK>(v, part);
+        const double sum[2] = {v[0], v[2]}, count[2] = {v[1], v[3]};
+        const Margin m = margin_of(a, sum, count);
 #pragma unroll
-    for (int k = 0; k < 2; ++k) pref_write<SEQ_BLOCK>(a.side[k], b, 0, a.side[k].L, threadIdx.x, ahead[k], pair_grad(a, m, k));
-    if (threadIdx.x == 0) {
-        pref_rewards(a, b, m);
-        a.pair[2 * b] = pair_loss(a, m);
-        a.pair[2 * b + 1] = m.z > 0.0 ? 1.0 : 0.0;
+        for (int k = 0; k < 2; ++k) pref_write<SEQ_BLOCK>(a.side[k], b, 0, a.side[k].L, threadIdx.x, ahead[k], pair_grad(a, m, k));
+        if (threadIdx.x == 0) {
+            pref_rewards(a, b, m);
+            a.pair[2 * b] = pair_loss(a, m);
+            a.pair[2 * b + 1] = m.z > 0.0 ? 1.0 : 0.0;
+        }
     }
 }
 
@@ -724,7 +726,7 @@ int ppo_preference_loss(const float *chosen, long chosen_stride, const float *re
         return ppo_launch_status();
     }
     if (chunks == 1) {
-        hipLaunchKernelGGL(k_pref_pair, dim3((unsigned)pairs), dim3(SEQ_BLOCK), 0, s, a);
+        hipLaunchKernelGGL(k_pref_pair, dim3((unsigned)(pairs < (1L << 20) ? pairs : 1L << 20)), dim3(SEQ_BLOCK), 0, s, a);
         const int rc = ppo_launch_status();
         if (rc) return rc;
         hipLaunchKernelGGL(k_pref_final, dim3(1), dim3(SEQ_BLOCK), 0, s, a);

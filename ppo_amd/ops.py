@@ -732,7 +732,7 @@ def _token_rows(name, logits, actions, temperature):
         _refuse(f"{name}: temperature {temperature} outside [1e-6, 1e6]")
     _device_tensors(name, logits, actions)
     if logits.dim() > 3:
-        logits = logits.reshape(-1, *logits.shape[-2:])
+        logits = logits.flatten(0, -3)
     strides = logits.stride()
     if strides[-1] != 1 and logits.shape[-1] > 1:
         logits = logits.contiguous()

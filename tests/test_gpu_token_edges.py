@@ -1,0 +1,90 @@
+"""GPU: token_logprobs, policy_kl_loss and preference_loss where a call needs more than one launch, and with infinite log-probs.
+
+Row counts: a launch of the head's kernels holds 2^31 threads, i.e. 2^28, 2^25 and 2^23 rows at 8, 64 and 256 threads each.
+Tolerances are those of test_gpu_token_losses.py."""
+import math
+
+import pytest
+import torch
+
+import token_reference as ref
+
+pytestmark = pytest.mark.gpu
+E = 2.0 ** -24
+
+
+@pytest.mark.parametrize("rows,A", [(2 ** 28 + 37, 2), (2 ** 25 + 5, 40), (2 ** 23 + 3, 1030)])
+def test_logprobs_rows_of_more_than_one_launch(rows, A):
+    from ppo_amd import ops
+    logits = torch.empty(rows, A, device="cuda", dtype=torch.bfloat16).normal_(generator=torch.Generator("cuda").manual_seed(A))
+    actions = torch.randint(0, A, (rows,), device="cuda", dtype=torch.int32, generator=torch.Generator("cuda").manual_seed(rows))
+    logp, H, stats = ops.token_logprobs_fwd(logits, actions)
+    ones = torch.ones(1, device="cuda").expand(rows).contiguous()
+    g = ops.token_logprobs_bwd(logits, actions, stats, None, ones)
+    assert bool(torch.isfinite(logp).all()) and bool((logp < 0).all()) and bool((H > 0).all())
+    most = 2 ** 31 // (8 if A <= 32 else 64 if A <= 1024 else 256)
+    for at in (slice(0, 200), slice(most - 100, most + 3), slice(rows - 64, rows)):
+        lp, h = ref.logprobs(logits[at], actions[at])
+        assert bool(((logp[at].double() - lp).abs() <= 90 * E + 4 * E * lp.abs()).all())
+        assert bool(((H[at].double() - h).abs() <= 180 * E * (1 + math.log(A))).all())
+        want, size = ref.logprobs_grad(logits[at], actions[at], ones[at], None)
+        tol = 2.0 ** -8 * want.abs() + (100 + 40 * (1 + math.log(A))) * E * size * 2 + 2.0 ** -126
+        assert bool(((g[at].double() - want).abs() <= tol).all())
+
+
+def test_preference_pairs_of_more_than_one_round():
+    from ppo_amd import ops
+    pairs = 2 ** 20 + 7
+    gen = torch.Generator("cuda").manual_seed(3)
+    c, r = (-torch.rand(pairs, n, device="cuda", generator=gen) for n in (3, 2))
+    out, rewards, gc, gr = ops.preference_loss_fwd_bwd(c, r, beta=0.3)
+    x, y = c.double().requires_grad_(True), r.double().requires_grad_(True)
+    loss, acc, want = ref.preference(x, y, beta=0.3)
+    wc, wr = torch.autograd.grad(loss, (x, y))
+    loss = loss.detach()
+    assert abs(float(out[0]) - float(loss)) <= 2 * E * float(loss) and abs(float(out[1]) - float(acc)) <= 2 * E
+    assert bool(((rewards.double() - want).abs() <= 2 * E * want.abs() + 1e-12).all())
+    for got, w in ((gc, wc), (gr, wr)):
+        assert bool(((got.double() - w).abs() <= 2 * E * w.abs()).all())
+
+
+@pytest.mark.parametrize("shape", [(1, 4), (300, 4), (2, 20000)])
+def test_preference_of_an_impossible_rejected_answer(shape):
+    """A rejected token of log-prob -inf: the margin is infinite, -ln s of it 0 and so is the gradient; the other way round inf."""
+    from ppo_amd import ops
+    c, r = torch.full(shape, -0.5, device="cuda"), torch.full(shape, -0.5, device="cuda")
+    r[:, 1] = -math.inf
+    out, _, gc, gr = ops.preference_loss_fwd_bwd(c, r)
+    assert float(out[0]) == 0.0 and float(out[1]) == 1.0 and float(gc.abs().max()) == 0.0 and float(gr.abs().max()) == 0.0
+    out, _, gc, gr = ops.preference_loss_fwd_bwd(c, r, kind="hinge")
+    assert float(out[0]) == 0.0 and float(gc.abs().max()) == 0.0
+    out, _, gc, gr = ops.preference_loss_fwd_bwd(r, c)
+    pairs = shape[0]
+    assert float(out[0]) == math.inf and float(out[1]) == 0.0
+    assert bool(((gc + 0.1 / pairs).abs() <= 2 * E * 0.1 / pairs).all()) and torch.equal(gr, -gc)
+
+
+@pytest.mark.parametrize("kl", ["k1", "k2", "k3"])
+@pytest.mark.parametrize("B,L", [(2, 9), (300, 70)])
+def test_policy_loss_with_a_reported_kl_only(B, L, kl):
+    """kl_coef 0: an infinite estimate is reported and changes neither the loss nor its gradient."""
+    from ppo_amd import ops
+    gen = torch.Generator("cuda").manual_seed(B)
+    new = -torch.rand(B, L, device="cuda", generator=gen)
+    adv = torch.randn(B, L, device="cuda", generator=gen)
+    old, refp = new - 0.1, new.clone()
+    refp[1, 3] = -math.inf
+    plain, g0 = ops.policy_kl_loss_fwd_bwd(new, old, adv)
+    out, g = ops.policy_kl_loss_fwd_bwd(new, old, adv, ref_lp=refp, kl=kl)
+    assert torch.equal(out[:2], plain[:2]) and torch.equal(out[3:], plain[3:]) and torch.equal(g, g0)
+    assert float(out[2]) == math.inf
+
+
+def test_logits_of_four_axes_and_no_tokens():
+    from ppo_amd import ops
+    for shape in ((2, 3, 0), (0, 3, 4), (2, 0, 4)):
+        logits = torch.zeros(*shape, 7, device="cuda", requires_grad=True)
+        logp, H = ops.token_logprobs(logits, torch.zeros(shape, dtype=torch.int64, device="cuda"))
+        assert logp.shape == H.shape == shape
+        (g,) = torch.autograd.grad(logp.sum() + H.sum(), logits)
+        assert g.shape == logits.shape
