@@ -360,7 +360,13 @@ int ppo_token_logprobs_fwd(const void *logits, int dtype, long batch, long lengt
     hipStream_t s = (hipStream_t)stream;
     return by_dtype(dtype, [&](auto t) {
         using T = decltype(t);
+        // the fewest lanes that hold a row in four registers each (262144 rows: 18 actions 11 us with 8 lanes, 17 with 16; 64
+        // actions 19 with 16, 34 with 32; 128 actions 37 with 32, 67 with 64); above 256 actions a wave each (65536 x 256: 20 us
+        // with 64 lanes in registers, 26 so), above 4096 a workgroup of 256, or of 1024 where rows are few (bf16, a wave / 256 /
+        // 1024 threads: 8192 x 4096 15 / 20 / 47, 1024 x 65536 32 / 25 / 27, 64 x 65536 24 / 11 / 11)
         if (a.A <= 32) return launch_rows(k_logprobs_short<T, 8>, a, 8, 256, s);
+        if (a.A <= 64) return launch_rows(k_logprobs_short<T, 16>, a, 16, 256, s);
+        if (a.A <= 128) return launch_rows(k_logprobs_short<T, 32>, a, 32, 256, s);
         if (a.A <= 256) return launch_rows(k_logprobs_short<T, 64>, a, 64, 256, s);
         if (a.A <= 4096) return launch_rows(k_logprobs_long<T, 64>, a, 64, 256, s);
         if (a.rows >= 1024) return launch_rows(k_logprobs_long<T, 256>, a, 256, 256, s);
@@ -386,12 +392,17 @@ int ppo_token_logprobs_bwd(const void *logits, int dtype, long batch, long lengt
     a.c = (float)(1.4426950408889634 / temperature);
     even_rows(a, batch);
     const long chunks = (a.A + 256 * 32 - 1) / (256 * 32);
-    PPO_REQUIRE(a.A <= 1024 || chunks < (1L << 23));   // a row's gradient is one launch at least
+    const bool chunked = a.A * dtype_bytes(dtype) > 8192;
+    PPO_REQUIRE(!chunked || chunks < (1L << 23));      // a row's gradient is one launch at least
     hipStream_t s = (hipStream_t)stream;
     return by_dtype(dtype, [&](auto t) {
         using T = decltype(t);
-        if (a.A <= 32) return launch_rows(k_logprobs_bwd_short<T, 8>, a, 8, 256, s);
-        if (a.A <= 1024) return launch_rows(k_logprobs_bwd_short<T, 64>, a, 64, 256, s);
+        // lanes a row, us with 8 / 16 / 64: f32 262144 x 64 23 / 24 / 46, x 128 57 / 51 / 63, 65536 x 300 36 / 29 / 29, x 500 87 / 60 /
+        // 45; bf16 262144 x 64 21 / 21 / 45, x 128 35 / 31 / 51.  Rows of 8 KB, a wave against workgroups: f32 16384 x 2048 45 / 63 and
+        // 8192 x 4096 52 / 43, bf16 8192 x 4096 27 / 30
+        if (a.A <= 64) return launch_rows(k_logprobs_bwd_short<T, 8>, a, 8, 256, s);
+        if (a.A <= 320) return launch_rows(k_logprobs_bwd_short<T, 16>, a, 16, 256, s);
+        if (!chunked) return launch_rows(k_logprobs_bwd_short<T, 64>, a, 64, 256, s);
         return launch_rows(k_logprobs_bwd_long<T>, a, chunks * 256, 256, s, (int)chunks);
     });
 }

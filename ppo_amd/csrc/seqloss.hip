@@ -109,7 +109,8 @@ __global__ void __launch_bounds__(SEQ_BLOCK) k_policy_count(PolicyArgs a)
 {
     __shared__ double part[SEQ_BLOCK / 64][2];
     double tot[2];
-    // a wave a row, eight rows a wave where they are short
+    // a wave a row, eight rows a wave where they are short (70000 x 128, the whole call: 40 us, 51 with a wave a row; as fast
+    // as that for 4096 rows of any length)
     if (a.L > 256)
         count_rows<64>(a, a.row_counts, (long)blockIdx.x * (SEQ_BLOCK / 64), (long)gridDim.x * (SEQ_BLOCK / 64), tot);
     else
@@ -271,14 +272,17 @@ __global__ void __launch_bounds__(FINAL_BLOCK) k_policy_final(PolicyArgs a, int 
 }
 
 // everything in one workgroup: a few thousand tokens, where launches are what costs
-constexpr int ONE_BLOCK = 512, ONE_ROWS = 256, ONE_GROUPS = 4096;
+constexpr int ONE_BLOCK = 512, ONE_ROWS = 256, ONE_GROUPS = 2048;
 __global__ void __launch_bounds__(ONE_BLOCK) k_policy_one(PolicyArgs a)
 {
     __shared__ double part2[ONE_BLOCK / 64][2];
     __shared__ double part[ONE_BLOCK / 64][NSUM];
     __shared__ int row_counts[ONE_ROWS];
     double tot[2], acc[NSUM] = {0.0, 0.0, 0.0, 0.0};
-    count_rows<64>(a, row_counts, 0, ONE_BLOCK / 64, tot);
+    if (a.L > 256)
+        count_rows<64>(a, row_counts, 0, ONE_BLOCK / 64, tot);
+    else
+        count_rows<8>(a, row_counts, 0, ONE_BLOCK / 8, tot);
     block_sum<2, ONE_BLOCK>(tot, part2);           // (its barriers are the row counts' too)
     policy_groups(a, row_counts, tot[0], tot[1], threadIdx.x, ONE_BLOCK, acc);
     block_sum<NSUM, ONE_BLOCK>(acc, part);
@@ -550,7 +554,10 @@ template <int LANES> __device__ __forceinline__ Margin margin_of_chunks(const Pr
         v[3] += p[2 * a.chunks + 1];
     }
 #pragma unroll
-    for (int k = 0; k < 4; ++k) v[k] = wave_sum(v[k]);
+    for (int off = LANES / 2; off > 0; off >>= 1) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] += __shfl_xor(v[k], off, 64);
+    }
     const double sum[2] = {v[0], v[2]}, count[2] = {v[1], v[3]};
     return margin_of(a, sum, count);
 }
@@ -558,13 +565,14 @@ template <int LANES> __device__ __forceinline__ Margin margin_of_chunks(const Pr
 // the last workgroup makes the mean over the pairs, the others write the gradients of their chunks
 __global__ void __launch_bounds__(SEQ_BLOCK) k_pref_grad(PrefArgs a)
 {
-    const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63;
     if (blockIdx.x == 2 * a.B * a.chunks) {
         __shared__ double part[SEQ_BLOCK / 64][2];
         double acc[2] = {0.0, 0.0};
-        for (long b = wid; b < a.B; b += SEQ_BLOCK / 64) {
-            const Margin m = margin_of_chunks<64>(a, b, lane);
-            if (lane == 0) {
+        const int lanes = a.chunks <= 8 ? 8 : 64;          // a pair (up to 256 pairs have two chunks: 32 of them at once)
+        for (long b = threadIdx.x / lanes; b < a.B; b += SEQ_BLOCK / lanes) {
+            const Margin m = lanes == 8 ? margin_of_chunks<8>(a, b, threadIdx.x % 8) : margin_of_chunks<64>(a, b, lane);
+            if (threadIdx.x % lanes == 0) {
                 acc[0] += pair_loss(a, m);
                 acc[1] += m.z > 0.0 ? 1.0 : 0.0;
                 pref_rewards(a, b, m);
@@ -612,14 +620,22 @@ __global__ void __launch_bounds__(ONE_BLOCK) k_pref_one(PrefArgs a)
     if (threadIdx.x == 0) pref_out(a, tot[0], tot[1]);
 }
 
-bool one_workgroup(long batch, long length) { return batch <= ONE_ROWS && batch * ((length + 3) / 4) <= ONE_GROUPS; }
+// One launch instead of three: 8192 tokens, four turns of a thread.  Measured, us, against three: 8 x 1024 11.9 / 18.8, 128 x 64
+// 11.9 / 19.4; 16384 tokens: 16 x 1024 19.5 / 19.5, 64 x 256 18.9 / 18.6, 256 x 64 19.9 / 19.0.
+bool one_workgroup(long batch, long length)
+{
+    return batch <= ONE_ROWS && batch * ((length + 3) / 4) <= ONE_GROUPS;
+}
 
-// workgroups a row is cut into: 0 = one for everything, 1 = one a pair, otherwise about 512 in all, of 2048 tokens at least
+// Workgroups a row is cut into: 0 = one for everything, where that is at most ten turns of a wave (measured, us, against a
+// workgroup a pair: 4 pairs of 2 x 1000 15 / 20, 16 of 2 x 512 15 / 19; 16 turns: 32 of 2 x 512 23 / 19, 64 of 2 x 128 31 / 19).
+// 1 = one a pair, up to 8192 tokens or where there are 256 pairs (against chunks: 64 of 2 x 8192 20 / 26, 16 of 2 x 8192 20 / 20;
+// 1 of 2 x 16384 31 / 19).  Otherwise about 512 in all, of 2048 tokens at least.
 int pref_chunks(long B, long Lc, long Lr)
 {
-    if (B <= 64 && B * (Lc + Lr) <= 32768) return 0;
     const long L = Lc > Lr ? Lc : Lr;
-    if (B >= 256 || L <= 4096) return 1;
+    if ((B + ONE_BLOCK / 64 - 1) / (ONE_BLOCK / 64) * ((Lc + 255) / 256 + (Lr + 255) / 256) <= 10) return 0;
+    if (B >= 256 || L <= 8192) return 1;
     long c = (512 + 2 * B - 1) / (2 * B);
     const long most = (L + 2047) / 2048;
     if (c > most) c = most;
