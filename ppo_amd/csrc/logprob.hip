@@ -6,7 +6,8 @@
 //     log p_a = z_a - top - ln s          H = -sum p ln p = ln s - u / s
 //     d log p_a / d z_k = [k = a] - p_k   d H / d z_k = -p_k (ln p_k + H)
 // One pass over the logits forward (running maximum; s and u are rescaled when it moves), one pass backward that reads
-// the logits again and writes their gradient.  Both are bound by HBM.  What is kept per row for the backward pass is the
+// the logits again and writes their gradient.  Both are bound by HBM: 8192 rows of 131072 f16 logits take 397 us forward (5.4
+// TB/s) and 735 us backward (5.8 TB/s); a large copy runs at 4.7 TB/s, a sum over a large array at 4.0.  What is kept per row for the backward pass is the
 // PAIR {max logit, ln s}: their sum, the usual log-sum-exp, loses ln s in rows of large magnitude (a row of the type's
 // lowest value is a uniform one), and (logit - max) is exact where the two are near.
 // All sums are f32 over chunks of at most 32 elements, then over the lanes' chunks, then over lanes: 131072 terms are
@@ -121,29 +122,31 @@ template <class T> __device__ __forceinline__ void write_row(const FwdArgs &a, l
     a.stats[2 * row + 1] = lns;
 }
 
-// G lanes a row, at most four elements a lane, all in registers: the lanes find the row's maximum first and then only
+// G lanes a row, at most N elements a lane, all in registers: the lanes find the row's maximum first and then only
 // add, where joining running sums would take two exponentials a step
-template <class T, int G> __global__ void __launch_bounds__(256) k_logprobs_short(FwdArgs a)
+template <class T, int G, int N> __global__ void __launch_bounds__(256) k_logprobs_short(FwdArgs a)
 {
     const long row = a.first + (long)blockIdx.x * (256 / G) + threadIdx.x / G;
     const int l = threadIdx.x % G, A = (int)a.A;
     if (row >= a.rows) return;
     const typename T::raw *x = reinterpret_cast<const typename T::raw *>(a.logits) + row_offset(row, a.rows, a.length, a.batch_stride, a.token_stride);
-    float v[4];                                        // (on their way while the action, which may be the ignored one, is)
+    float v[N];                                        // (on their way while the action, which may be the ignored one, is)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = l + i * G < A ? T::load(x[l + i * G]) : -INFINITY;
+    for (int i = 0; i < N; ++i) v[i] = l + i * G < A ? T::load(x[l + i * G]) : -INFINITY;
     const long act = action_of(a.actions, a.action_bytes, row);
     if (act == a.ignore) {
         if (l == 0) write_ignored(a, row);
         return;
     }
-    float m = fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3]));
+    float m = v[0];
+#pragma unroll
+    for (int i = 1; i < N; ++i) m = fmaxf(m, v[i]);
 #pragma unroll
     for (int off = G / 2; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor(m, off, 64));
     const float base = m == -INFINITY ? 0.0f : m;
     Row r = {m, 0.0f, 0.0f};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < N; ++i) {
         const float t = (v[i] - base) * a.c, e = __builtin_amdgcn_exp2f(t);
         r.s += e;
         r.u = __builtin_fmaf(e, fmaxf(t, LOWEST), r.u);
@@ -360,14 +363,16 @@ int ppo_token_logprobs_fwd(const void *logits, int dtype, long batch, long lengt
     hipStream_t s = (hipStream_t)stream;
     return by_dtype(dtype, [&](auto t) {
         using T = decltype(t);
-        // the fewest lanes that hold a row in four registers each (262144 rows: 18 actions 11 us with 8 lanes, 17 with 16; 64
-        // actions 19 with 16, 34 with 32; 128 actions 37 with 32, 67 with 64); above 256 actions a wave each (65536 x 256: 20 us
-        // with 64 lanes in registers, 26 so), above 4096 a workgroup of 256, or of 1024 where rows are few (bf16, a wave / 256 /
-        // 1024 threads: 8192 x 4096 15 / 20 / 47, 1024 x 65536 32 / 25 / 27, 64 x 65536 24 / 11 / 11)
-        if (a.A <= 32) return launch_rows(k_logprobs_short<T, 8>, a, 8, 256, s);
-        if (a.A <= 64) return launch_rows(k_logprobs_short<T, 16>, a, 16, 256, s);
-        if (a.A <= 128) return launch_rows(k_logprobs_short<T, 32>, a, 32, 256, s);
-        if (a.A <= 256) return launch_rows(k_logprobs_short<T, 64>, a, 64, 256, s);
+        // the fewest lanes that hold a row in 16 registers each (f32, us, 262144 rows: 64 actions 14 with 8 lanes, 19 with 16; 128
+        // actions 22 with 8, 26 with 16; 65536 rows: 256 actions 13 with 16, 16 with 32, 500 actions 22 with 32, 28 with 64, 32
+        // with a wave's loop, which is no slower than 32 lanes for 512 in 16 bits); above, a wave a row, above 4096 a workgroup of
+        // 256, or of 1024 where rows are few (bf16, a wave / 256 / 1024 threads: 8192 x 4096 15 / 20 / 47, 1024 x 65536 32 / 25 / 27,
+        // 64 x 65536 24 / 11 / 11)
+        if (a.A <= 32) return launch_rows(k_logprobs_short<T, 8, 4>, a, 8, 256, s);
+        if (a.A <= 64) return launch_rows(k_logprobs_short<T, 8, 8>, a, 8, 256, s);
+        if (a.A <= 128) return launch_rows(k_logprobs_short<T, 8, 16>, a, 8, 256, s);
+        if (a.A <= 256) return launch_rows(k_logprobs_short<T, 16, 16>, a, 16, 256, s);
+        if (a.A <= 512) return launch_rows(k_logprobs_short<T, 32, 16>, a, 32, 256, s);
         if (a.A <= 4096) return launch_rows(k_logprobs_long<T, 64>, a, 64, 256, s);
         if (a.rows >= 1024) return launch_rows(k_logprobs_long<T, 256>, a, 256, 256, s);
         return launch_rows(k_logprobs_long<T, 1024>, a, 1024, 1024, s);
