@@ -482,27 +482,26 @@ __device__ __forceinline__ void pref_out(const PrefArgs &a, double loss, double 
     a.out2[1] = (float)(hits * a.inv_pairs);
 }
 
-// a workgroup a pair
-__global__ void __launch_bounds__(SEQ_BLOCK) k_pref_pair(PrefArgs a)
+// a workgroup a pair, from pair `first` on
+__global__ void __launch_bounds__(SEQ_BLOCK) k_pref_pair(PrefArgs a, long first)
 {
     __shared__ double part[SEQ_BLOCK / 64][4];
-    for (long b = blockIdx.x; b < a.B; b += gridDim.x) {
-        double v[4], acc[2];
-        pref_sum<SEQ_BLOCK>(a.side[0], b, 0, a.side[0].L, threadIdx.x, acc);
-        v[0] = acc[0]; v[1] = acc[1];
-        pref_sum<SEQ_BLOCK>(a.side[1], b, 0, a.side[1].L, threadIdx.x, acc);
-        v[2] = acc[0]; v[3] = acc[1];
-        const Ahead ahead[2] = {pref_ahead<SEQ_BLOCK>(a.side[0], b, 0, a.side[0].L, threadIdx.x), pref_ahead<SEQ_BLOCK>(a.side[1], b, 0, a.side[1].L, threadIdx.x)};
-        block_sum<4, SEQ_BLOCK>(v, part);
-        const double sum[2] = {v[0], v[2]}, count[2] = {v[1], v[3]};
-        const Margin m = margin_of(a, sum, count);
+    const long b = first + blockIdx.x;
+    double v[4], acc[2];
+    pref_sum<SEQ_BLOCK>(a.side[0], b, 0, a.side[0].L, threadIdx.x, acc);
+    v[0] = acc[0]; v[1] = acc[1];
+    pref_sum<SEQ_BLOCK>(a.side[1], b, 0, a.side[1].L, threadIdx.x, acc);
+    v[2] = acc[0]; v[3] = acc[1];
+    const Ahead ahead[2] = {pref_ahead<SEQ_BLOCK>(a.side[0], b, 0, a.side[0].L, threadIdx.x), pref_ahead<SEQ_BLOCK>(a.side[1], b, 0, a.side[1].L, threadIdx.x)};
+    block_sum<4, SEQ_BLOCK>(v, part);
+    const double sum[2] = {v[0], v[2]}, count[2] = {v[1], v[3]};
+    const Margin m = margin_of(a, sum, count);
 #pragma unroll
-        for (int k = 0; k < 2; ++k) pref_write<SEQ_BLOCK>(a.side[k], b, 0, a.side[k].L, threadIdx.x, ahead[k], pair_grad(a, m, k));
-        if (threadIdx.x == 0) {
-            pref_rewards(a, b, m);
-            a.pair[2 * b] = pair_loss(a, m);
-            a.pair[2 * b + 1] = m.z > 0.0 ? 1.0 : 0.0;
-        }
+    for (int k = 0; k < 2; ++k) pref_write<SEQ_BLOCK>(a.side[k], b, 0, a.side[k].L, threadIdx.x, ahead[k], pair_grad(a, m, k));
+    if (threadIdx.x == 0) {
+        pref_rewards(a, b, m);
+        a.pair[2 * b] = pair_loss(a, m);
+        a.pair[2 * b + 1] = m.z > 0.0 ? 1.0 : 0.0;
     }
 }
 
@@ -743,9 +742,12 @@ int ppo_preference_loss(const float *chosen, long chosen_stride, const float *re
         return ppo_launch_status();
     }
     if (chunks == 1) {
-        hipLaunchKernelGGL(k_pref_pair, dim3((unsigned)(pairs < (1L << 20) ? pairs : 1L << 20)), dim3(SEQ_BLOCK), 0, s, a);
-        const int rc = ppo_launch_status();
-        if (rc) return rc;
+        constexpr long MOST = 1L << 20;            // a launch has fewer than 2^32 threads
+        for (long first = 0; first < pairs; first += MOST) {
+            hipLaunchKernelGGL(k_pref_pair, dim3((unsigned)(pairs - first < MOST ? pairs - first : MOST)), dim3(SEQ_BLOCK), 0, s, a, first);
+            const int rc = ppo_launch_status();
+            if (rc) return rc;
+        }
         hipLaunchKernelGGL(k_pref_final, dim3(1), dim3(SEQ_BLOCK), 0, s, a);
     } else {
         hipLaunchKernelGGL(k_pref_sum, dim3((unsigned)(2 * pairs * chunks)), dim3(SEQ_BLOCK), 0, s, a);
