@@ -564,7 +564,8 @@ int ppo_token_logprobs_bwd(const void *logits, int dtype, long batch, long lengt
  *   out6 = {mean l, mean surrogate term, mean k, share of r outside the clip range, mean r - 1 - ln r, unmasked tokens}
  * sequence_mean 0: means over the unmasked tokens; 1: over the sequences that have one, of their tokens' means.  No token
  * unmasked: 0.  mask [batch, length] u8 (0 = masked) or NULL; what masked tokens hold is not used, their gradient is 0.
- * advantages [batch, length], or with per_sequence [batch] (adv_stride apart).  ref_log_probs may be NULL (no KL term).
+ * advantages [batch, length], or with per_sequence [batch] (adv_stride apart).  ref_log_probs may be NULL (no KL term); with
+ * kl_coef 0 the KL is reported and nothing else depends on it, even where it is infinite.
  * Every array has rows of its own stride (elements, >= 0) and contiguous tokens; g_log_probs [batch, length] contiguous or
  * NULL.  clip_low in [0, 1), clip_high >= 0.  Workspace: ppo_policy_kl_loss_workspace_bytes(batch, length), 8-byte
  * aligned; none (0, NULL) for a few thousand tokens.
@@ -583,7 +584,8 @@ int ppo_policy_kl_loss(const float *log_probs, long lp_stride, const float *old_
  * unmasked tokens, D = sum(chosen - ref_chosen) - sum(rejected - ref_rejected) (means instead of sums with `average`; a
  * sequence without tokens counts 0), z = beta D:
  *   PPO_PREF_SIGMOID: -(1 - label_smoothing) ln s(z) - label_smoothing ln s(-z);  PPO_PREF_HINGE: max(0, 1 - z);
- *   PPO_PREF_IPO: (D - 1 / (2 beta))^2
+ *   PPO_PREF_IPO: (D - 1 / (2 beta))^2.  A rejected log-prob of -inf makes z infinite: the first two give 0 and no gradient
+ *   (the first without label_smoothing).
  *   out2 = {mean loss, share of pairs with z > 0};  rewards [pairs, 2] = beta times the two sums (means)
  * The two sides have lengths and row strides (elements, >= 0) of their own; ref_* and mask_* may be NULL; g_chosen
  * [pairs, chosen_length] and g_rejected contiguous, or NULL.  Workspace: ppo_preference_loss_workspace_bytes(...), 8-byte
@@ -611,8 +613,7 @@ int ppo_preference_loss(const float *chosen, long chosen_stride, const float *re
  * ppo_linear_act_bwd: with u = g_y * deriv (deriv NULL: u = g_y), rounded to `dtype`:
  *   g_x [rows, inputs] = u W, g_weight [outputs, inputs] = u^T x, g_bias [outputs] = column sums of the unrounded u; each
  *   contiguous, of `dtype`, or NULL.  The residual's gradient is g_y.
- * rows, inputs, outputs and strides are at most 2^22 - 128, and no matrix has more than
- * 2^38 elements.  Results do not depend on anything but the arguments (sums have a fixed order).
+ * rows, inputs, outputs and strides are at most 2^22 - 128, and no matrix has more than 2^38 elements.  Results do not depend on anything but the arguments (sums have a fixed order).
  * Workspaces: the two functions' bytes, 16-byte aligned.  No output may overlap an input.
  */
 #define PPO_ACT_NONE 0

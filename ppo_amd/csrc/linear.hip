@@ -19,6 +19,9 @@
 // next stages on their way while the matrix cores work on this one.  16-byte pieces are swizzled inside their row so that what
 // a fragment read touches falls into different banks.  The operands of v_mfma are swapped (B first), so that a lane's
 // accumulators run along n.
+// Measured: bf16 8192 x 4096 -> 16384 with gelu 907 us forward (1.21 PFLOP/s) and 1750 us backward (1.26, of them 180 for u and
+// its column sums); f32 4096 x 4096 -> 4096 625 us forward (220 TFLOP/s, as bf16 products 1.32 PFLOP/s).  Plain library products
+// of these sizes reach 1.6 PFLOP/s in bf16 and 0.154 in f32.
 #include "token_common.h"
 #include "mfma_split.h"
 
@@ -44,7 +47,7 @@ template <class T> __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4
 // quarter of the instructions: the hardware's exp2 and reciprocal, and for the normal distribution's tail,
 // P(> a) = e^(-a^2 / 2) h(1 / (1 + 0.38 a / sqrt 2)), whose exponential is the density that the derivative needs as well,
 // a polynomial h of degree 7, fitted by Lawson's iteration: 1e-6 of the tail as far as f16 and bf16 results go.  (With
-// the library's functions the gelu layer's forward product took 1284 us, and takes 969 without an activation.)
+// the library's functions bf16 8192 x 4096 -> 16384 with gelu took 1284 us forward, and took 970 with no activation at all.)
 __device__ __forceinline__ float exp_fast(float x) { return __builtin_amdgcn_exp2f(x * 1.442695041f); }
 
 template <bool FAST> __device__ __forceinline__ void activate(int act, float z, float &y, float &d)
