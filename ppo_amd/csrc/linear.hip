@@ -19,8 +19,8 @@
 // next stages on their way while the matrix cores work on this one.  16-byte pieces are swizzled inside their row so that what
 // a fragment read touches falls into different banks.  The operands of v_mfma are swapped (B first), so that a lane's
 // accumulators run along n.
-// Measured: bf16 8192 x 4096 -> 16384 with gelu 907 us forward (1.21 PFLOP/s) and 1750 us backward (1.26, of them 180 for u and
-// its column sums); f32 4096 x 4096 -> 4096 625 us forward (220 TFLOP/s, as bf16 products 1.32 PFLOP/s).  Plain library products
+// Measured: bf16 8192 x 4096 -> 16384 with gelu 875 us forward (1.26 PFLOP/s) and 1715 us backward (1.28, of them 180 for u and
+// its column sums); f32 4096 x 4096 -> 4096 608 us forward (226 TFLOP/s, as bf16 products 1.36 PFLOP/s).  Plain library products
 // of these sizes reach 1.6 PFLOP/s in bf16 and 0.154 in f32.
 #include "token_common.h"
 #include "mfma_split.h"
@@ -43,75 +43,135 @@ template <class T> __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4
 }
 
 // ---- activations: value and derivative ------------------------------------------------------------------------------
-// To f32's accuracy for f32 layers; for 16-bit ones to a few 1e-7 of max(1, |value|), far below their half steps, in a
-// quarter of the instructions: the hardware's exp2 and reciprocal, and for the normal distribution's tail,
-// P(> a) = e^(-a^2 / 2) h(1 / (1 + 0.38 a / sqrt 2)), whose exponential is the density that the derivative needs as well,
-// a polynomial h of degree 7, fitted by Lawson's iteration: 1e-6 of the tail as far as f16 and bf16 results go.  (With
-// the library's functions bf16 8192 x 4096 -> 16384 with gelu took 1284 us forward, and took 970 with no activation at all.)
+// No library functions, whose branches cost more than the rest of an epilogue (with them bf16 8192 x 4096 -> 16384 with gelu took
+// 1284 us forward, and 970 with no activation at all; f32 191 x 106 -> 607 43 us, 33 with these, and 19 with a piece's values
+// worked out together, 15 with no activation).
+// FAST, for 16-bit layers: a few 1e-7 of max(1, |value|), far below their half steps.  Otherwise, for f32 ones: the rounding of an
+// exponential's argument is put right, a reciprocal gets a Newton step; values and derivatives are within 8 half steps of f32.
+// The normal distribution's tail is P(> a) = e^(-a^2 / 2) h(t) t, t = 1 / (1 + 0.38 a / sqrt 2), whose exponential is the density that the
+// derivative needs as well, h a polynomial fitted by Lawson's iteration for a up to 20: of degree 7, 1e-6 of the tail, or 10, 1e-9.
 __device__ __forceinline__ float exp_fast(float x) { return __builtin_amdgcn_exp2f(x * 1.442695041f); }
 
-template <bool FAST> __device__ __forceinline__ void activate(int act, float z, float &y, float &d)
+// e^x, -208 <= x <= 0
+__device__ __forceinline__ float exp_near(float x)
+{
+    const float t = x * 1.442695041f;
+    const float lost = __builtin_fmaf(x, 1.925963e-8f, __builtin_fmaf(x, 1.442695041f, -t));   // of x log2 e
+    const float e = __builtin_amdgcn_exp2f(t);
+    return __builtin_fmaf(e, lost * 0.6931471806f, e);
+}
+
+// 1 / x, x >= 1
+template <bool FAST> __device__ __forceinline__ float inverse(float x)
+{
+    const float r = __builtin_amdgcn_rcpf(x);
+    return FAST ? r : __builtin_fmaf(__builtin_fmaf(-x, r, 1.0f), r, r);
+}
+
+template <bool FAST> __device__ __forceinline__ void tanh_of(float z, float &y, float &d)
+{
+    const float a = fabsf(z);
+    const float e = FAST ? exp_fast(-2.0f * a) : exp_near(-2.0f * fminf(a, 52.0f)), r = inverse<FAST>(1.0f + e);
+    float t = (1.0f - e) * r;
+    if constexpr (FAST) {
+        t = a < 0.02f ? a - a * a * a * (1.0f / 3) : t;   // (what is left out: 2 a^5 / 15)
+    } else {
+        const float q = a * a;                            // the series to a^11: what is left out is below 2^-32
+        float p = -1382.0f / 155925;
+        p = __builtin_fmaf(p, q, 62.0f / 2835);
+        p = __builtin_fmaf(p, q, -17.0f / 315);
+        p = __builtin_fmaf(p, q, 2.0f / 15);
+        p = __builtin_fmaf(p, q, -1.0f / 3);
+        t = a < 0.25f ? __builtin_fmaf(a * q, p, a) : t;
+    }
+    y = copysignf(t, z);
+    d = 4.0f * e * r * r;                               // 1 - tanh^2 without its cancellation
+    if constexpr (!FAST) {
+        y = z != z ? z : y;
+        d = z != z ? z : d;
+    }
+}
+
+template <bool FAST> __device__ __forceinline__ void gelu_of(float z, float &y, float &d)
+{
+    float q, g;                                         // P(> |z|) and sqrt(2 pi) times the density
+    if constexpr (FAST) {
+        const float a = fabsf(z), t = inverse<FAST>(__builtin_fmaf(a, 0.38f * 0.70710678f, 1.0f));
+        g = __builtin_amdgcn_exp2f(a * a * -0.7213475204f);
+        q = -0.0627071038f;
+        q = __builtin_fmaf(q, t, 0.168012768f);
+        q = __builtin_fmaf(q, t, -0.0349497572f);
+        q = __builtin_fmaf(q, t, 0.123912774f);
+        q = __builtin_fmaf(q, t, 0.0902986899f);
+        q = __builtin_fmaf(q, t, 0.108288437f);
+        q = __builtin_fmaf(q, t, 0.107143678f);
+        q = q * t * g;
+    } else {
+        const float a = fminf(fabsf(z), 20.0f), t = inverse<FAST>(__builtin_fmaf(a, 0.38f * 0.70710678f, 1.0f));
+        const float s = a * a, lost = __builtin_fmaf(a, a, -s);
+        g = exp_near(-0.5f * s);
+        g = __builtin_fmaf(g, -0.5f * lost, g);
+        q = -0.015613814815878868f;
+        q = __builtin_fmaf(q, t, 0.0887872651219368f);
+        q = __builtin_fmaf(q, t, -0.19097009301185608f);
+        q = __builtin_fmaf(q, t, 0.18277713656425476f);
+        q = __builtin_fmaf(q, t, -0.10117244720458984f);
+        q = __builtin_fmaf(q, t, 0.0877317488193512f);
+        q = __builtin_fmaf(q, t, 0.04822973534464836f);
+        q = __builtin_fmaf(q, t, 0.08668842911720276f);
+        q = __builtin_fmaf(q, t, 0.09912792593240738f);
+        q = __builtin_fmaf(q, t, 0.10721877962350845f);
+        q = __builtin_fmaf(q, t, 0.10719534009695053f);
+        q = q * t * g;
+    }
+    const float phi = z > 0.0f ? 1.0f - q : q;
+    const bool far = fabsf(z) > 20.0f;                  // (NaN: near)
+    y = far ? fmaxf(z, 0.0f) : z * phi;
+    d = far ? (z > 0.0f ? 1.0f : 0.0f) : __builtin_fmaf(z * 0.3989422804f, g, phi);
+}
+
+template <bool FAST> __device__ __forceinline__ void silu_of(float z, float &y, float &d)
+{
+    float s;
+    if constexpr (FAST) {
+        s = inverse<FAST>(1.0f + exp_fast(-z));
+    } else {
+        const float e = exp_near(-fminf(fabsf(z), 104.0f)), r = inverse<FAST>(1.0f + e);
+        s = z >= 0.0f ? r : e * r;
+    }
+    y = z == -INFINITY ? 0.0f : z * s;
+    d = fabsf(z) == INFINITY ? s : s * (1.0f + z * (1.0f - s));
+}
+
+// N values at once
+template <bool FAST, int N> __device__ __forceinline__ void activate(int act, const float (&z)[N], float (&y)[N], float (&d)[N])
 {
     switch (act) {
-    case PPO_ACT_TANH: {
-        const float a = fabsf(z);
-        float e, r;
-        if constexpr (FAST) {
-            e = exp_fast(-2.0f * a);
-            r = __builtin_amdgcn_rcpf(1.0f + e);
-        } else {
-            e = expf(-2.0f * a);
-            r = 1.0f / (1.0f + e);
-        }
-        float t = (1.0f - e) * r;
-        if constexpr (FAST)
-            t = a < 0.02f ? a - a * a * a * (1.0f / 3) : t;   // (what is left out: 2 a^5 / 15)
-        else if (a < 0.1f)
-            t = tanhf(a);
-        y = copysignf(t, z);
-        d = 4.0f * e * r * r;                               // 1 - tanh^2 without its cancellation
+    case PPO_ACT_TANH:
+#pragma unroll
+        for (int j = 0; j < N; ++j) tanh_of<FAST>(z[j], y[j], d[j]);
         break;
-    }
     case PPO_ACT_RELU:
-        y = z > 0.0f ? z : (z != z ? z : 0.0f);
-        d = z > 0.0f ? 1.0f : 0.0f;
-        break;
-    case PPO_ACT_GELU: {
-        float phi, g;                                       // the normal distribution's P(< z), and sqrt(2 pi) times its density
-        if constexpr (FAST) {
-            const float a = fabsf(z), t = __builtin_amdgcn_rcpf(__builtin_fmaf(a, 0.38f * 0.70710678f, 1.0f));
-            g = __builtin_amdgcn_exp2f(a * a * -0.7213475204f);
-            float q = -0.0627071038f;
-            q = __builtin_fmaf(q, t, 0.168012768f);
-            q = __builtin_fmaf(q, t, -0.0349497572f);
-            q = __builtin_fmaf(q, t, 0.123912774f);
-            q = __builtin_fmaf(q, t, 0.0902986899f);
-            q = __builtin_fmaf(q, t, 0.108288437f);
-            q = __builtin_fmaf(q, t, 0.107143678f);
-            q = q * t * g;
-            phi = z > 0.0f ? 1.0f - q : q;
-        } else {
-            phi = 0.5f * erfcf(-0.70710678f * z);           // no cancellation in the left tail
-            g = expf(-0.5f * z * z);
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            y[j] = z[j] > 0.0f ? z[j] : (z[j] != z[j] ? z[j] : 0.0f);
+            d[j] = z[j] > 0.0f ? 1.0f : 0.0f;
         }
-        const bool far = fabsf(z) > 20.0f;                  // (NaN: near)
-        y = far ? fmaxf(z, 0.0f) : z * phi;
-        d = far ? (z > 0.0f ? 1.0f : 0.0f) : __builtin_fmaf(z * 0.3989422804f, g, phi);
         break;
-    }
-    case PPO_ACT_SILU: {
-        float s;
-        if constexpr (FAST)
-            s = __builtin_amdgcn_rcpf(1.0f + exp_fast(-z));
-        else
-            s = 1.0f / (1.0f + expf(-z));
-        y = z == -INFINITY ? 0.0f : z * s;
-        d = fabsf(z) == INFINITY ? s : s * (1.0f + z * (1.0f - s));
+    case PPO_ACT_GELU:
+#pragma unroll
+        for (int j = 0; j < N; ++j) gelu_of<FAST>(z[j], y[j], d[j]);
         break;
-    }
+    case PPO_ACT_SILU:
+#pragma unroll
+        for (int j = 0; j < N; ++j) silu_of<FAST>(z[j], y[j], d[j]);
+        break;
     default:
-        y = z;
-        d = 1.0f;
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            y[j] = z[j];
+            d[j] = 1.0f;
+        }
     }
 }
 
@@ -261,35 +321,48 @@ template <class T> __device__ __forceinline__ void finish(const GemmArgs &g, lon
 {
     using raw = typename T::raw;
     if (g.bias) z += T::load(reinterpret_cast<const raw *>(g.bias)[n]);
-    activate<T::BYTES == 2>(g.act, z, y, d);
+    const float in[1] = {z};
+    float value[1], slope[1];
+    activate<T::BYTES == 2, 1>(g.act, in, value, slope);
+    y = value[0];
+    d = slope[0];
     if (g.residual) y += T::load(reinterpret_cast<const raw *>(g.residual)[m * g.res_ld + n]);
 }
 
-// 16 bytes of neighbouring results of row m; `bias` is theirs
+// 16 bytes of neighbouring results of row m, or as many as the row still has; `bias` is theirs
 template <class T> __device__ __forceinline__ void epilogue(const GemmArgs &g, long m, long n, const float (&z)[16 / T::BYTES], const float (&bias)[16 / T::BYTES])
 {
     using raw = typename T::raw;
     constexpr int E = 16 / T::BYTES;
     raw *out = reinterpret_cast<raw *>(g.out) + m * g.N + n;
     typename D<T>::raw *der = g.deriv ? reinterpret_cast<typename D<T>::raw *>(g.deriv) + m * g.N + n : nullptr;
-    if (n + E <= g.N) {
-        float r[E], y[E], d[E];
-        if (g.residual) load16<T>(reinterpret_cast<const raw *>(g.residual) + m * g.res_ld + n, r);
+    const bool whole = n + E <= g.N;
+    float r[E], v[E], y[E], d[E];
+    if (g.residual) {
+        const raw *p = reinterpret_cast<const raw *>(g.residual) + m * g.res_ld + n;
+        if (whole) {
+            load16<T>(p, r);
+        } else {
 #pragma unroll
-        for (int j = 0; j < E; ++j) {
-            activate<T::BYTES == 2>(g.act, z[j] + bias[j], y[j], d[j]);
-            if (g.residual) y[j] += r[j];
+            for (int j = 0; j < E; ++j) r[j] = n + j < g.N ? T::load(p[j]) : 0.0f;
         }
+    }
+#pragma unroll
+    for (int j = 0; j < E; ++j) v[j] = z[j] + bias[j];
+    activate<T::BYTES == 2, E>(g.act, v, y, d);             // (together: one after the other they wait for each other)
+    if (g.residual) {
+#pragma unroll
+        for (int j = 0; j < E; ++j) y[j] += r[j];
+    }
+    if (whole) {
         store16<T>(out, y);
         if (der) store_n<D<T>, E>(der, d);
     } else {
 #pragma unroll
         for (int j = 0; j < E; ++j) {
             if (n + j < g.N) {
-                float y, d;
-                finish<T>(g, m, n + j, z[j], y, d);
-                out[j] = T::store(y);
-                if (der) der[j] = D<T>::store(d);
+                out[j] = T::store(y[j]);
+                if (der) der[j] = D<T>::store(d[j]);
             }
         }
     }
