@@ -895,13 +895,14 @@ template <class T, int ROWS, int COLS> __global__ void __launch_bounds__(256) k_
 
 // ---- host: how a product is cut -------------------------------------------------------------------------------------
 // Which calls go to k_few_rows.  Measured, that against the matrix cores, us: weights of a few MB, which stay in L2 when
-// they are read once for every 8 rows, 1000 x 1024 and 32 rows 9.7 / 14 in bf16, 10.7 / 15 in f32 (64 rows 12.5 / 13.5); 134 MB of
-// bf16 and 8 rows 46 / 32 (4 rows 30), the same not in place, where the matrix cores need a padded copy of the weights
-// first, 12 rows 98 / 87 (8 rows 54); 268 MB of f32 and 16 rows 109 / 104 (12 rows 106 / 109), not in place and 32 rows 178 / 196.
+// they are read once for every 8 rows, 1000 x 1024 and 32 rows 10 / 15 in bf16, 12 / 15 in f32 (40 rows 12 / 14, 14 / 14); bf16
+// 4000 x 4096 and 4 rows 12 / 15 (6 rows 27 / 14), 16384 x 4096 25 / 26 (6 rows 37 / 27), the same not in place, where the matrix
+// cores need a padded copy of the weights first, 8 rows 44 / 83 (10 rows 87 / 83); f32 4000 x 4096 and 4 rows 20 / 24 (6 rows
+// 33 / 24), 268 MB and 8 rows 65 / 72 (10 rows 105 / 73).
 bool few_rows(long rows, long N, long K, long e, bool in_place)
 {
     if (N * K * e <= 4L << 20) return rows <= 32;
-    return rows <= (e == 2 ? (in_place ? 4 : 10) : (in_place ? 12 : 32));
+    return rows <= (e == 2 ? (in_place ? 4 : 8) : (N * K * e > 128L << 20 ? 8 : 4));
 }
 constexpr long MOST_K = (1L << 22) - 128;   // 256 padded rows of so many floats still have 32-bit offsets
 
@@ -915,14 +916,15 @@ struct Plan {
 };
 
 // The tile, and how many workgroups share a tile's k: the cheapest by a model of the 256 CUs fitted to measurements (us; 16-bit /
-// f32).  A round of 256 x 256 tiles, one a CU: 19 + 1.4 / 4.6 a stage.  Of 128 x 128: 10 + 0.5 / 1.43 a stage alone on a CU, 10 +
-// 0.9 / 2.6 for two together; of the narrow ones 0.4 / 0.88 and 0.6 / 1.25.  Joining splits: 3 + 8 bytes a partial result at 4.5 TB/s.
-// Measured, large against small tiles, best splits of each: bf16 4096 x 4096 x 4096 111 against 124 us, 4096 x 4096 x 1024 45 / 49,
-// 6000 x 3000 x 512 61 / 45, 2048 x 2048 x 2048 45 / 28, 1024 x 1024 x 8192 45 (8 splits) / 34 (4; unsplit 60); f32 16384 x 512 x 3136
-// 303 (2) / 274, 512 x 3136 x 16384 319 (8) / 292 (5; unsplit 733).  Small against narrow tiles, at most 64 rows or columns: f32
-// 4020 x 33 x 6985 51 (16) / 36 (16), 16384 x 64 x 2048 54 (4) / 41 (2), 65536 x 64 x 64 20 / 14, 64 x 512 x 16384 26 (64) / 21 (64),
-// 64 x 64 x 65536 33 (256; unsplit 2877) / 28 (128); bf16 4020 x 33 x 6985 48 (16) / 46 (16), 16384 x 18 x 512 15 (2) / 12, 64 x 64 x
-// 65536 18 (64) / 15 (64), 64 x 16384 x 4096 29 (2) / 29 (2).
+// f32).  A round of 256 x 256 tiles, one a CU: 19 + 1.4 / 4.6 a stage.  Of 128 x 128: 10 + 0.5 / 1.43 a stage alone on a CU, 0.9 / 2.6
+// for two together; of the narrow ones 0.4 / 0.88 and 0.6 / 1.25.  Joining splits: 3 + 8 bytes a partial result at 4.5 TB/s.
+// (Constants closer to single runs chose small tiles for bf16 3000 x 3000 x 3000, 85 us against 67.)
+// Measured, large against small tiles, best splits of each: bf16 4096 x 4096 x 4096 99 against 115 us, 4096 x 4096 x 1024 35 / 39,
+// 6000 x 3000 x 512 41 / 32, 2048 x 2048 x 2048 44 / 24, 1024 x 1024 x 8192 45 (8 splits) / 34 (4; unsplit 57), 300 x 1000 x 1024 22 (4) / 13;
+// f32 16384 x 512 x 3136 286 (2) / 259, 512 x 3136 x 16384 314 (8) / 287 (5; unsplit 727).  Small against narrow tiles, at most 64 rows or
+// columns: f32 4020 x 33 x 6985 51 (16) / 36 (16), 16384 x 64 x 2048 54 (4) / 37 (4), 65536 x 64 x 64 16 / 12, 64 x 512 x 16384 26 (64) / 20
+// (64), 64 x 64 x 65536 33 (256; unsplit 2875) / 28 (256); bf16 4020 x 33 x 6985 47 (16) / 46 (16), 16384 x 64 x 2048 21 (2) / 18, 64 x 64 x
+// 65536 17 (64) / 14 (64), 64 x 16384 x 4096 29 (2) / 29 (2).
 Plan plan_of(long M, long N, long K, long e)
 {
     Plan p{};
@@ -932,13 +934,14 @@ Plan plan_of(long M, long N, long K, long e)
         if ((shape == NARROW_N && N > 64) || (shape == NARROW_M && M > 64)) continue;
         const long bm = shape == LARGE ? 256 : shape == NARROW_M ? 64 : 128, bn = shape == LARGE ? 256 : shape == NARROW_N ? 64 : 128;
         const long tm = (M + bm - 1) / bm, tn = (N + bn - 1) / bn;
+        const double fixed = shape == LARGE ? 19.0 : 10.0;
         const double one = shape == LARGE ? (e == 2 ? 1.4 : 4.6) : shape == SMALL ? (e == 2 ? 0.5 : 1.43) : (e == 2 ? 0.4 : 0.88);
         const double two = shape == SMALL ? (e == 2 ? 0.9 : 2.6) : (e == 2 ? 0.6 : 1.25);
         for (int splits : {1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 24, 32, 48, 64, 96, 128, 192, 256}) {
             if (splits > 1 && (p.steps < 4 * splits || (double)splits * M * N > 2.5e8)) break;
             const int per = (p.steps + splits - 1) / splits;
             const long rounds = (tm * tn * splits + 255) / 256;
-            double us = shape == LARGE ? rounds * (19.0 + one * per) : rounds / 2 * (10.0 + two * per) + rounds % 2 * (10.0 + one * per);
+            double us = shape == LARGE ? rounds * (fixed + one * per) : rounds / 2 * (fixed + two * per) + rounds % 2 * (fixed + one * per);
             if (splits > 1) us += 3.0 + (double)splits * M * N * 8.0 / 4.5e6;
             if (best != 0.0 && us >= best) continue;
             best = us;
