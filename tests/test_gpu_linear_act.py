@@ -100,6 +100,31 @@ def test_narrow_sizes(M, K, N, dtype):
     _check(*_make(M + K + N, M, K, N, dtype), "tanh")
 
 
+def test_the_most_rows_and_offsets_beyond_32_bits():
+    """2^22 - 128 rows, and results of more than 2^31 elements: the last rows, and a sum over all of them."""
+    from ppo_amd import ops
+    M = 2 ** 22 - 128
+    _check(*_make(5, M, 33, 18, torch.bfloat16, residual=False), "silu")
+    g = _gen(6)
+    x, w = torch.randn(M, 32, device="cuda", generator=g).bfloat16(), (torch.randn(640, 32, device="cuda", generator=g) / 6).bfloat16()
+    y, d = ops.linear_act_fwd(x, w, None, "tanh", want_deriv=True)
+    got = ops.linear_act_bwd(y, x, w, d)
+    h = 2.0 ** -8
+    for at in (slice(0, 70), slice(M - 300, M)):
+        xs = x[at].double().requires_grad_(True)
+        want = torch.tanh(xs @ w.double().t())
+        ez = _product_error(32) * (xs.detach().abs() @ w.double().abs().t())
+        assert bool(((y[at].double() - want).abs() <= h * want.abs() + 1.2 * ez + 32 * E).all())
+        (gx,) = torch.autograd.grad(want, xs, y[at].double())
+        u = (y[at].double() * (1 - want * want)).abs()
+        err = (y[at].double().abs() * (2.0 ** -11 + ez + 32 * E) + h * u) @ w.double().abs()
+        assert bool(((got[0][at].double() - gx).abs() <= h * gx.abs() + err + _product_error(640) * (u @ w.double().abs())).all())
+    # g_b sums f32 products of the y and d that the backward pass was given
+    want = sum((a.double() * b.double()).sum(0) for a, b in zip(y.split(1 << 18), d.split(1 << 18)))
+    size = sum((a.double() * b.double()).abs().sum(0) for a, b in zip(y.split(1 << 18), d.split(1 << 18)))
+    assert bool(((got[2].double() - want).abs() <= h * want.abs() + _product_error(M) * size).all())
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("rows", [4, 5, 10, 11, 12, 13, 32, 33])
 def test_few_rows_of_large_weights(rows, dtype):
