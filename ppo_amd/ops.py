@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes as C
 import functools
+import inspect
 import os
 
 import torch
@@ -696,16 +697,21 @@ def _refuse(what: str):
 
 
 def _on_tensor_device(fn):
-    """Launches go to the first tensor's device and that device's current stream."""
+    """Launches go to the first tensor's device and that device's current stream; that tensor may be named, too."""
+    name = next(iter(inspect.signature(fn).parameters))
+
     @functools.wraps(fn)
-    def call(first, *args, **kwargs):
+    def call(*args, **kwargs):
+        if not args and name not in kwargs:
+            return fn(**kwargs)                        # (Python's own error)
+        first = args[0] if args else kwargs[name]
         if not isinstance(first, torch.Tensor):
             _refuse(f"{fn.__name__} takes tensors")
         index = first.get_device()
         if index >= 0 and index != torch._C._cuda_getDevice():
             with torch.cuda.device(index):
-                return fn(first, *args, **kwargs)
-        return fn(first, *args, **kwargs)
+                return fn(*args, **kwargs)
+        return fn(*args, **kwargs)
     return call
 
 

@@ -1,0 +1,36 @@
+"""CPU: how the token-policy operators may be called, seen from what they refuse before anything is launched."""
+import pytest
+import torch
+
+from ppo_amd import _lib, ops
+
+BAD = _lib.PpoAmdError
+
+
+def z(*shape, dtype=torch.float32):
+    return torch.zeros(*shape, dtype=dtype)
+
+
+CALLS = [
+    (ops.token_logprobs_fwd, {"logits": z(2, 3, 4), "actions": z(2, 3, dtype=torch.int64)}),
+    (ops.token_logprobs_bwd, {"logits": z(2, 3, 4), "actions": z(2, 3, dtype=torch.int64), "stats": z(2, 3, 2), "entropy": z(2, 3), "g_logp": z(2, 3)}),
+    (ops.policy_kl_loss_fwd_bwd, {"new_lp": z(3, 5), "old_lp": z(3, 5), "adv": z(3)}),
+    (ops.preference_loss_fwd_bwd, {"chosen_lp": z(3, 5), "rejected_lp": z(3, 4)}),
+    (ops.linear_act_fwd, {"x": z(3, 5), "weight": z(4, 5)}),
+    (ops.linear_act_bwd, {"g": z(3, 4), "x": z(3, 5), "weight": z(4, 5)}),
+    (ops.token_logprobs, {"logits": z(2, 3, 4), "actions": z(2, 3, dtype=torch.int64)}),
+    (ops.policy_kl_loss, {"new_lp": z(3, 5), "old_lp": z(3, 5), "adv": z(3)}),
+    (ops.preference_loss, {"chosen_lp": z(3, 5), "rejected_lp": z(3, 4)}),
+    (ops.linear_act, {"x": z(3, 5), "weight": z(4, 5)}),
+]
+
+
+@pytest.mark.parametrize("fn,args", CALLS, ids=[c[0].__name__ for c in CALLS])
+def test_every_argument_may_be_named(fn, args):
+    """Host tensors: the refusal that comes after all checks of shapes and types, however the call is written."""
+    with pytest.raises(BAD, match="HIP device tensors"):
+        fn(**args)
+    with pytest.raises(BAD, match="HIP device tensors"):
+        fn(*args.values())
+    with pytest.raises(TypeError):
+        fn()
