@@ -13,6 +13,7 @@ import inspect
 import os
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -715,7 +716,14 @@ def _on_tensor_device(fn):
     return call
 
 
+def _no_tangents(name: str, *tensors):
+    """Forward-mode derivatives (torch.autograd.forward_ad) do not pass through these calls: none is dropped in silence."""
+    if forward_ad._current_level >= 0 and any(isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        _refuse(f"{name} has no forward-mode derivative")
+
+
 def _device_tensors(name: str, first, *others):
+    _no_tangents(name, first, *others)
     index = first.get_device()
     if index < 0:
         _refuse(f"{name} needs HIP device tensors; there is no CPU fallback")
@@ -778,6 +786,7 @@ def token_logprobs_bwd(logits, actions, stats, entropy, g_logp, g_entropy=None, 
     from the inputs and outputs of token_logprobs_fwd.  g_logp or g_entropy may be None."""
     lib = _lib.load()
     name = "token_logprobs_bwd"
+    _no_tangents(name, stats, entropy, g_logp, g_entropy)
     lg, act, batch, length, bs, ts = _token_rows(name, logits, actions, temperature)
     shape = act.shape
     if g_logp is None and g_entropy is None:
@@ -822,6 +831,7 @@ class _TokenLogprobs(torch.autograd.Function):
 def token_logprobs(logits, actions, temperature=1.0, ignore_index=-100):
     """(log p(action), entropy) of token_logprobs_fwd, both differentiable with respect to the logits."""
     if torch.is_grad_enabled() and logits.requires_grad:
+        _no_tangents("token_logprobs", logits)             # (inside apply they are not to be seen)
         return _TokenLogprobs.apply(logits, actions, float(temperature), int(ignore_index))
     return token_logprobs_fwd(logits, actions, temperature, ignore_index)[:2]
 
@@ -1094,5 +1104,6 @@ def linear_act(x, weight, bias=None, activation="none", residual=None):
     """y of linear_act_fwd, differentiable with respect to x, weight, bias and residual.  (ops.linear, for the agents'
     layers of at most 64 x 64, keeps their f32 library product.)"""
     if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in (x, weight, bias, residual)):
+        _no_tangents("linear_act", x, weight, bias, residual)
         return _LinearAct.apply(x, weight, bias, activation, residual)
     return linear_act_fwd(x, weight, bias, activation, residual)[0]

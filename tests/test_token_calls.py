@@ -34,3 +34,20 @@ def test_every_argument_may_be_named(fn, args):
         fn(*args.values())
     with pytest.raises(TypeError):
         fn()
+
+
+@pytest.mark.parametrize("fn,args", CALLS, ids=[c[0].__name__ for c in CALLS])
+def test_forward_mode_inputs_are_refused(fn, args):
+    """A tangent (torch.autograd.forward_ad) on any of the inputs would be lost: an error, also where a gradient is recorded."""
+    for key, t in args.items():
+        if not t.is_floating_point():
+            continue
+        for grad in (False, True):
+            with torch.autograd.forward_ad.dual_level():
+                dual = torch.autograd.forward_ad.make_dual(t.clone().requires_grad_(grad), torch.ones_like(t))
+                with pytest.raises(BAD, match="forward-mode"):
+                    fn(**{**args, key: dual})
+                with torch.no_grad(), pytest.raises(BAD, match="forward-mode"):
+                    fn(**{**args, key: dual})
+                with pytest.raises(BAD, match="HIP device tensors"):       # inside the level, but without tangents
+                    fn(**args)
