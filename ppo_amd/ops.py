@@ -228,6 +228,15 @@ class _AttachGrad(torch.autograd.Function):
         return (grad * g_out.to(grad.device)).to(dev).reshape(shape), None, None
 
 
+class _AttachGradOnce(_AttachGrad):
+    """The same for a gradient that is a constant here but not in truth: differentiating it again raises."""
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g_out):
+        return _AttachGrad.backward(ctx, g_out)
+
+
 def ppo_losses(x, new_v, old_lp, old_v, adv, clip, norm_adv, clip_va, ratio_input, stats3=None):
     """(policy_loss, value_loss, clip_frac, kl_div), each 0-d f32 on x.device; the first two are
     differentiable w.r.t. x (ratios or new log-probs) and new_v respectively."""
@@ -905,7 +914,7 @@ def policy_kl_loss(new_lp, old_lp, adv, mask=None, ref_lp=None, clip_low=0.2, cl
         out6, g = policy_kl_loss_fwd_bwd(new_lp, old_lp, adv, mask, ref_lp, clip_low, clip_high, kl_coef, kl, reduction, want_grad=need)
     loss = out6[0]
     if need:
-        loss = _AttachGrad.apply(new_lp, loss, g)
+        loss = _AttachGradOnce.apply(new_lp, loss, g)
     return loss, out6[1], out6[2], out6[3], out6[4]
 
 

@@ -51,3 +51,21 @@ def test_forward_mode_inputs_are_refused(fn, args):
                     fn(**{**args, key: dual})
                 with pytest.raises(BAD, match="HIP device tensors"):       # inside the level, but without tangents
                     fn(**args)
+
+
+def _on_the_host(monkeypatch):
+    """policy_kl_loss and preference_loss with a loss sum x^2 in the kernels' place: what their autograd nodes do needs no GPU."""
+    monkeypatch.setattr(ops, "policy_kl_loss_fwd_bwd", lambda new, *a, **k: (torch.full((6,), float((new * new).sum())), 2 * new))
+    monkeypatch.setattr(ops, "preference_loss_fwd_bwd", lambda c, r, *a, **k: (torch.full((2,), float((c * c).sum() + (r * r).sum())), z(2, 2), 2 * c, 2 * r))
+
+
+@pytest.mark.parametrize("which", ["policy", "preference"])
+def test_second_derivatives_of_the_losses_raise(which, monkeypatch):
+    """The gradients come from the kernels as constants: a second derivative would leave out the loss's own curvature."""
+    _on_the_host(monkeypatch)
+    x = torch.arange(6.0).reshape(2, 3).requires_grad_(True)
+    loss = ops.policy_kl_loss(x, x, x)[0] if which == "policy" else ops.preference_loss(x, z(2, 3))[0]
+    (g,) = torch.autograd.grad(loss * loss, x, create_graph=True)
+    assert torch.equal(g, 2 * loss.detach() * 2 * x.detach())
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        g.sum().backward()
