@@ -633,8 +633,8 @@ bool one_workgroup(long batch, long length)
 // 1 of 2 x 16384 31 / 19).  Otherwise about 512 in all, of 2048 tokens at least.
 int pref_chunks(long B, long Lc, long Lr)
 {
-    const long L = Lc > Lr ? Lc : Lr;
-    if ((B + ONE_BLOCK / 64 - 1) / (ONE_BLOCK / 64) * ((Lc + 255) / 256 + (Lr + 255) / 256) <= 10) return 0;
+    const long L = Lc > Lr ? Lc : Lr, turns = (Lc + 255) / 256 + (Lr + 255) / 256;
+    if ((B + ONE_BLOCK / 64 - 1) / (ONE_BLOCK / 64) * (turns > 0 ? turns : 1) <= 10) return 0;   // (a pair without tokens has a loss, too)
     if (B >= 256 || L <= 8192) return 1;
     long c = (512 + 2 * B - 1) / (2 * B);
     const long most = (L + 2047) / 2048;

@@ -88,3 +88,13 @@ def test_logits_of_four_axes_and_no_tokens():
         assert logp.shape == H.shape == shape
         (g,) = torch.autograd.grad(logp.sum() + H.sum(), logits)
         assert g.shape == logits.shape
+
+
+@pytest.mark.parametrize("pairs", [3, 80, 81, 70000])
+def test_preference_of_pairs_without_tokens(pairs):
+    """D = 0 of every pair: ln 2, no pair preferred, rewards 0."""
+    from ppo_amd import ops
+    none = torch.zeros(pairs, 0, device="cuda")
+    out, rewards, gc, gr = ops.preference_loss_fwd_bwd(none, none)
+    assert abs(float(out[0]) - math.log(2.0)) <= 2 * E * math.log(2.0) and float(out[1]) == 0.0
+    assert float(rewards.abs().max()) == 0.0 and gc.shape == gr.shape == (pairs, 0)

@@ -69,3 +69,12 @@ def test_second_derivatives_of_the_losses_raise(which, monkeypatch):
     assert torch.equal(g, 2 * loss.detach() * 2 * x.detach())
     with pytest.raises(RuntimeError, match="once_differentiable"):
         g.sum().backward()
+
+
+def test_pairs_without_tokens_are_shared_out():
+    """Both sides of length 0: as soon as there are more pairs than one workgroup takes in a few turns the others have work, and a
+    workspace for its results, as with one token a side."""
+    lib = _lib.load()
+    for pairs in (1, 8, 80, 81, 5000, 1 << 20):
+        one, none = (lib.ppo_preference_loss_workspace_bytes(pairs, n, 0) for n in (1, 0))
+        assert one == none and (none > 0) == (pairs > 80), pairs
