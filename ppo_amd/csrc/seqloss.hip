@@ -193,8 +193,11 @@ __device__ __forceinline__ void policy_groups(const PolicyArgs &a, const int *ro
                     } else if (a.kl == PPO_KL_K2) {
                         k = 0.5f * e * e; dk = e;
                     } else {
-                        k = fabsf(e) > 0.5f ? expf(-e) - 1.0f + e : expm1mx_near(-e);
-                        dk = e - k;                    // 1 - e^-e
+                        // 1 - e^-e: as it stands far from 0 (e = inf where the reference's log-prob is -inf: 1), e - k near it
+                        const bool far = fabsf(e) > 0.5f;
+                        const float x = expf(-e);
+                        k = far ? x - 1.0f + e : expm1mx_near(-e);
+                        dk = far ? 1.0f - x : e - k;
                     }
                     s_kl += k;
                     if (a.kl_coef_f != 0.0f) dl = __builtin_fmaf(a.kl_coef_f, dk, dl);   // (only reported: an infinite one is no 0 * inf)

@@ -98,3 +98,33 @@ def test_preference_of_pairs_without_tokens(pairs):
     out, rewards, gc, gr = ops.preference_loss_fwd_bwd(none, none)
     assert abs(float(out[0]) - math.log(2.0)) <= 2 * E * math.log(2.0) and float(out[1]) == 0.0
     assert float(rewards.abs().max()) == 0.0 and gc.shape == gr.shape == (pairs, 0)
+
+
+@pytest.mark.parametrize("kl,slope", [("k1", 1.0), ("k2", math.inf), ("k3", 1.0)])
+@pytest.mark.parametrize("B,L", [(2, 9), (300, 70)])
+def test_policy_loss_of_a_token_the_reference_excludes(B, L, kl, slope):
+    """A reference log-prob of -inf, and one that is 2^26 lower: the estimate is infinite or 2^26 (its square), its derivative
+    1 - e^-e = 1 (e for k2), and the other tokens' gradients are those without it.  A gradient is w (surrogate + c dk): three
+    roundings of its terms."""
+    from ppo_amd import ops
+    gen = torch.Generator("cuda").manual_seed(B + 1)
+    new = -torch.rand(B, L, device="cuda", generator=gen)
+    adv = torch.randn(B, L, device="cuda", generator=gen)
+    old, refp = new - 0.1, new - 0.2
+    coef, far = 0.25, 2.0 ** 26
+    want, g0 = ops.policy_kl_loss_fwd_bwd(new, old, adv, ref_lp=refp, kl_coef=coef, kl=kl)
+    _, plain = ops.policy_kl_loss_fwd_bwd(new, old, adv)
+    for low, dk in ((-math.inf, slope), (-far, {"k1": 1.0, "k2": far, "k3": 1.0}[kl])):
+        refp[1, 3] = low
+        out, g = ops.policy_kl_loss_fwd_bwd(new, old, adv, ref_lp=refp, kl_coef=coef, kl=kl)
+        others = torch.ones_like(new, dtype=torch.bool)
+        others[1, 3] = False
+        assert torch.equal(g[others], g0[others])
+        at = float(plain[1, 3]) + coef * dk / (B * L)
+        if math.isinf(dk):
+            assert float(g[1, 3]) == math.inf
+        else:
+            assert abs(float(g[1, 3]) - at) <= 4 * E * (abs(float(plain[1, 3])) + coef * dk / (B * L))
+        if math.isinf(low):
+            assert float(out[0]) == float(out[2]) == math.inf
+        assert torch.equal(out[[1, 3, 4, 5]], want[[1, 3, 4, 5]])
