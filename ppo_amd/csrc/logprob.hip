@@ -19,7 +19,9 @@ using namespace ppo_token;
 namespace {
 
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
-constexpr float LOWEST = -1e30f;   // stands for -inf as the factor of a weight that is 0 (0 * -inf would be NaN)
+// Stands for -inf, and all that is lower, as the factor of a weight 2^t that is 0 (0 * -inf would be NaN).  2^t is 0 below
+// -149 already, and neither a gradient of 1e35 nor a sum of 2^40 weights overflows when it is multiplied by this.
+constexpr float LOWEST = -1000.0f;
 
 struct Row {
     float m, s, u;   // max of the raw logits; sum 2^t; sum t 2^t with t = (x - m) * c, c = log2(e) / temperature

@@ -128,3 +128,25 @@ def test_policy_loss_of_a_token_the_reference_excludes(B, L, kl, slope):
         if math.isinf(low):
             assert float(out[0]) == float(out[2]) == math.inf
         assert torch.equal(out[[1, 3, 4, 5]], want[[1, 3, 4, 5]])
+
+
+@pytest.mark.parametrize("g_entropy,temperature", [(600.0, 1e-6), (65536.0, 1e-4), (1e28, 1e-6), (-3e9, 1.0)])
+@pytest.mark.parametrize("A", [18, 300, 3000, 9000])
+def test_masked_actions_under_large_entropy_gradients(A, g_entropy, temperature):
+    """The gradient of an illegal action is 0, however large its factors: g_entropy / temperature up to 1e34.  Logits whose
+    differences are of the temperature's size; tolerances as in test_gpu_token_losses.py."""
+    from ppo_amd import ops
+    gen = torch.Generator("cuda").manual_seed(A)
+    logits = torch.randn(5, A, device="cuda", generator=gen) * temperature
+    off = torch.rand(5, A, device="cuda", generator=gen) < 0.4
+    off[:, 0] = False
+    logits[off] = -math.inf
+    logits[3, 1] = torch.finfo(torch.float32).min              # masked by the type's lowest value
+    actions = torch.zeros(5, dtype=torch.int64, device="cuda")
+    logp, H, stats = ops.token_logprobs_fwd(logits, actions, temperature)
+    gh = torch.full_like(logp, g_entropy)
+    g = ops.token_logprobs_bwd(logits, actions, stats, H, None, gh, temperature)
+    want, size = ref.logprobs_grad(logits, actions, torch.zeros_like(gh), gh, temperature)
+    assert bool((g[off] == 0).all()) and float(g[3, 1]) == 0.0
+    tol = E * want.abs() + (100 + 40 * (1 + math.log(A))) * E * size * 2
+    assert bool(((g.double() - want).abs() <= tol).all())
