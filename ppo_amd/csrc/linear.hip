@@ -12,7 +12,7 @@
 //   * 16-bit inputs: v_mfma_f32_16x16x32_{bf16,f16}, f32 accumulators.
 //   * f32 inputs: every operand split in registers into three bf16 pieces that represent it exactly (mfma_split.h), six
 //     products of order <= 2 into one f32 accumulator: the three left out are below 2^-23 of the product.  f32 matrix
-//     instructions run at 1/16 of the bf16 rate, so six of these are 2.7 times as fast.  An infinite operand gives NaN.
+//     instructions run at 1/16 of the bf16 rate, so six of these are 2.7 times as fast.  Tiles with an infinite operand take those.
 // A workgroup of 8 waves computes 256 x 256 of C (4 waves: 128 x 128 where there would be too few of the larger ones, 128 x 64
 // or 64 x 128 where C has no more columns or rows), a wave 128 x 64, 64 x 64 or 32 x 64 of it.  Rows of 128 bytes of k (64
 // halves, 32 floats; where an operand's rows go along k, as many rows of the tile's width) are brought straight into LDS, the
@@ -308,6 +308,8 @@ template <class T> __global__ void __launch_bounds__(1024) k_bias_grad(const flo
 }
 
 // ---- the product -----------------------------------------------------------------------------------------------------
+constexpr uint32_t KEEP = 0x7fc5a5a5u;        // marks a result that is not written again
+
 struct GemmArgs {
     const void *A, *B;                 // [M, k], [N, k]; rows lda, ldb bytes apart
     long M, N, lda, ldb;
@@ -482,8 +484,9 @@ __global__ void __launch_bounds__(64 * WAVES_M * WAVES_N) k_gemm(GemmArgs g)
             return d;
         }
     };
-    Along al{pa0 + (long)s0 * KS * g.lda, (g.K - (long)s0 * KS - 1) * g.lda + ((g.M - m0) * T::BYTES + 3) / 4 * 4, KS * g.lda};
-    Along bl{pb0 + (long)s0 * KS * g.ldb, (g.K - (long)s0 * KS - 1) * g.ldb + ((g.N - n0) * T::BYTES + 3) / 4 * 4, KS * g.ldb};
+    auto along_a = [&] { return Along{pa0 + (long)s0 * KS * g.lda, (g.K - (long)s0 * KS - 1) * g.lda + ((g.M - m0) * T::BYTES + 3) / 4 * 4, KS * g.lda}; };
+    auto along_b = [&] { return Along{pb0 + (long)s0 * KS * g.ldb, (g.K - (long)s0 * KS - 1) * g.ldb + ((g.N - n0) * T::BYTES + 3) / 4 * 4, KS * g.ldb}; };
+    Along al = along_a(), bl = along_b();
     auto load_a = [&](int s, int to, int i) {
         const uint32_t at = base + wave * 1024 + to + i * WAVES * 1024;
         if constexpr (KA)
@@ -523,6 +526,66 @@ __global__ void __launch_bounds__(64 * WAVES_M * WAVES_N) k_gemm(GemmArgs g)
         for (int j = 0; j < NI; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     ppo_net::Bf16Select sel;
     if constexpr (T::BYTES == 4) sel.init();
+
+    // acc[i][j][e] is C[m0 + wm WM + 16 i + q][n0 + wn WN + 16 j + 4 kg + e].  The results go through LDS, PI rows of
+    // products of every wave at a time, so that a wave finishes and stores whole rows: from the accumulators' layout a
+    // store touched 32 cache lines, and each residual and derivative as many again.  (A pad of 16 bytes a row puts the 16
+    // rows of a write into different banks.)
+    constexpr int E = 16 / T::BYTES, LANES = BN / E, STEP = 64 * WAVES / LANES;
+    static_assert(MI % PI == 0, "whole passes");
+    const int col = threadIdx.x % LANES * E, row0 = threadIdx.x / LANES;
+    const long nn = n0 + col;
+    auto leave = [&](auto second, auto value) {             // second: only what is not KEEP
+        float bias[E];
+        load_bias<T>(g, nn, bias);
+#pragma unroll
+        for (int pass = 0; pass < MI / PI; ++pass) {
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < PI; ++i)
+#pragma unroll
+                for (int j = 0; j < NI; ++j)
+                    *reinterpret_cast<f32x4 *>(lds + ((wm * PI + i) * 16 + q) * LD + (wn * WN + j * 16 + kg * 4) * 4) = value(pass * PI + i, j);
+            __syncthreads();
+#pragma clang loop unroll(disable)
+            for (int r = row0; r < ROWS; r += STEP) {
+                const long m = m0 + r / (16 * PI) * WM + pass * 16 * PI + r % (16 * PI);
+                if (m >= g.M || nn >= g.N) continue;
+                float z[E];
+#pragma unroll
+                for (int j = 0; j < E; j += 4) {
+                    const f32x4 v = *reinterpret_cast<const f32x4 *>(lds + r * LD + (col + j) * 4);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) z[j + e] = v[e];
+                }
+                if constexpr (second()) {
+#pragma unroll
+                    for (int e = 0; e < E; ++e) {
+                        if (nn + e >= g.N || __builtin_bit_cast(uint32_t, z[e]) == KEEP) continue;
+                        if (g.partial) {
+                            g.partial[((long)blockIdx.y * g.M + m) * g.N + nn + e] = z[e];
+                        } else {
+                            float y, d;
+                            finish<T>(g, m, nn + e, z[e], y, d);
+                            reinterpret_cast<typename T::raw *>(g.out)[m * g.N + nn + e] = T::store(y);
+                            if (g.deriv) reinterpret_cast<typename D<T>::raw *>(g.deriv)[m * g.N + nn + e] = D<T>::store(d);
+                        }
+                    }
+                } else if (g.partial) {
+                    float *p = g.partial + ((long)blockIdx.y * g.M + m) * g.N + nn;
+                    if (nn + E <= g.N) {
+                        store_n<F32, E>(p, z);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < E; ++e)
+                            if (nn + e < g.N) p[e] = z[e];
+                    }
+                } else {
+                    epilogue<T>(g, m, nn, z, bias);
+                }
+            }
+        }
+    };
 
     if constexpr (T::BYTES == 2) {
         // A stage is two halves of 32 k.  While the matrix cores work on one half's fragments the next half's are read, so
@@ -647,10 +710,10 @@ __global__ void __launch_bounds__(64 * WAVES_M * WAVES_N) k_gemm(GemmArgs g)
         if (n > 2) turn(s++, std::integral_constant<int, 2>{});
         if (n > 1) turn(s++, std::integral_constant<int, 1>{});
         turn(s, std::integral_constant<int, 0>{});
+        leave(std::false_type{}, [&](int i, int j) { return acc[i][j]; });
     } else {
-        stage_a(s0, 0);
-        stage_b(s0, 0);
-        auto step = [&](int s, auto last) {
+        // plain: by the f32 matrix instructions, for the few tiles that need it (below)
+        auto step = [&](int s, auto last, auto plain) {
             asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
             __builtin_amdgcn_s_barrier();                   // stage s has landed for every wave, and nobody reads the other one
             asm volatile("" ::: "memory");
@@ -707,75 +770,102 @@ __global__ void __launch_bounds__(64 * WAVES_M * WAVES_N) k_gemm(GemmArgs g)
                     }
                 }
             };
-            u32x4 fb[NI][3];
+            if constexpr (plain()) {
+                // lane q, kg has k = 8 kg + e of row q for e = 0 .. 7: four k of a product of 16 x 16 x 4 for each e
+                f32x4 fb[NI][2];
 #pragma unroll
-            for (int j = 0; j < NI; ++j) {
-                f32x4 lo, hi;
-                read_b(j, lo, hi);
-                cut(lo, hi);
-                split(lo, hi, fb[j]);
-            }
+                for (int j = 0; j < NI; ++j) {
+                    read_b(j, fb[j][0], fb[j][1]);
+                    cut(fb[j][0], fb[j][1]);
+                }
 #pragma unroll
-            for (int i = 0; i < MI; ++i) {
-                f32x4 lo, hi;
-                u32x4 fa[3];
-                read_a(i, lo, hi);
-                cut(lo, hi);
-                split(lo, hi, fa);
+                for (int i = 0; i < MI; ++i) {
+                    f32x4 fa[2];
+                    read_a(i, fa[0], fa[1]);
+                    cut(fa[0], fa[1]);
 #pragma unroll
-                for (int t = 0; t < 6; ++t) {
-                    constexpr int PA[6] = {0, 2, 1, 0, 1, 0}, PB[6] = {2, 0, 1, 1, 0, 0};   // small terms first
+                    for (int e = 0; e < 8; ++e)
 #pragma unroll
-                    for (int j = 0; j < NI; ++j) acc[i][j] = mfma<BF16>(fb[j][PB[t]], fa[PA[t]], acc[i][j]);
+                        for (int j = 0; j < NI; ++j)
+                            acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(fb[j][e / 4][e % 4], fa[e / 4][e % 4], acc[i][j], 0, 0, 0);
+                }
+            } else {
+                u32x4 fb[NI][3];
+#pragma unroll
+                for (int j = 0; j < NI; ++j) {
+                    f32x4 lo, hi;
+                    read_b(j, lo, hi);
+                    cut(lo, hi);
+                    split(lo, hi, fb[j]);
+                }
+#pragma unroll
+                for (int i = 0; i < MI; ++i) {
+                    f32x4 lo, hi;
+                    u32x4 fa[3];
+                    read_a(i, lo, hi);
+                    cut(lo, hi);
+                    split(lo, hi, fa);
+#pragma unroll
+                    for (int t = 0; t < 6; ++t) {
+                        constexpr int PA[6] = {0, 2, 1, 0, 1, 0}, PB[6] = {2, 0, 1, 1, 0, 0};   // small terms first
+#pragma unroll
+                        for (int j = 0; j < NI; ++j) acc[i][j] = mfma<BF16>(fb[j][PB[t]], fa[PA[t]], acc[i][j]);
+                    }
                 }
             }
         };
-        for (int s = s0; s + 1 < s1; ++s) step(s, std::false_type{});
-        step(s1 - 1, std::true_type{});
-    }
-
-    // acc[i][j][e] is C[m0 + wm WM + 16 i + q][n0 + wn WN + 16 j + 4 kg + e].  The results go through LDS, PI rows of
-    // products of every wave at a time, so that a wave finishes and stores whole rows: from the accumulators' layout a
-    // store touched 32 cache lines, and each residual and derivative as many again.  (A pad of 16 bytes a row puts the 16
-    // rows of a write into different banks.)
-    constexpr int E = 16 / T::BYTES, LANES = BN / E, STEP = 64 * WAVES / LANES;
-    static_assert(MI % PI == 0, "whole passes");
-    const int col = threadIdx.x % LANES * E, row0 = threadIdx.x / LANES;
-    const long nn = n0 + col;
-    float bias[E];
-    load_bias<T>(g, nn, bias);
+        auto run = [&](auto plain) {
+            stage_a(s0, 0);
+            stage_b(s0, 0);
+            for (int s = s0; s + 1 < s1; ++s) step(s, std::false_type{}, plain);
+            step(s1 - 1, std::true_type{}, plain);
+        };
+        run(std::false_type{});
+        // An operand that is infinite, or above 3.38e38, where its first piece is, leaves NaN in every product that it is in.  Where a
+        // tile holds a NaN it is worked out again by the f32 matrix instructions (4096^3 with a NaN in every tile: 2.1 times as long), and what was
+        // NaN is replaced: such operands give what f32 arithmetic gives, as on the vector units, and the other results keep their
+        // bits.  (KEEP is a NaN itself: a result that has its bits is left as the NaN that it was.)
+        uint32_t nan[MI] = {}, found = 0;                   // bit 4 j + e of word i: acc[i][j][e]
+        float sum = 0.0f;                                   // NaN where one of them is, or infinite
 #pragma unroll
-    for (int pass = 0; pass < MI / PI; ++pass) {
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < PI; ++i)
+        for (int i = 0; i < MI; ++i)
 #pragma unroll
             for (int j = 0; j < NI; ++j)
-                *reinterpret_cast<f32x4 *>(lds + ((wm * PI + i) * 16 + q) * LD + (wn * WN + j * 16 + kg * 4) * 4) = acc[pass * PI + i][j];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sum = __builtin_fmaf(acc[i][j][e], 0.0f, sum);
+        if (__any(sum != sum)) {
+#pragma unroll
+            for (int i = 0; i < MI; ++i) {
+#pragma unroll
+                for (int j = 0; j < NI; ++j)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) nan[i] |= (acc[i][j][e] != acc[i][j][e] ? 1u : 0u) << (4 * j + e);
+                found |= nan[i];
+            }
+        }
+        leave(std::false_type{}, [&](int i, int j) { return acc[i][j]; });
+        __syncthreads();                                    // (the results have left LDS)
+        const bool mine = __any(found != 0);
+        if (lane == 0) reinterpret_cast<int *>(lds)[wave] = mine;
         __syncthreads();
-#pragma clang loop unroll(disable)
-        for (int r = row0; r < ROWS; r += STEP) {
-            const long m = m0 + r / (16 * PI) * WM + pass * 16 * PI + r % (16 * PI);
-            if (m >= g.M || nn >= g.N) continue;
-            float z[E];
+        int again = 0;
 #pragma unroll
-            for (int j = 0; j < E; j += 4) {
-                const f32x4 v = *reinterpret_cast<const f32x4 *>(lds + r * LD + (col + j) * 4);
+        for (int w = 0; w < WAVES; ++w) again |= reinterpret_cast<const int *>(lds)[w];
+        if (__builtin_amdgcn_readfirstlane(again) != 0) {
+            __syncthreads();                                // (the flags have been read)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) z[j + e] = v[e];
-            }
-            if (g.partial) {
-                float *p = g.partial + ((long)blockIdx.y * g.M + m) * g.N + nn;
-                if (nn + E <= g.N) {
-                    store_n<F32, E>(p, z);
-                } else {
+            for (int i = 0; i < MI; ++i)
 #pragma unroll
-                    for (int e = 0; e < E; ++e)
-                        if (nn + e < g.N) p[e] = z[e];
-                }
-            } else {
-                epilogue<T>(g, m, nn, z, bias);
-            }
+                for (int j = 0; j < NI; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            al = along_a();
+            bl = along_b();
+            run(std::true_type{});
+            leave(std::true_type{}, [&](int i, int j) {
+                f32x4 v;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = nan[i] >> (4 * j + e) & 1 ? acc[i][j][e] : __builtin_bit_cast(float, KEEP);
+                return v;
+            });
         }
     }
 }

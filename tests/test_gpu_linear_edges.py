@@ -31,3 +31,83 @@ def test_silu_derivative_keeps_its_digits(low, high):
         d = _of_bias(z[:: 1 if rows == 1 else 64].contiguous(), "silu", rows)[1].double()
         w = want[:: 1 if rows == 1 else 64]
         assert bool(((d - w).abs() <= E * (9 * w.abs() + 2) + 1e-37).all()), float(((d - w).abs() / (9 * w.abs() + 2)).max() / E)
+
+
+LIMITS = {  # act(z), act'(z) for z = inf and -inf
+    "none": (math.inf, -math.inf, None, None), "tanh": (1.0, -1.0, 0.0, 0.0), "relu": (math.inf, 0.0, 1.0, 0.0),
+    "gelu": (math.inf, 0.0, 1.0, 0.0), "silu": (math.inf, 0.0, 1.0, 0.0)}
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("act", list(LIMITS))
+@pytest.mark.parametrize("M,K,N", [(1, 70, 40), (8, 2, 3), (300, 70, 270), (60, 4000, 50)])
+def test_infinite_arguments_of_activations(M, K, N, act, dtype):
+    """z = inf and -inf, by the bias and by an operand, at one row, a few and on the matrix cores, with and without splits of k: the
+    limits of the activation and of its derivative; everything else is as without them, bit for bit."""
+    from ppo_amd import ops
+    g = torch.Generator("cuda").manual_seed(M + K)
+    x, w, b, r = (torch.randn(s, device="cuda", generator=g).to(dtype) for s in ((M, K), (N, K), (N,), (M, N)))
+    want, dwant = ops.linear_act_fwd(x, w, b, act, r, want_deriv=True)
+    up, down, d_up, d_down = LIMITS[act]
+    want[:, 1], want[:, 2] = (up + r[:, 1].float()).to(dtype), (down + r[:, 2].float()).to(dtype)
+    if dwant is not None:
+        dwant[:, 1], dwant[:, 2] = d_up, d_down
+    bias = b.clone()
+    bias[1], bias[2] = math.inf, -math.inf
+    y, d = ops.linear_act_fwd(x, w, bias, act, r, want_deriv=True)
+    assert torch.equal(y, want) and (d is None or torch.equal(d, dwant))
+    # the same by rows of the weights, against an input that is 1 there
+    x = x.clone()
+    x[:, K // 2] = 1.0
+    want, dwant = ops.linear_act_fwd(x, w, b, act, r, want_deriv=True)
+    want[:, 1], want[:, 2] = (up + r[:, 1].float()).to(dtype), (down + r[:, 2].float()).to(dtype)
+    if dwant is not None:
+        dwant[:, 1], dwant[:, 2] = d_up, d_down
+    weight = w.clone()
+    weight[1, K // 2], weight[2, K // 2] = math.inf, -math.inf
+    y, d = ops.linear_act_fwd(x, weight, b, act, r, want_deriv=True)
+    assert torch.equal(y, want) and (d is None or torch.equal(d, dwant))
+
+
+HUGE = 3.4e38                                               # above the largest bf16 value
+
+
+@pytest.mark.parametrize("M,K,N", [(3, 70, 40), (40, 70, 300), (300, 70, 301), (300, 1000, 270), (60, 4000, 50), (20001, 64, 40), (3585, 700, 3601), (3700, 3601, 700)])
+def test_infinite_and_huge_operands_of_f32_layers(M, K, N):
+    """The three products, f32, with infinities, a NaN and values that bf16 rounds to infinity: what 64 bits give rounded to f32, at any
+    number of rows (a few, and each tile, with splits and without), and the other rows and columns keep their bits.  A finite sum
+    is off by (8 + 4 sqrt K) e of its terms' magnitudes (test_gpu_linear_act.py)."""
+    from ppo_amd import ops
+    gen = torch.Generator("cuda").manual_seed(M + K + N)
+    r = lambda *s: torch.randn(s, device="cuda", generator=gen)  # noqa: E731
+
+    def check(call, a, b, k):
+        """call(a, b) = a b^T over k, both with rows along k here; specials into rows 1, 2 of a and row 5 of b"""
+        a, b = a.clamp(-2, 2), b.clamp(-2, 2)
+        clean = call(a, b)
+        a2, b2 = a.clone(), b.clone()
+        a2[1, k // 3], a2[1, k // 2] = math.inf, 1.5
+        a2[2, k - 1] = HUGE
+        a2[0, 0] = math.nan
+        b2[5, k // 2], b2[5, k - 1] = -math.inf, 0.25
+        b[:, k - 1] *= 0.25                                 # HUGE times these stays finite
+        b2[:, k - 1] *= 0.25
+        clean = call(a, b)
+        got, want = call(a2, b2), (a2.double() @ b2.double().t())
+        want32 = want.float()
+        assert torch.equal(torch.isnan(got), torch.isnan(want32)) and torch.equal(got == math.inf, want32 == math.inf)
+        assert torch.equal(got == -math.inf, want32 == -math.inf)
+        assert bool(torch.isinf(got[1]).any()) and bool(torch.isfinite(got[2, 6:]).all())
+        size = a2.double().abs() @ b2.double().abs().t()
+        fin = torch.isfinite(want32)
+        assert bool(((got.double() - want).abs()[fin] <= ((8 + 4 * math.sqrt(k)) * E * size)[fin]).all())
+        rows, cols = torch.ones(a.shape[0], dtype=torch.bool), torch.ones(b.shape[0], dtype=torch.bool)
+        rows[:3] = False
+        cols[5] = False
+        if rows.any():
+            assert torch.equal(got[rows][:, cols], clean[rows][:, cols])
+
+    check(lambda a, b: ops.linear_act_fwd(a, b)[0], r(M, K), r(N, K), K)
+    x, w = r(M, K), r(N, K)
+    check(lambda a, b: ops.linear_act_bwd(a, x, b.t().contiguous(), want_weight=False, want_bias=False)[0], r(M, N), r(K, N), N)
+    check(lambda a, b: ops.linear_act_bwd(a.t().contiguous(), b.t().contiguous(), w, want_input=False, want_bias=False)[1], r(N, M), r(K, M), M)
