@@ -111,3 +111,71 @@ def test_infinite_and_huge_operands_of_f32_layers(M, K, N):
     x, w = r(M, K), r(N, K)
     check(lambda a, b: ops.linear_act_bwd(a, x, b.t().contiguous(), want_weight=False, want_bias=False)[0], r(M, N), r(K, N), N)
     check(lambda a, b: ops.linear_act_bwd(a.t().contiguous(), b.t().contiguous(), w, want_input=False, want_bias=False)[1], r(N, M), r(K, M), M)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("M,K,N", [(3600, 3500, 3700), (3601, 3501, 3703), (1500, 8192, 3000), (1501, 3001, 8191), (8191, 2999, 1500), (2048, 16385, 3000)])
+def test_large_tiles_in_every_product(M, K, N, dtype):
+    """The tile of 256 x 256 forward and in both gradients, whole and cut, operands in place and copied, through many stages of its
+    ring; the last four have splits of k in it: forward (3 in 16 bits), g_x (3), g_W (3) and forward again (2)."""
+    from test_gpu_linear_act import _check, _make
+    _check(*_make(M + K + N, M, K, N, dtype), "silu")
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_small_magnitudes(dtype):
+    """Inputs of 2^-100 in f32 and bf16 (f32's third bf16 piece ends at 2^-126), 2^-10 in f16: as exact, relative to the terms, as others."""
+    from ppo_amd import ops
+    gen = torch.Generator("cuda").manual_seed(7)
+    x, w = (torch.randn(s, device="cuda", generator=gen).to(dtype) for s in ((200, 300), (150, 300)))
+    x *= 2.0 ** (-10 if dtype == torch.float16 else -100)
+    y = ops.linear_act_fwd(x, w)[0].double()
+    want, size = x.double() @ w.double().t(), x.double().abs() @ w.double().abs().t()
+    tiny = 2.0 ** -25 if dtype == torch.float16 else 0.0
+    assert bool(((y - want).abs() <= torch.finfo(dtype).eps / 2 * want.abs() + (8 + 4 * math.sqrt(300)) * E * size + tiny).all())
+
+
+class _Guarded:
+    """Buffers on the GPU inside one that is full of 0xab, and whether what is around them still is."""
+
+    def __init__(self):
+        self.raw, self.used = [], []
+
+    def of(self, nbytes, align):
+        raw = torch.full((nbytes + 4096,), 0xAB, dtype=torch.uint8, device="cuda")
+        at = 1024 + align                                   # torch's own blocks begin at multiples of 512
+        self.raw.append(raw)
+        self.used.append((at, nbytes))
+        return raw.data_ptr() + at, raw[at:at + nbytes]
+
+    def check(self):
+        for raw, (at, n) in zip(self.raw, self.used):
+            assert bool((raw[:at] == 0xAB).all()) and bool((raw[at + n:] == 0xAB).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("M,K,N", [(1, 7, 5), (3, 70, 41), (9, 33, 15), (40, 2049, 301), (129, 127, 257), (300, 1031, 71), (20001, 63, 41), (61, 8001, 127),
+                                   (3601, 701, 3603), (3701, 3601, 701), (701, 3601, 3585)])
+def test_nothing_beside_the_outputs_is_written(M, K, N, dtype):
+    """The C entries with every output and the workspace between guards: odd sizes at the outputs' least alignment, each tile."""
+    from ppo_amd import _lib, ops
+    lib = _lib.load()
+    gen = torch.Generator("cuda").manual_seed(M * N)
+    x, w, b, r, g = (torch.randn(s, device="cuda", generator=gen).to(dtype) for s in ((M, K), (N, K), (N,), (M, N), (M, N)))
+    e, dt = x.element_size(), {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}[dtype]
+    de, ddt = (2, torch.float16) if dtype == torch.bfloat16 else (4, torch.float32)
+    guard = _Guarded()
+    nws = lib.ppo_linear_act_fwd_workspace_bytes(M, K, N, dt)
+    (py, y), (pd, d), (pw, _) = guard.of(M * N * e, e), guard.of(M * N * de, de), guard.of(nws, 16)
+    stream = torch.cuda.current_stream().cuda_stream
+    assert lib.ppo_linear_act_fwd(x.data_ptr(), K, w.data_ptr(), K, b.data_ptr(), r.data_ptr(), N, dt, M, K, N, 2, py, pd, pw, nws, stream) == 0
+    guard.check()
+    want, dwant = ops.linear_act_fwd(x, w, b, "relu", r, want_deriv=True)
+    y, d = y.clone().view(dtype).view(M, N), d.clone().view(ddt).view(M, N)
+    assert torch.equal(y, want) and torch.equal(d, dwant)
+    nws = lib.ppo_linear_act_bwd_workspace_bytes(M, K, N, dt)
+    (px, gx), (pgw, gw), (pb, gb), (pw, _) = guard.of(M * K * e, e), guard.of(N * K * e, e), guard.of(N * e, e), guard.of(nws, 16)
+    assert lib.ppo_linear_act_bwd(g.data_ptr(), N, x.data_ptr(), K, w.data_ptr(), K, dwant.data_ptr(), dt, M, K, N, px, pgw, pb, pw, nws, stream) == 0
+    guard.check()
+    for got, q in zip((gx, gw, gb), ops.linear_act_bwd(g, x, w, dwant)):
+        assert torch.equal(got.clone().view(dtype).view(q.shape), q)
