@@ -150,3 +150,35 @@ def test_masked_actions_under_large_entropy_gradients(A, g_entropy, temperature)
     assert bool((g[off] == 0).all()) and float(g[3, 1]) == 0.0
     tol = E * want.abs() + (100 + 40 * (1 + math.log(A))) * E * size * 2
     assert bool(((g.double() - want).abs() <= tol).all())
+
+
+@pytest.mark.parametrize("rows,A,most_fwd,most_bwd", [(2 ** 27 + 5, 129, 2 ** 27, 2 ** 27), (2 ** 26 + 9, 257, 2 ** 26, None), (2 ** 25 + 5, 513, 2 ** 25, 2 ** 25),
+                                                      (2 ** 23 + 3, 4097, 2 ** 23, 2 ** 23), (2 ** 22 + 3, 8193, None, 2 ** 22)])
+def test_logprobs_rows_of_more_than_one_launch_each_kernel(rows, A, most_fwd, most_bwd):
+    """bf16 rows just beyond what one launch of 2^31 threads holds (None: it holds them all): 129 actions have 16 lanes a row in both
+    directions, 257 have 32 forward, 513 a wave in both, 4097 a workgroup of 256 in both, 8193 two workgroups backward.  Rows on both
+    sides of the border, the first and the last, at the tolerances of test_gpu_token_losses.py."""
+    from ppo_amd import ops
+    torch.cuda.empty_cache()
+    logits = torch.empty(rows, A, device="cuda", dtype=torch.bfloat16).normal_(generator=torch.Generator("cuda").manual_seed(A))
+    actions = torch.randint(0, A, (rows,), device="cuda", dtype=torch.int32, generator=torch.Generator("cuda").manual_seed(rows))
+    logp, H, stats = ops.token_logprobs_fwd(logits, actions)
+    ones = torch.ones(1, device="cuda").expand(rows).contiguous()
+    g = ops.token_logprobs_bwd(logits, actions, stats, None, ones)
+    assert bool(torch.isfinite(logp).all()) and bool((logp < 0).all()) and bool((H > 0).all())
+    slices = [slice(0, 64), slice(rows - 64, rows)] + [slice(m - 64, min(m + 64, rows)) for m in {most_fwd, most_bwd} - {None}]
+    for at in slices:
+        lp, h = ref.logprobs(logits[at], actions[at])
+        assert bool(((logp[at].double() - lp).abs() <= 90 * E + 4 * E * lp.abs()).all())
+        assert bool(((H[at].double() - h).abs() <= 180 * E * (1 + math.log(A))).all())
+        want, size = ref.logprobs_grad(logits[at], actions[at], ones[at], None)
+        tol = 2.0 ** -8 * want.abs() + (100 + 40 * (1 + math.log(A))) * E * size * 2 + 2.0 ** -126
+        assert bool(((g[at].double() - want).abs() <= tol).all())
+    # every row's gradient sums to 0: p_a - 1 against the rest, each rounded to bf16
+    del logits
+    step = max(1, 2 ** 31 // A)
+    for at in range(0, rows, step):
+        part = g[at:at + step]
+        assert bool((part.sum(-1, dtype=torch.float32).abs() <= 2.0 ** -8 * part.abs().sum(-1, dtype=torch.float32) + 1e-3).all())
+    del part, g
+    torch.cuda.empty_cache()
