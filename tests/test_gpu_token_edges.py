@@ -182,3 +182,43 @@ def test_logprobs_rows_of_more_than_one_launch_each_kernel(rows, A, most_fwd, mo
         assert bool((part.sum(-1, dtype=torch.float32).abs() <= 2.0 ** -8 * part.abs().sum(-1, dtype=torch.float32) + 1e-3).all())
     del part, g
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("B,L,A", [(1, 1, 1), (3, 5, 18), (7, 33, 129), (2, 9, 513), (5, 3, 4099), (3, 20001, 3), (300, 71, 2)])
+def test_nothing_beside_the_outputs_is_written(B, L, A):
+    """The C entries with every output and workspace between guards, odd sizes, outputs at their least alignment: the bits of the
+    wrappers' results, and the guards are as they were."""
+    from ppo_amd import _lib, ops
+    from test_gpu_linear_edges import _Guarded
+    lib, gen, guard = _lib.load(), torch.Generator("cuda").manual_seed(B + L + A), _Guarded()
+    stream = torch.cuda.current_stream().cuda_stream
+    f32 = lambda view, *shape: view.clone().view(torch.float32).view(shape)  # noqa: E731
+    actions = torch.randint(0, A, (B, L), device="cuda", generator=gen)
+    for dt, dtype in ((0, torch.float32), (1, torch.bfloat16), (2, torch.float16)):
+        logits = torch.randn(B, L, A, device="cuda", generator=gen).to(dtype)
+        (pl, lp), (ph, h), (ps, st) = guard.of(B * L * 4, 4), guard.of(B * L * 4, 4), guard.of(B * L * 8, 8)
+        (pg, g) = guard.of(logits.numel() * logits.element_size(), logits.element_size())
+        assert lib.ppo_token_logprobs_fwd(logits.data_ptr(), dt, B, L, A, L * A, A, actions.data_ptr(), 8, 0.8, -100, pl, ph, ps, stream) == 0
+        want = ops.token_logprobs_fwd(logits, actions, 0.8)
+        assert lib.ppo_token_logprobs_bwd(logits.data_ptr(), dt, B, L, A, L * A, A, actions.data_ptr(), 8, ps, ph, pl, ph, 0.8, -100, pg, stream) == 0
+        guard.check()
+        assert torch.equal(f32(lp, B, L), want[0]) and torch.equal(f32(h, B, L), want[1]) and torch.equal(f32(st, B, L, 2), want[2])
+        assert torch.equal(g.clone().view(dtype).view(B, L, A), ops.token_logprobs_bwd(logits, actions, want[2], want[1], want[0], want[1], 0.8))
+    new, old, adv, refp = (-torch.rand(B, L, device="cuda", generator=gen) for _ in range(4))
+    mask = torch.rand(B, L, device="cuda", generator=gen) < 0.7
+    n = lib.ppo_policy_kl_loss_workspace_bytes(B, L)
+    (po, out), (pg, g), (pw, _) = guard.of(24, 4), guard.of(B * L * 4, 4), guard.of(n, 8)
+    assert lib.ppo_policy_kl_loss(new.data_ptr(), L, old.data_ptr(), L, adv.data_ptr(), L, 0, refp.data_ptr(), L, mask.data_ptr(), L, B, L, 0.2, 0.2, 0.1, 3, 1,
+                                  po, pg, pw, n, stream) == 0
+    guard.check()
+    want = ops.policy_kl_loss_fwd_bwd(new, old, adv, mask, refp, kl_coef=0.1, reduction="sequence")
+    assert torch.equal(f32(out, 6), want[0]) and torch.equal(f32(g, B, L), want[1])
+    m = L // 2                                               # the rejected answers are shorter, none at all with one token
+    n = lib.ppo_preference_loss_workspace_bytes(B, L, m)
+    (po, out), (pr, rew), (pc, gc), (pj, gr), (pw, _) = guard.of(8, 4), guard.of(B * 8, 4), guard.of(B * L * 4, 4), guard.of(B * m * 4, 4), guard.of(n, 8)
+    assert lib.ppo_preference_loss(new.data_ptr(), L, refp.data_ptr(), L, mask.data_ptr(), L, L, old.data_ptr(), L, adv.data_ptr(), L, mask.data_ptr(), L, m, B, 0,
+                                   0.1, 0.0, 0, po, pr, pc, pj, pw, n, stream) == 0
+    guard.check()
+    want = ops.preference_loss_fwd_bwd(new, old[:, :m], refp, adv[:, :m], mask, mask[:, :m])
+    for got, w in zip((out, rew, gc, gr), want):
+        assert torch.equal(f32(got, *w.shape), w)
