@@ -567,7 +567,7 @@ int ppo_token_logprobs_bwd(const void *logits, int dtype, long batch, long lengt
  * advantages [batch, length], or with per_sequence [batch] (adv_stride apart).  ref_log_probs may be NULL (no KL term); with
  * kl_coef 0 the KL is reported and nothing else depends on it, even where it is infinite.
  * Every array has rows of its own stride (elements, >= 0) and contiguous tokens; g_log_probs [batch, length] contiguous or
- * NULL.  clip_low in [0, 1), clip_high >= 0.  Workspace: ppo_policy_kl_loss_workspace_bytes(batch, length), 8-byte
+ * NULL.  clip_low in [0, 1), clip_high in [0, 1e30], kl_coef in [-1e30, 1e30].  Workspace: ppo_policy_kl_loss_workspace_bytes(batch, length), 8-byte
  * aligned; none (0, NULL) for a few thousand tokens.
  */
 #define PPO_KL_K1 1

@@ -670,7 +670,7 @@ int ppo_policy_kl_loss(const float *log_probs, long lp_stride, const float *old_
     PPO_REQUIRE(!ref_log_probs || rows_ok(ref_log_probs, batch, length, ref_stride));
     PPO_REQUIRE(!mask || (mask_stride >= 0 && (__int128)(batch - 1) * mask_stride + length < ((__int128)1 << 60)));
     PPO_REQUIRE(out6 && ppo_aligned(out6, 4) && ppo_aligned(g_log_probs, 4));
-    PPO_REQUIRE(clip_low >= 0.0 && clip_low < 1.0 && clip_high >= 0.0 && clip_high <= 1e30 && kl_coef == kl_coef);
+    PPO_REQUIRE(clip_low >= 0.0 && clip_low < 1.0 && clip_high >= 0.0 && clip_high <= 1e30 && kl_coef >= -1e30 && kl_coef <= 1e30);
     PPO_REQUIRE(kl_kind == PPO_KL_K1 || kl_kind == PPO_KL_K2 || kl_kind == PPO_KL_K3);
     const bool one = one_workgroup(batch, length);
     PPO_REQUIRE(one || (workspace && ppo_aligned(workspace, 8) && workspace_bytes >= ppo_policy_kl_loss_workspace_bytes(batch, length)));

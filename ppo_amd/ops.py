@@ -879,8 +879,8 @@ def policy_kl_loss_fwd_bwd(new_lp, old_lp, adv, mask=None, ref_lp=None, clip_low
         _refuse(f"{name}: log-probs are [sequences, tokens]")
     if kl not in KL_KINDS or reduction not in ("token", "sequence"):
         _refuse(f"{name}: kl is one of {sorted(KL_KINDS)}, reduction 'token' or 'sequence'")
-    if not (0.0 <= clip_low < 1.0 and 0.0 <= clip_high <= 1e30 and kl_coef == kl_coef):
-        _refuse(f"{name}: clip_low in [0, 1), clip_high >= 0, kl_coef a number")
+    if not (0.0 <= clip_low < 1.0 and 0.0 <= clip_high <= 1e30 and -1e30 <= kl_coef <= 1e30):
+        _refuse(f"{name}: clip_low in [0, 1), clip_high in [0, 1e30], kl_coef in [-1e30, 1e30]")
     if old_lp is None or adv is None:
         _refuse(f"{name}: old_lp and adv are needed")
     shape = new_lp.shape

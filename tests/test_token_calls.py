@@ -1,4 +1,6 @@
 """CPU: how the token-policy operators may be called, seen from what they refuse before anything is launched."""
+import ctypes
+
 import pytest
 import torch
 
@@ -78,3 +80,15 @@ def test_pairs_without_tokens_are_shared_out():
     for pairs in (1, 8, 80, 81, 5000, 1 << 20):
         one, none = (lib.ppo_preference_loss_workspace_bytes(pairs, n, 0) for n in (1, 0))
         assert one == none and (none > 0) == (pairs > 80), pairs
+
+
+@pytest.mark.parametrize("kl_coef", [float("inf"), -float("inf"), 1e31, 1e300])
+def test_kl_coefficients_that_f32_does_not_hold_are_refused(kl_coef):
+    """As infinity they made a token whose estimate is 0 NaN."""
+    x = z(3, 5)
+    for fn in (ops.policy_kl_loss, ops.policy_kl_loss_fwd_bwd):
+        with pytest.raises(BAD, match="kl_coef"):
+            fn(x, x, x, ref_lp=x, kl_coef=kl_coef)
+    buf = (ctypes.c_char * 4096)()
+    p = (ctypes.addressof(buf) + 63) // 64 * 64
+    assert _lib.load().ppo_policy_kl_loss(p, 4, p, 4, p, 4, 0, p, 4, p, 4, 2, 4, 0.2, 0.2, kl_coef, 3, 0, p, p, None, 0, None) == 1
