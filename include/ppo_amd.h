@@ -614,7 +614,9 @@ int ppo_preference_loss(const float *chosen, long chosen_stride, const float *re
  * ppo_linear_act_bwd: with u = g_y * deriv (deriv NULL: u = g_y), rounded to `dtype`:
  *   g_x [rows, inputs] = u W, g_weight [outputs, inputs] = u^T x, g_bias [outputs] = column sums of the unrounded u; each
  *   contiguous, of `dtype`, or NULL.  The residual's gradient is g_y.
- * rows, inputs, outputs and strides are at most 2^22 - 128, and no matrix has more than 2^38 elements.  Results do not depend on anything but the arguments (sums have a fixed order).
+ * rows, inputs, outputs and strides are at most 2^22 - 128, and no matrix has more than 2^38 elements; those that a call has
+ * to copy, multiply by deriv or sum up first have no more than 2^36 together (in tiles of 64 x 64; refused otherwise).
+ * Results do not depend on anything but the arguments (sums have a fixed order).
  * Workspaces: the two functions' bytes, 16-byte aligned.  No output may overlap an input.
  */
 #define PPO_ACT_NONE 0

@@ -5,8 +5,9 @@
 // asked for; then for a gradient g of y
 //     u = g d,   g_x = u W,   g_W = u^T x,   g_b = sum over rows of u.
 // d is kept rather than z: act'(z) of a z rounded to bf16 is off by 1.5 % for tanh at z = 4.  It is kept in f16 for bf16
-// layers (|d| < 1.2: 8 times finer than bf16) and in f32 for the others, so that the one rounding that counts beside the
-// outputs' own is that of u to the inputs' type, which the two products need; g_b sums u unrounded, in f32.
+// layers (|d| < 1.2; 8 times finer than bf16 for |d| >= 2^-14, steps of 2^-24 below, where g d hardly counts beside others) and in f32
+// for the others, so that the one rounding that counts beside the outputs' own is that of u to the inputs' type, which the two
+// products need: g_x and g_W are off by sqrt 2 of what the outputs' rounding alone leaves.  g_b sums u unrounded, in f32.
 //
 // One product, C[m, n] = sum_k A[m, k] B[n, k], serves all three, each operand with its rows along m (n) or along k.
 //   * 16-bit inputs: v_mfma_f32_16x16x32_{bf16,f16}, f32 accumulators.

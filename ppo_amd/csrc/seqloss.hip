@@ -367,8 +367,8 @@ __device__ __forceinline__ Margin margin_of(const PrefArgs &a, const double (&su
 }
 
 // e^-x for x >= 0 and ln(1 + y) for y in [0, 1]: short chains, since few lanes wait for them.  Taylor's series of e^r,
-// |r| <= ln 2 / 2, to r^12 / 12!; ln(1 + y) = 2 artanh(y / (2 + y)), whose argument is at most 1/3, to its 19th power: 2e-16
-// and 1e-11 relative.
+// |r| <= ln 2 / 2, to r^12 / 12!, where r = -x - k ln 2 in two steps (Cody and Waite's reduction, with fdlibm's ln2HI and ln2LO);
+// ln(1 + y) = 2 artanh(y / (2 + y)), whose argument is at most 1/3, to its 19th power: 2e-16 and 1e-11 relative.
 __device__ __forceinline__ double exp_minus(double x)
 {
     if (x > 700.0) return 0.0;

@@ -92,3 +92,18 @@ def test_kl_coefficients_that_f32_does_not_hold_are_refused(kl_coef):
     buf = (ctypes.c_char * 4096)()
     p = (ctypes.addressof(buf) + 63) // 64 * 64
     assert _lib.load().ppo_policy_kl_loss(p, 4, p, 4, p, 4, 0, p, 4, p, 4, 2, 4, 0.2, 0.2, kl_coef, 3, 0, p, p, None, 0, None) == 1
+
+
+def test_preparing_more_than_2_36_elements_is_refused():
+    """u of 2^22 - 128 rows and 16500 outputs, and an input of as many odd columns: no launch holds their tiles of 64 x 64."""
+    lib = _lib.load()
+    buf = (ctypes.c_char * 4096)()
+    p = (ctypes.addressof(buf) + 63) // 64 * 64
+    rows, wide = (1 << 22) - 128, 16501
+    for outputs, inputs in ((wide, 8), (8, wide)):
+        n = max(lib.ppo_linear_act_fwd_workspace_bytes(rows, inputs, outputs, 1), lib.ppo_linear_act_bwd_workspace_bytes(rows, inputs, outputs, 1))
+        assert n > 1 << 36
+        if inputs == wide:
+            assert lib.ppo_linear_act_fwd(p, inputs, p, inputs, None, None, 0, 1, rows, inputs, outputs, 0, p, None, p, n, None) == 1
+        else:
+            assert lib.ppo_linear_act_bwd(p, outputs, p, inputs, p, inputs, p, 1, rows, inputs, outputs, p, p, p, p, n, None) == 1
