@@ -609,8 +609,8 @@ int ppo_preference_loss(const float *chosen, long chosen_stride, const float *re
  *   y [rows, outputs] contiguous; deriv the same or NULL: act'(z) for the backward call, f16 for PPO_DTYPE_BF16, f32 for
  *   the other types.
  * Sums are f32: 16-bit inputs on the 16-bit matrix cores; f32 inputs as three bf16 pieces each (PPO_NET_BF16X3), f32-grade
- * for magnitudes from 2^-110 on (below, the third piece and then the second underflow); infinite and NaN operands give what f32
- * arithmetic gives, at up to 2.2 times the cost of the products that they reach.
+ * for magnitudes from 2^-110 on (below, the third piece and then the second underflow); infinite and NaN operands and sums give
+ * what f32 arithmetic gives, at up to 2.2 times the cost of the products that they reach.
  * ppo_linear_act_bwd: with u = g_y * deriv (deriv NULL: u = g_y), rounded to `dtype`:
  *   g_x [rows, inputs] = u W, g_weight [outputs, inputs] = u^T x, g_bias [outputs] = column sums of the unrounded u; each
  *   contiguous, of `dtype`, or NULL.  The residual's gradient is g_y.

@@ -822,12 +822,13 @@ __global__ void __launch_bounds__(64 * WAVES_M * WAVES_N) k_gemm(GemmArgs g)
             step(s1 - 1, std::true_type{}, plain);
         };
         run(std::false_type{});
-        // An operand that is infinite, or above 3.38e38, where its first piece is, leaves NaN in every product that it is in.  Where a
-        // tile holds a NaN it is worked out again by the f32 matrix instructions (4096^3 with a NaN in every tile: 2.1 times as long), and what was
-        // NaN is replaced: such operands give what f32 arithmetic gives, as on the vector units, and the other results keep their
-        // bits.  (KEEP is a NaN itself: a result that has its bits is left as the NaN that it was.)
-        uint32_t nan[MI] = {}, found = 0;                   // bit 4 j + e of word i: acc[i][j][e]
-        float sum = 0.0f;                                   // NaN where one of them is, or infinite
+        // An operand that is infinite, or above 3.38e38, where its first piece is, leaves NaN in every product that it is in, and the first
+        // pieces of two large ones may have an infinite product where theirs is finite.  Where a tile holds a result that is not finite
+        // it is worked out again by the f32 matrix instructions (4096^3 with a NaN in every tile: 2.1 times as long), and what was not
+        // finite is replaced: such operands give what f32 arithmetic gives, as on the vector units, and the other results keep their
+        // bits.  (KEEP is a NaN itself, which no product makes and an operand can only pass on: then the result was NaN and stays.)
+        uint32_t wild[MI] = {}, found = 0;                  // bit 4 j + e of word i: acc[i][j][e] is not finite
+        float sum = 0.0f;                                   // NaN where one is not
 #pragma unroll
         for (int i = 0; i < MI; ++i)
 #pragma unroll
@@ -840,8 +841,8 @@ __global__ void __launch_bounds__(64 * WAVES_M * WAVES_N) k_gemm(GemmArgs g)
 #pragma unroll
                 for (int j = 0; j < NI; ++j)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) nan[i] |= (acc[i][j][e] != acc[i][j][e] ? 1u : 0u) << (4 * j + e);
-                found |= nan[i];
+                    for (int e = 0; e < 4; ++e) wild[i] |= (fabsf(acc[i][j][e]) < INFINITY ? 0u : 1u) << (4 * j + e);
+                found |= wild[i];
             }
         }
         leave(std::false_type{}, [&](int i, int j) { return acc[i][j]; });
@@ -864,7 +865,7 @@ __global__ void __launch_bounds__(64 * WAVES_M * WAVES_N) k_gemm(GemmArgs g)
             leave(std::true_type{}, [&](int i, int j) {
                 f32x4 v;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = nan[i] >> (4 * j + e) & 1 ? acc[i][j][e] : __builtin_bit_cast(float, KEEP);
+                for (int e = 0; e < 4; ++e) v[e] = wild[i] >> (4 * j + e) & 1 ? acc[i][j][e] : __builtin_bit_cast(float, KEEP);
                 return v;
             });
         }

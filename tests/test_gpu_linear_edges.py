@@ -179,3 +179,19 @@ def test_nothing_beside_the_outputs_is_written(M, K, N, dtype):
     guard.check()
     for got, q in zip((gx, gw, gb), ops.linear_act_bwd(g, x, w, dwant)):
         assert torch.equal(got.clone().view(dtype).view(q.shape), q)
+
+
+@pytest.mark.parametrize("M,K,N", [(3, 2, 40), (300, 2, 301), (40, 8000, 300), (60, 4000, 50)])
+def test_f32_products_below_the_largest_value(M, K, N):
+    """1.9901 2^127 times 1.0041 is finite (1.9983 2^127) although the product of their first bf16 pieces is not; twice that is infinite."""
+    from ppo_amd import ops
+    x, w = torch.zeros(M, K, device="cuda"), torch.zeros(N, K, device="cuda")
+    x[:, 1], w[:, 1] = 1.9901 * 2.0 ** 127, 1.0041
+    w[1::2, 1] *= -1.0
+    w[2] *= 2.0
+    x[1, 0], w[:, 0] = 1.0, torch.arange(N, device="cuda").float()
+    want = x.double() @ w.double().t()
+    got = ops.linear_act_fwd(x, w)[0]
+    assert torch.equal(torch.isinf(got), torch.isinf(want.float())) and bool(torch.isinf(got[:, 2]).all())
+    fin = torch.isfinite(want.float())
+    assert bool(((got.double() - want).abs()[fin] <= 4 * E * want.abs()[fin]).all())
